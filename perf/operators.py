@@ -126,6 +126,7 @@ def prepare(case, seed):
             st["op"] = dense_ops.DeltaRule(H, G, d, dv, dt, q_scale=st["q_scale"], eps=st["eps"], taps=c["taps"], conv=st["conv"],
                                            conv_b=st["conv_b"], dt_bias=st["dt_bias"], A=st["A"])
             st["len"] = torch.full((1,), st["pos"], dtype=torch.int32, device="cuda")
+            st["ticket"] = torch.zeros(1, dtype=torch.int32, device="cuda")
             st["o"] = torch.empty(H, dv, device="cuda")
         return st
     lengths = [int(x) for x in c["lengths"].split(",")]
@@ -314,7 +315,7 @@ def run(st):
     H, dv = c["heads"], c["vdim"]
     if kind == "step":
         op.step(st["row"].data_ptr(), st["dt"].data_ptr(), st["beta"].data_ptr(), st["ring"].data_ptr(), st["S"][0].data_ptr(),
-                st["o"].data_ptr(), st["len"].data_ptr())
+                st["o"].data_ptr(), st["len"].data_ptr(), st["ticket"].data_ptr())
         return st["o"], st["S"][0], st["ring"]
     rows = st["rows"]
     T, C = rows.shape
