@@ -218,6 +218,75 @@ int lt_dn_gqa_step_tickets(int H, int G);
 int lt_dn_gqa_step(const void* y, void* kc, void* vc, void* vfirst, int vmix_store, const float* gate, void* out, int f32, int* len,
                    const lt_dn_gqa* h_a, int splits, float* ws, int* tickets, void* stream);
 
+/* Gated delta rule.  Per head, with k and q of its group (H a multiple of G) brought to unit length,
+ *   k <- k / sqrt(sum k^2 + eps),  q <- q_scale * q / sqrt(sum q^2 + eps):
+ *   S <- e^la_t S,  u = beta_t (v_t - S k_t),  S <- S + u k_t^T,  o_t = S q_t      (S fp32, stored [H][dvp][dp])
+ * la (logarithms of the decays, <= 0 in a decaying memory; minus infinity forgets) and beta are fp32 [row][ldh]. */
+typedef struct {
+    int H, G, dp, dvp;       /* heads, key heads, padded key and value sizes */
+    float q_scale, eps;      /* eps > 0 */
+    int taps;                /* what follows: lt_dn_delta_step alone */
+    const float* conv;       /* [taps][C], C = H*dvp + 2*G*dp; the last tap is the current token's */
+    const float* conv_b;     /* [C] */
+    const float* dt_bias;    /* [H] */
+    const float* A;          /* [H]: log decay per unit of step size (negative) */
+} lt_dn_delta;
+
+/* Sequences of a pass: rows start .. start + rows - 1 belong to the state S (rows 0: the state stays as it is).  Rows of no
+ * sequence are neither read nor written; two sequences share neither rows nor a state. */
+#define LT_DN_SEQS 8
+typedef struct {
+    int n;
+    int start[LT_DN_SEQS], rows[LT_DN_SEQS];
+    float* S[LT_DN_SEQS];
+} lt_dn_seqs;
+
+/* Rows of up to LT_DN_SEQS sequences, in token order.  q, k: element type, key head g at columns g*dp; v: head h at h*dvp; row
+ * stride ld for all three.  o: fp32, row stride ldo. */
+int lt_dn_delta_rows(const void* q, const void* k, const void* v, int ld, const float* la, const float* beta, int ldh, float* o, int ldo,
+                     int f32, const lt_dn_delta* h_d, const lt_dn_seqs* h_q, void* stream);
+
+/* One token at position *len (then *len += 1): convolution, silu, step size la = A softplus(dt + dt_bias) and recurrence in one
+ * launch.  vkq: one row, values (H*dvp), keys (G*dp), queries (G*dp), ahead of the convolution, whose last inputs are in the ring
+ * as in lt_dn_ssd_rows.  dt, beta [H]; o [H*dvp] fp32.  ticket: one int of the sequence, zero between launches. */
+int lt_dn_delta_step(const void* vkq, const float* dt, const float* beta, void* ring, float* S, float* o, int f32, int* len, int* ticket,
+                     const lt_dn_delta* h_d, void* stream);
+
+/* Routing: row t of logits chooses `top` of n experts (n <= 1024, top <= 32).  s = softmax(l) or sigmoid(l); the choice goes by
+ * s + bias, inside the top_groups groups (n / groups consecutive experts each, at most 32 groups) whose two best values have the
+ * largest sum; equal values: the lowest index.  ids [T][top] in descending order of choice; w = s (/ the sum of the chosen s, with
+ * renorm; 0 if that is 0) * scale.  A logit of minus infinity or NaN: the expert has score 0 and is behind all others of the kept groups. */
+#define LT_DN_SCORE_SOFTMAX 0
+#define LT_DN_SCORE_SIGMOID 1
+typedef struct {
+    int n, top, score, groups, top_groups, renorm;
+    float scale;
+    const float* bias;       /* [n] or NULL */
+} lt_dn_router;
+int lt_dn_route(const float* logits, int ld, int* ids, float* w, int T, const lt_dn_router* h_r, void* stream);
+
+/* Experts of T tokens: place (t, j) is expert ids[t*top + j] of n.  An id below zero leaves its place out; one of n or more does
+ * too and sets LT_STATUS_BAD_TOKEN.  plan: NULL, or what lt_dn_experts_plan made of the same ids: the first place of every expert
+ * [n + 1], then the places in order of expert, each expert's ascending. */
+typedef struct {
+    const int* ids;
+    const int* plan;
+    int T, top, n;
+} lt_dn_choice;
+long lt_dn_experts_plan_ints(int T, int top, int n);
+int lt_dn_experts_plan(const int* ids, int T, int top, int n, int* plan, void* stream);
+
+/* H[t*top + j] = glu(gate, up) of x_t and the expert's matrix: W [n][2F][ldw], F gate rows, then F up rows.  h_epi: LT_DN_GLU.
+ * Rows of H whose place is left out stay as they are. */
+int lt_dn_experts_glu(const void* W, int ldw, const void* X, int ldx, void* H, int ldh, int f32, int F, int K, const lt_dn_choice* h_c,
+                      const lt_dn_epilogue* h_epi, void* stream);
+
+/* Y[t] (fp32) += ls * sum_j w[t*top + j] * (W of the expert) H[t*top + j]; W [n][M][ldw]; ls [M] or NULL (1).  With a plan ws holds
+ * lt_dn_experts_sum_ws(T, top, M) fp32 elements. */
+long lt_dn_experts_sum_ws(int T, int top, int M);
+int lt_dn_experts_sum(const void* W, int ldw, const void* H, int ldh, float* Y, int ldy, int f32, int M, int K, const lt_dn_choice* h_c,
+                      const float* w, const float* ls, float* ws, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -136,6 +136,27 @@ class DnGqa(ctypes.Structure):
                [(n, _f) for n in ("scale", "softcap", "eps", "vmix")] + [(n, _vp) for n in ("freq", "qnorm", "knorm")]
 
 
+DN_SEQS = 8
+DN_SCORE = {"softmax": 0, "sigmoid": 1}
+
+
+class DnDelta(ctypes.Structure):
+    _fields_ = [(n, _i) for n in ("H", "G", "dp", "dvp")] + [("q_scale", _f), ("eps", _f), ("taps", _i)] + \
+               [(n, _vp) for n in ("conv", "conv_b", "dt_bias", "A")]
+
+
+class DnSeqs(ctypes.Structure):
+    _fields_ = [("n", _i), ("start", _i * DN_SEQS), ("rows", _i * DN_SEQS), ("S", _vp * DN_SEQS)]
+
+
+class DnRouter(ctypes.Structure):
+    _fields_ = [(n, _i) for n in ("n", "top", "score", "groups", "top_groups", "renorm")] + [("scale", _f), ("bias", _vp)]
+
+
+class DnChoice(ctypes.Structure):
+    _fields_ = [("ids", _vp), ("plan", _vp), ("T", _i), ("top", _i), ("n", _i)]
+
+
 DENSE_SIGNATURES = {
     "lt_dn_embed": [_vp, _i, _i, _vp, _f, _vp, _f, _vp, _vp, _i, _i, _i, _i, _vp],
     "lt_dn_norm_rows": [_vp, _i, _vp, _vp, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _f, _i, _i, _i, _vp],
@@ -151,11 +172,19 @@ DENSE_SIGNATURES = {
     "lt_dn_ssd_step": [_vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, ctypes.POINTER(DnSsd), _vp],
     "lt_dn_gqa_rows": [_vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, ctypes.POINTER(DnGqa), _vp],
     "lt_dn_gqa_attn": [_vp, _i, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, ctypes.POINTER(DnGqa), _vp],
+    "lt_dn_delta_rows": [_vp, _vp, _vp, _i, _vp, _vp, _i, _vp, _i, _i, ctypes.POINTER(DnDelta), ctypes.POINTER(DnSeqs), _vp],
+    "lt_dn_delta_step": [_vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, ctypes.POINTER(DnDelta), _vp],
+    "lt_dn_route": [_vp, _i, _vp, _vp, _i, ctypes.POINTER(DnRouter), _vp],
+    "lt_dn_experts_plan": [_vp, _i, _i, _i, _vp, _vp],
+    "lt_dn_experts_glu": [_vp, _i, _vp, _i, _vp, _i, _i, _i, _i, ctypes.POINTER(DnChoice), ctypes.POINTER(DnEpilogue), _vp],
+    "lt_dn_experts_sum": [_vp, _i, _vp, _i, _vp, _i, _i, _i, _i, ctypes.POINTER(DnChoice), _vp, _vp, _vp, _vp],
     "lt_dn_gqa_step": [_vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _vp, ctypes.POINTER(DnGqa), _i, _vp, _vp, _vp],
 }
 _DENSE_QUERIES = {"lt_dn_gqa_step_ws": ([_i, _i, _i], ctypes.c_long),
                   "lt_dn_gqa_step_tickets": ([_i, _i], _i),
                   "lt_dn_latent_step_ws": ([_i, _i, _i, _i], ctypes.c_long),
+                  "lt_dn_experts_plan_ints": ([_i, _i, _i], ctypes.c_long),
+                  "lt_dn_experts_sum_ws": ([_i, _i, _i], ctypes.c_long),
                   "lt_dn_recurrence_chunked_ws": ([_i, _i, _i, _i], ctypes.c_long)}
 # what the common library exports (the Q8_0 library passes these through to its users as well)
 _COMMON_NAMES = ("lt_last_error", "lt_version", "lt_launch_count", "lt_set_chained_launch", "lt_device_status",

@@ -118,3 +118,114 @@ def typed_input(x):
 
 def cast_input(x, n1, x2=None):
     return _lib.DnPrologue(_lib.DN_IN_CAST, n1, 0, 0, 0.0, x, x2, None, 0, None, 0, 0, 0)
+
+
+# --------------------------------------------------------------------------- sparse feed-forwards
+
+def _here(t, what):
+    """Launches go to the current device: an operand of another one is refused."""
+    if t.device.type != "cuda" or t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{what} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+    return t
+
+
+class Router:
+    """Choice of `top` of n experts for rows of fp32 scores, and the weights of the chosen (lt_dn_route)."""
+
+    def __init__(self, n, top, score="softmax", bias=None, groups=1, top_groups=1, renorm=True, scale=1.0):
+        if score not in _lib.DN_SCORE:
+            raise ValueError(f"score {score!r}: known are {', '.join(sorted(_lib.DN_SCORE))}")
+        if not (1 <= top <= 32 and 1 <= n <= 1024 and 1 <= groups <= 32 and n % groups == 0 and 1 <= top_groups <= groups
+                and top <= n // groups * top_groups):
+            raise ValueError(f"top {top} of {n} experts in {top_groups} of {groups} groups")
+        if bias is not None and tuple(bias.shape) != (n,):
+            raise ValueError(f"bias {tuple(bias.shape)} for {n} experts")
+        self.n, self.top = n, top
+        self.bias = None if bias is None else bias.float().cuda().contiguous()
+        self.desc = _lib.DnRouter(n, top, _lib.DN_SCORE[score], groups, top_groups, int(renorm), float(scale),
+                                  None if bias is None else self.bias.data_ptr())
+        self._ref = ctypes.byref(self.desc)
+
+    def rows(self, logits, ld, ids, w, T):
+        """ids int32 [T][top] and w fp32 [T][top] of T rows of logits."""
+        _lib.call("lt_dn_route", logits, ld, ids, w, T, self._ref, dr._stream())
+
+
+class Places:
+    """Chosen experts of T tokens (ids int32 [T, top]) and, with `plan`, the order of the places by expert."""
+
+    def __init__(self, ids, n, plan=None):
+        self.ids, self.buf = ids, plan
+        self.T, self.top = ids.shape
+        self.desc = _lib.DnChoice(ids.data_ptr(), None if plan is None else plan.data_ptr(), self.T, self.top, n)
+        self.ref = ctypes.byref(self.desc)
+
+
+class Experts:
+    """A matrix per expert, [n, rows, columns].  gated: rows are gate rows and as many up rows, and `hidden` stores their gated
+    product; else `add_sum` adds the weighted sum of the chosen experts' outputs to fp32 rows.  glu: as in `epilogue`."""
+
+    def __init__(self, W, gated, glu=(_lib.DN_GLU_GELU, 0.0, 0.0)):
+        if W.dim() != 3 or W.dtype not in DTYPES.values():
+            raise ValueError(f"matrices {tuple(W.shape)} of {W.dtype}")
+        n, M, K = W.shape
+        if gated and M % 2:
+            raise ValueError(f"{M} gate and up rows")
+        if K % 8:
+            W = torch.cat([W, W.new_zeros(n, M, pad8(K) - K)], dim=2)
+        self.W = W.cuda().contiguous()
+        self.n, self.M, self.K = n, M // 2 if gated else M, pad8(K)
+        self.gated, self.f32 = gated, int(W.dtype == torch.float32)
+        self.ptr = self.W.data_ptr()
+        self.epi = epilogue(_lib.DN_GLU, glu=glu) if gated else None
+
+    def plan(self, ids, T):
+        """The places of T tokens, ids int32 [T, top]."""
+        if ids.dtype != torch.int32 or ids.dim() != 2 or ids.shape[0] != T or not ids.is_contiguous():
+            raise ValueError(f"ids must be contiguous int32 [{T}, top], got {ids.dtype} {tuple(ids.shape)}")
+        _here(ids, "ids")
+        _here(self.W, "the experts' matrix")
+        return Places(ids, self.n)
+
+    def hidden(self, x, ldx, places, h, ldh):
+        """h[t*top + j] = glu of the gate and up rows of place (t, j)'s expert, for the rows of x."""
+        _lib.call("lt_dn_experts_glu", self.ptr, self.K, x, ldx, h, ldh, self.f32, self.M, self.K, places.ref, ctypes.byref(self.epi),
+                  dr._stream())
+
+    def add_sum(self, h, ldh, places, w, y, ldy, ls=None):
+        """y[t] += ls * sum over j of w[t][j] W h[t*top + j]."""
+        ws = None
+        _lib.call("lt_dn_experts_sum", self.ptr, self.K, h, ldh, y, ldy, self.f32, self.M, self.K, places.ref, w, ls, ws, dr._stream())
+
+
+# --------------------------------------------------------------------------- delta rule
+
+class DeltaRule:
+    """Gated delta rule of H heads on G key heads: rows() over the rows of sequences, step() for one token with its convolution
+    (taps, conv, conv_b, dt_bias and A as in lt_dn_delta, on the device).  dim and vdim are the padded sizes."""
+
+    def __init__(self, H, G, dim, vdim, dtype, q_scale, eps, taps=0, conv=None, conv_b=None, dt_bias=None, A=None):
+        if H % G or dim % 8 or vdim % 8:
+            raise ValueError(f"{H} heads on {G} key heads, sizes {dim} and {vdim} (multiples of 8)")
+        self.H, self.G, self.dim, self.vdim = H, G, dim, vdim
+        self.f32 = int(dtype == torch.float32)
+        self.keep = [None if t is None else t.float().contiguous() for t in (conv, conv_b, dt_bias, A)]
+        self.desc = _lib.DnDelta(H, G, dim, vdim, float(q_scale), float(eps), taps, *[None if t is None else _here(t, "a constant").data_ptr()
+                                                                                   for t in self.keep])
+        self._ref = ctypes.byref(self.desc)
+
+    def rows(self, q, k, v, ld, la, beta, ldh, o, ldo, states, rows):
+        """Consecutive rows of sequences: rows[i] of them with the state at states[i], from row 0 on."""
+        if len(states) != len(rows):
+            raise ValueError(f"{len(states)} states for {len(rows)} sequences")
+        at = 0
+        for i in range(0, len(rows), _lib.DN_SEQS):
+            part = rows[i:i + _lib.DN_SEQS]
+            seqs = _lib.DnSeqs(n=len(part))
+            for j, r in enumerate(part):
+                seqs.start[j], seqs.rows[j], seqs.S[j] = at, r, states[i + j]
+                at += r
+            _lib.call("lt_dn_delta_rows", q, k, v, ld, la, beta, ldh, o, ldo, self.f32, self._ref, ctypes.byref(seqs), dr._stream())
+
+    def step(self, row, dt, beta, ring, S, o, len_, ticket):
+        _lib.call("lt_dn_delta_step", row, dt, beta, ring, S, o, self.f32, len_, ticket, self._ref, dr._stream())

@@ -1,0 +1,415 @@
+"""GPU: routing, the experts' products and the delta rule, each alone against plain 64-bit arithmetic, at sizes and masks where it
+can go wrong.
+
+Tolerances.  fp32 sums of n products of unit variance are off by at most n 2^-24 of their absolute values and by about sqrt(n) 2^-24
+as a rule; tests allow 8 sqrt(n) 2^-24 of the outputs' size, and half a step (2^-9 of the power of two below, so 2^-8 of the value at
+most) for a result that is rounded to bf16."""
+import numpy as np
+import pytest
+import torch
+
+from llamatov_b200 import _lib, dense_ops as P
+from oracle import layered as L
+from tests.gpu_util import stream
+
+pytestmark = pytest.mark.gpu
+DT = {0: torch.bfloat16, 1: torch.float32}
+E32 = 2.0 ** -24
+
+
+@pytest.fixture(autouse=True)
+def _clean_status():
+    yield
+    torch.cuda.synchronize()
+    assert _lib.device_status() == set()
+
+
+def _np(t):
+    return t.detach().double().cpu().numpy()
+
+
+def _randn(shape, seed, dtype=torch.float32, scale=1.0):
+    return (torch.randn(*shape, generator=torch.Generator().manual_seed(seed)) * scale).to(dtype).cuda()
+
+
+def _off(got, want, size=None):
+    """Largest difference over the size (the largest) of the wanted values."""
+    got, want = np.asarray(got, np.float64), np.asarray(want, np.float64)
+    assert np.isfinite(got).all()
+    size = np.abs(want).max() if size is None else size
+    return float(np.abs(got - want).max() / size if size else np.abs(got).max())
+
+
+# --------------------------------------------------------------------------- routing
+
+def route64(l, top, score, bias, groups, top_groups, renorm, scale):
+    """Row by row, from the definition."""
+    T, n = l.shape
+    ids, w = np.zeros((T, top), np.int64), np.zeros((T, top))
+    for t in range(T):
+        x = np.where(np.isnan(l[t]), -np.inf, l[t])
+        gone = x == -np.inf
+        with np.errstate(invalid="ignore"):
+            if score == "softmax":
+                s = np.zeros(n) if gone.all() else np.exp(x - x.max())
+                s = s / s.sum() if s.sum() > 0 else s
+            else:
+                s = 1 / (1 + np.exp(-x))
+        s[gone] = 0
+        c = s + (bias if bias is not None else 0)
+        c[gone] = -np.inf
+        size = n // groups
+        best = [np.sort(c[g * size:(g + 1) * size])[::-1][:2].sum() for g in range(groups)]
+        kept = sorted(range(groups), key=lambda g: (-best[g], g))[:top_groups]
+        order = sorted((e for g in kept for e in range(g * size, (g + 1) * size)), key=lambda e: (-c[e], e))[:top]
+        ids[t], w[t] = order, s[order]
+        if renorm:
+            w[t] = w[t] / w[t].sum() if w[t].sum() > 0 else 0
+    return ids, w * scale
+
+
+def _route(l, n, top, ld=None, bias=None, **kw):
+    T = l.shape[0]
+    ids = torch.full((T + 1, top), -7, dtype=torch.int32, device="cuda")
+    w = torch.full((T + 1, top), -7.0, device="cuda")
+    P.Router(n, top, bias=bias, **kw).rows(l.data_ptr(), l.shape[1], ids.data_ptr(), w.data_ptr(), T)
+    assert (ids[T:] == -7).all() and (w[T:] == -7).all()
+    return ids[:T].cpu().numpy(), _np(w[:T])
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("T,n,top,groups,top_groups,biased", [
+    (1, 1, 1, 1, 1, False), (1, 64, 6, 1, 1, False), (5, 33, 32, 1, 1, True), (257, 64, 8, 8, 3, True), (31, 96, 4, 32, 5, False),
+    (64, 256, 8, 8, 4, True), (3, 300, 10, 4, 4, True), (9, 1024, 32, 16, 2, True), (7, 512, 1, 2, 1, False), (130, 12, 3, 12, 3, True)])
+def test_route(score, T, n, top, groups, top_groups, biased):
+    l = _randn((T, n + 3), T + n, scale=2.0)
+    bias = _randn((n,), 5, scale=0.2) if biased else None
+    ids, w = _route(l, n, top, bias=bias, score=score, groups=groups, top_groups=top_groups, scale=2.5)
+    want, ww = route64(_np(l)[:, :n], top, score, None if bias is None else _np(bias), groups, top_groups, True, 2.5)
+    assert np.array_equal(ids, want)
+    assert np.allclose(w, ww, rtol=2 * E32, atol=0)        # one rounding of a 64-bit value
+    ids2, w2 = _route(l, n, top, bias=bias, score=score, groups=groups, top_groups=top_groups, renorm=False)
+    assert np.array_equal(ids2, want)
+    assert np.allclose(w2, route64(_np(l)[:, :n], top, score, None if bias is None else _np(bias), groups, top_groups, False, 1.0)[1],
+                       rtol=2 * E32, atol=0)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_route_ties_and_masks(score):
+    n, inf = 16, float("inf")
+    rows = [[0.0] * n, [1.0, 2.0] * 8, [-inf] * n, [-inf] * 15 + [3.0], [float("nan")] * 8 + [0.5] * 8, [5.0] + [-inf] * 14 + [float("nan")],
+            [inf] + [0.0] * 15, [3.4e38] * n, [-3.4e38] * n, [-800.0] * 8 + [0.0] * 8, [88.0, -88.0] * 8]
+    l = torch.tensor(rows).cuda()
+    x = _np(torch.tensor(rows).clamp(max=3.402823466e38))
+    for groups, top_groups, top in ((1, 1, 5), (4, 2, 6), (4, 4, 16), (16, 3, 3)):
+        for bias in (None, -_randn((n,), 3).abs()):
+            ids, w = _route(l, n, top, score=score, bias=bias, groups=groups, top_groups=top_groups)
+            want, ww = route64(x, top, score, None if bias is None else _np(bias), groups, top_groups, True, 1.0)
+            assert np.array_equal(ids, want), (groups, bias)
+            assert np.allclose(w, ww, rtol=2 * E32, atol=1e-38)
+    assert (w[2] == 0).all()
+
+
+def test_route_decides_near_ties_in_64_bits():
+    """Scores whose sums with the bias differ by far less than 2^-24."""
+    n = 64
+    l = torch.full((40, n), 0.25)
+    l[torch.arange(40), torch.arange(40)] += 2.0 ** -24                # two steps up from 0.25
+    ids, _ = _route(l.cuda(), n, 2, score="sigmoid", bias=torch.full((n,), 1000.0).cuda())
+    assert np.array_equal(ids[:, 0], np.arange(40)) and np.array_equal(ids[:, 1], np.where(np.arange(40) == 0, 1, 0))
+
+
+# --------------------------------------------------------------------------- experts
+
+def _gelu(z):
+    return L.gelu_tanh(z)
+
+
+def _clamped(limit):
+    return lambda g, u: np.minimum(g, limit) * L.sigmoid(1.702 * np.minimum(g, limit)) * (np.clip(u, -limit, limit) + 1)
+
+
+GLU = {"gelu": ((0, 0.0, 0.0), lambda g, u: _gelu(g) * u), "clamped": ((1, 1.702, 1.2), _clamped(1.2))}
+
+
+def _ids(T, top, n, seed, how="spread"):
+    g = torch.Generator().manual_seed(seed)
+    if how == "one":                                   # everything to one expert (and its neighbours)
+        return (torch.arange(top).repeat(T, 1) + n // 2).remainder(n).int()
+    if how == "same":                                  # the same expert twice
+        return torch.randint(0, n, (T, 1), generator=g).expand(T, top).contiguous().int()
+    return torch.rand(T, n, generator=g).argsort(dim=1)[:, :top].contiguous().int()
+
+
+SIZES = [  # T, top, n, K, F or M
+    (1, 1, 1, 8, 1), (1, 2, 4, 24, 9), (1, 8, 64, 264, 136), (2, 3, 5, 40, 130), (17, 2, 3, 72, 33), (37, 4, 16, 896, 616), (64, 4, 8, 64, 128),
+    (65, 1, 2, 128, 256), (200, 8, 16, 136, 264), (33, 32, 40, 16, 24), (300, 2, 70, 520, 136)]
+
+
+def _check_glu(T, top, n, K, F, f32, how="spread", act="gelu", seed=1, ids=None, form=None):
+    W, X = _randn((n, 2 * F, K), seed, DT[f32], 1.5 * K ** -0.5), _randn((T, K + 8), seed + 1, DT[f32])
+    ids = _ids(T, top, n, seed + 2, how) if ids is None else ids
+    dids = ids.cuda()
+    op = P.Experts(W, gated=True, glu=GLU[act][0])
+    H = torch.full((T * top + 2, F + 3), 7.0, dtype=DT[f32], device="cuda")
+    op.hidden(X.data_ptr(), K + 8, op.plan(dids, T), H.data_ptr(), F + 3)
+    x, w = _np(X)[:, :K], _np(W)
+    got = _np(H)
+    assert (got[T * top:] == 7).all() and (got[:, F:] == 7).all()
+    for t in range(T):
+        for j in range(top):
+            e, row = int(ids[t, j]), got[t * top + j, :F]
+            if not 0 <= e < n:
+                assert (row == 7).all()
+                continue
+            v = w[e] @ x[t]
+            want = GLU[act][1](v[:F], v[F:])
+            # |d glu| <= |u| |d gelu| + |gelu| |du| with products of size about 1.5: sums of K products off by 8 sqrt(K) 2^-24
+            tol = (8 * K ** 0.5 + 16) * E32 * (1 + np.abs(v[:F])) * (1 + np.abs(v[F:])) * 3
+            assert (np.abs(row - want) <= tol + (0 if f32 else 2.0 ** -8 * np.abs(want))).all(), (t, j, np.abs(row - want).max())
+
+
+@pytest.mark.parametrize("f32", [0, 1])
+@pytest.mark.parametrize("T,top,n,K,F", SIZES)
+def test_experts_glu(f32, T, top, n, K, F):
+    _check_glu(T, top, n, K, F, f32)
+
+
+@pytest.mark.parametrize("f32", [0, 1])
+@pytest.mark.parametrize("how", ["one", "same"])
+def test_experts_glu_crowded(f32, how):
+    _check_glu(150, 3, 9, 72, 136, f32, how, "clamped")
+    _check_glu(3, 3, 9, 72, 136, f32, how, "clamped")
+
+
+def _check_sum(T, top, n, K, M, f32, how="spread", ls=True, seed=11, ids=None):
+    W, H = _randn((n, M, K), seed, DT[f32], K ** -0.5), _randn((T * top, K + 8), seed + 1, DT[f32])
+    ids = _ids(T, top, n, seed + 2, how) if ids is None else ids
+    w = torch.rand(T, top, generator=torch.Generator().manual_seed(seed)).cuda()
+    s = _randn((M,), seed + 3) if ls else None
+    Y0 = _randn((T + 1, M + 5), seed + 4)
+    Y = Y0.clone()
+    op = P.Experts(W, gated=False)
+    op.add_sum(H.data_ptr(), K + 8, op.plan(ids.cuda(), T), w.data_ptr(), Y.data_ptr(), M + 5, ls=None if s is None else s.data_ptr())
+    assert torch.equal(Y[T:], Y0[T:]) and torch.equal(Y[:, M:], Y0[:, M:])
+    h, Wn, wn = _np(H)[:, :K].reshape(T, top, K), _np(W), _np(w)
+    want, size = _np(Y0)[:T, :M].copy(), np.abs(_np(Y0)[:T, :M])
+    for t in range(T):
+        for j in range(top):
+            e = int(ids[t, j])
+            if 0 <= e < n:
+                v = wn[t, j] * (Wn[e] @ h[t, j]) * (_np(s) if ls else 1)
+                want[t] += v
+                size[t] += wn[t, j] * (np.abs(Wn[e]) @ np.abs(h[t, j])) * (np.abs(_np(s)) if ls else 1)
+    # a sum of K + top + 2 terms, each partial sum at most the sum of absolute values: n 2^-24 of it in the worst case
+    assert (np.abs(_np(Y)[:T, :M] - want) <= (8 * K ** 0.5 + top + 2) * E32 * size).all()
+
+
+@pytest.mark.parametrize("f32", [0, 1])
+@pytest.mark.parametrize("T,top,n,K,M", SIZES)
+def test_experts_sum(f32, T, top, n, K, M):
+    _check_sum(T, top, n, K, M, f32)
+
+
+@pytest.mark.parametrize("f32", [0, 1])
+@pytest.mark.parametrize("how", ["one", "same"])
+def test_experts_sum_crowded(f32, how):
+    _check_sum(150, 3, 9, 72, 136, f32, how, ls=False)
+    _check_sum(3, 3, 9, 72, 136, f32, how, ls=False)
+
+
+@pytest.mark.parametrize("f32", [0, 1])
+@pytest.mark.parametrize("T", [2, 90])
+def test_experts_places_left_out(f32, T):
+    """Ids below zero leave a place out; a token all of whose places are left out keeps its row."""
+    ids = _ids(T, 4, 8, 3)
+    ids[0] = -1
+    ids[1, 2] = -5
+    ids[T // 2, 0] = -1
+    _check_glu(T, 4, 8, 72, 40, f32, ids=ids)
+    _check_sum(T, 4, 8, 72, 40, f32, ids=ids)
+    _check_glu(T, 4, 8, 72, 40, f32, ids=torch.full_like(ids, -1))
+    _check_sum(T, 4, 8, 72, 40, f32, ids=torch.full_like(ids, -1))
+
+
+@pytest.mark.parametrize("T", [2, 90])
+def test_experts_ids_out_of_range_are_reported(T):
+    ids = _ids(T, 4, 8, 3)
+    ids[1, 1] = 8
+    ids[T - 1, 3] = 2 ** 31 - 1
+    _check_glu(T, 4, 8, 72, 40, 0, ids=ids)
+    torch.cuda.synchronize()
+    assert _lib.device_status() == {"bad_token"}
+    _check_sum(T, 4, 8, 72, 40, 0, ids=ids)
+    torch.cuda.synchronize()
+    assert _lib.device_status() == {"bad_token"}
+
+
+@pytest.mark.parametrize("T,top,n", [(1, 1, 1), (1, 8, 64), (100, 3, 7), (2048, 8, 256), (513, 2, 1024)])
+def test_plan(T, top, n):
+    ids = _ids(T, min(top, n), n, 7)
+    ids.reshape(-1)[::11] = -1
+    d = ids.cuda()
+    plan = torch.full((_lib.dense().lt_dn_experts_plan_ints(T, ids.shape[1], n) + 1,), -9, dtype=torch.int32, device="cuda")
+    _lib.call("lt_dn_experts_plan", d.data_ptr(), T, ids.shape[1], n, plan.data_ptr(), stream())
+    flat, got = ids.reshape(-1).numpy(), plan.cpu().numpy()
+    used = np.flatnonzero(flat >= 0)
+    order = used[np.argsort(flat[used], kind="stable")]
+    assert np.array_equal(got[:n + 1], np.searchsorted(np.sort(flat[used]), np.arange(n + 1)))
+    assert np.array_equal(got[n + 1:n + 1 + len(order)], order)
+    assert (got[n + 1 + len(order):] == -9).all()
+
+
+# --------------------------------------------------------------------------- delta rule
+
+def delta64(q, k, v, la, beta, S, q_scale, eps):
+    """q, k [T, G, d], v [T, H, dv], S [H, dv, d] (a copy is advanced)."""
+    T, H = v.shape[:2]
+    per = H // q.shape[1]
+    q, k = np.repeat(q, per, axis=1), np.repeat(k, per, axis=1)
+    q = q_scale * q / np.sqrt((q ** 2).sum(-1, keepdims=True) + eps)
+    k = k / np.sqrt((k ** 2).sum(-1, keepdims=True) + eps)
+    S, o = S.copy(), np.zeros(v.shape)
+    for t in range(T):
+        S *= np.exp(la[t])[:, None, None]
+        u = beta[t][:, None] * (v[t] - np.einsum("hvd,hd->hv", S, k[t]))
+        S += u[:, :, None] * k[t][:, None, :]
+        o[t] = np.einsum("hvd,hd->hv", S, q[t])
+    return o, S
+
+
+def _delta_case(lengths, H, G, d, dv, f32, seed=0, gap=0, strong=False, la=None, beta=None):
+    """Rows [v | k | q | unused] of the sequences with `gap` rows between them."""
+    g = torch.Generator().manual_seed(seed)
+    C = H * dv + 2 * G * d
+    R = sum(lengths) + gap * len(lengths)
+    rows = torch.randn(R, C + 8, generator=g).to(DT[f32]).cuda()
+    if la is None:
+        la = -torch.rand(R, H, generator=g) * (30.0 if strong else 0.3)
+    if beta is None:
+        beta = torch.rand(R, H, generator=g)
+    S = [torch.randn(H, dv, d, generator=g).cuda() for _ in lengths]
+    return rows, la.float().cuda(), beta.float().cuda(), S
+
+
+def _delta_run(rows, la, beta, S, lengths, H, G, d, dv, f32, gap=0, q_scale=0.25, eps=1e-6, call=None):
+    """The rows through lt_dn_delta_rows, against 64 bits: largest error of o and of the states, over their size."""
+    R, ld = rows.shape
+    es = rows.element_size()
+    o = torch.full((R, H * dv + 2), 7.0, device="cuda")
+    op = P.DeltaRule(H, G, d, dv, DT[f32], q_scale, eps)
+    v = rows.data_ptr()
+    k = v + H * dv * es
+    before = [s.clone() for s in S]
+    if gap == 0:
+        op.rows(k + G * d * es, k, v, ld, la.data_ptr(), beta.data_ptr(), H, o.data_ptr(), H * dv + 2, [s.data_ptr() for s in S], lengths)
+    else:
+        seqs = _lib.DnSeqs(n=len(lengths))
+        at = 0
+        for i, n in enumerate(lengths):
+            at += gap
+            seqs.start[i], seqs.rows[i], seqs.S[i] = at, n, S[i].data_ptr()
+            at += n
+        call(op, k + G * d * es, k, v, ld, la, beta, o, seqs)
+    at, eo, eS = 0, 0.0, 0.0
+    x, lan, ben, got = _np(rows), _np(la), _np(beta), _np(o)
+    assert (got[:, H * dv:] == 7).all()
+    for i, n in enumerate(lengths):
+        assert (got[at:at + gap] == 7).all()
+        at += gap
+        r = x[at:at + n]
+        if n:
+            wo, wS = delta64(r[:, H * dv + G * d:H * dv + 2 * G * d].reshape(n, G, d), r[:, H * dv:H * dv + G * d].reshape(n, G, d),
+                             r[:, :H * dv].reshape(n, H, dv), lan[at:at + n], ben[at:at + n], _np(before[i]), q_scale, eps)
+            eo = max(eo, _off(got[at:at + n, :H * dv], wo.reshape(n, -1)))
+            eS = max(eS, _off(_np(S[i]), wS))
+        else:
+            assert torch.equal(S[i], before[i])
+        at += n
+    return eo, eS
+
+
+# A token's u k^T passes about 20 roundings (convolution, silu, norms, the product with the state, the correction), each 2^-24 of
+# the value that is rounded, and so is off in proportion to its own size, not to the mean size of the state: errors are counted
+# against the largest value.  They add up over tokens as random signs do, and what an error does to later corrections stays
+# bounded (unit keys, beta at most 1): 16 sqrt(T) 2^-24, at least 64 2^-24 for few tokens (20 roundings, threefold).
+def _delta_tol(n):
+    return max(64, 16 * n ** 0.5) * E32
+
+
+DELTA = [  # lengths, H, G, d, dv
+    ([1], 1, 1, 8, 8), ([1], 3, 1, 24, 40), ([2, 1, 5], 4, 2, 16, 24), ([16], 2, 2, 64, 64), ([17, 0, 33], 4, 4, 128, 128), ([63, 64, 65], 6, 2, 40, 72),
+    ([200], 2, 1, 136, 8), ([7] * 8, 2, 2, 8, 136), ([3] * 11, 1, 1, 32, 32), ([130, 1], 2, 2, 264, 16), ([5, 40], 1, 1, 512, 24), ([333], 3, 3, 72, 48)]
+
+
+@pytest.mark.parametrize("f32", [0, 1])
+@pytest.mark.parametrize("lengths,H,G,d,dv", DELTA)
+def test_delta_rows(f32, lengths, H, G, d, dv):
+    for strong in (False, True):
+        rows, la, beta, S = _delta_case(lengths, H, G, d, dv, f32, seed=len(lengths) + d, strong=strong)
+        eo, eS = _delta_run(rows, la, beta, S, lengths, H, G, d, dv, f32)
+        assert eo <= _delta_tol(max(lengths)) and eS <= _delta_tol(max(lengths)), (eo, eS)
+
+
+@pytest.mark.parametrize("f32", [0, 1])
+def test_delta_rows_between_other_rows(f32):
+    lengths, H, G, d, dv = [5, 0, 70], 4, 2, 24, 40
+
+    def call(op, q, k, v, ld, la, beta, o, seqs):
+        import ctypes
+        _lib.call("lt_dn_delta_rows", q, k, v, ld, la.data_ptr(), beta.data_ptr(), H, o.data_ptr(), H * dv + 2, f32, op._ref, ctypes.byref(seqs), stream())
+    rows, la, beta, S = _delta_case(lengths, H, G, d, dv, f32, seed=4, gap=3)
+    eo, eS = _delta_run(rows, la, beta, S, lengths, H, G, d, dv, f32, gap=3, call=call)
+    assert eo <= _delta_tol(70) and eS <= _delta_tol(70)
+
+
+@pytest.mark.parametrize("f32", [0, 1])
+@pytest.mark.parametrize("T", [3, 150])
+def test_delta_extremes(f32, T):
+    """Nothing written (beta 0), everything forgotten (la minus infinity), no decay, zero keys and queries, full corrections with
+    keys that repeat, a growing state."""
+    H, G, d, dv = 6, 6, 32, 24
+    rows, la, beta, S = _delta_case([T], H, G, d, dv, f32, seed=9)
+    la[:, 1:] = 0.0
+    la[:, 0] = -float("inf")
+    la[T // 2, 1] = -float("inf")
+    la[:, 2] = -1e30
+    la[:, 3] = 0.01
+    beta[:, 1] = 0.0
+    beta[:, 4] = 1.0
+    k0 = H * dv
+    rows[:, k0 + 4 * d:k0 + 5 * d] = rows[0, k0 + 4 * d:k0 + 5 * d]        # head 4: one key for all tokens
+    rows[:, k0 + 5 * d:k0 + 6 * d] = 0.0                                   # head 5: no key
+    rows[1, k0 + G * d:k0 + 2 * G * d] = 0.0                               # token 1: no query
+    eo, eS = _delta_run(rows, la, beta, S, [T], H, G, d, dv, f32)
+    assert eo <= _delta_tol(T) and eS <= _delta_tol(T), (eo, eS)
+
+
+@pytest.mark.parametrize("f32", [0, 1])
+@pytest.mark.parametrize("H,G,d,dv,taps", [(1, 1, 8, 8, 1), (4, 2, 16, 24, 4), (6, 3, 40, 72, 3), (2, 2, 128, 128, 4), (3, 1, 264, 16, 5), (2, 1, 512, 40, 2)])
+def test_delta_steps(f32, H, G, d, dv, taps):
+    """Tokens one by one from an empty ring, each with its convolution, against the whole sequence in 64 bits."""
+    T, C = 2 * taps + 3, H * dv + 2 * G * d
+    u = _randn((T, C), 1, DT[f32])
+    conv, conv_b = _randn((taps, C), 2, scale=taps ** -0.5), _randn((C,), 3, scale=0.1)
+    dt, beta, dt_bias, A = _randn((T, H), 4), torch.sigmoid(_randn((T, H), 5)), _randn((H,), 6), -torch.exp(_randn((H,), 7))
+    op = P.DeltaRule(H, G, d, dv, DT[f32], d ** -0.5, 1e-6, taps=taps, conv=conv, conv_b=conv_b, dt_bias=dt_bias, A=A)
+    S = torch.zeros(H, dv, d, device="cuda")
+    ring = torch.full((taps, C), float("nan"), dtype=DT[f32], device="cuda")       # rows of positions that do not exist are not read
+    ln, ticket = torch.zeros(1, dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    o = torch.empty(T, H * dv, device="cuda")
+    for t in range(T):
+        op.step(u[t].data_ptr(), dt[t].data_ptr(), beta[t].data_ptr(), ring.data_ptr(), S.data_ptr(), o[t].data_ptr(), ln.data_ptr(),
+                ticket.data_ptr())
+    assert ln.item() == T and ticket.item() == 0
+    x = np.zeros((T, C))
+    for t in range(T):
+        for i in range(taps):
+            if t - (taps - 1 - i) >= 0:
+                x[t] += _np(conv)[i] * _np(u)[t - (taps - 1 - i)]
+    x = L.silu(x + _np(conv_b))
+    la = _np(A) * np.log1p(np.exp(_np(dt) + _np(dt_bias)))
+    wo, wS = delta64(x[:, H * dv + G * d:].reshape(T, G, d), x[:, H * dv:H * dv + G * d].reshape(T, G, d), x[:, :H * dv].reshape(T, H, dv), la,
+                     _np(beta), np.zeros((H, dv, d)), d ** -0.5, 1e-6)
+    eo, eS = _off(_np(o), wo.reshape(T, -1)), _off(_np(S), wS)
+    assert eo <= _delta_tol(T) and eS <= _delta_tol(T)

@@ -1,0 +1,123 @@
+"""CPU: bindings and refusals of routing, the experts' products and the delta rule."""
+import ctypes
+
+import pytest
+import torch
+
+from llamatov_b200 import _lib, dense_ops as P
+
+
+def _refused(name, text, *args):
+    assert getattr(_lib.dense(), name)(*args) == 1
+    assert text in _lib.last_error(), _lib.last_error()
+
+
+one = ctypes.c_void_p(256)     # never dereferenced: validation fails first
+
+
+def router(**kw):
+    d = dict(n=64, top=6, score=0, groups=1, top_groups=1, renorm=1, scale=1.0)
+    d.update(kw)
+    return ctypes.byref(_lib.DnRouter(**d))
+
+
+def choice(**kw):
+    d = dict(ids=256, plan=None, T=3, top=2, n=8)
+    d.update(kw)
+    return ctypes.byref(_lib.DnChoice(**d))
+
+
+def delta(**kw):
+    d = dict(H=4, G=2, dp=16, dvp=24, q_scale=1.0, eps=1e-6, taps=4, conv=256, conv_b=256, dt_bias=256, A=256)
+    d.update(kw)
+    return ctypes.byref(_lib.DnDelta(**d))
+
+
+def seqs(*items):
+    q = _lib.DnSeqs(n=len(items))
+    for i, (start, rows, S) in enumerate(items):
+        q.start[i], q.rows[i], q.S[i] = start, rows, S
+    return ctypes.byref(q)
+
+
+@pytest.mark.parametrize("kw,ld,T,text", [
+    (dict(), 63, 4, "ld=63"), (dict(n=1025), 2000, 4, "n=1025"), (dict(), 64, 0, "T=0"), (dict(score=2), 64, 4, "unknown score"),
+    (dict(groups=7), 64, 4, "7 groups"), (dict(groups=64, top_groups=8), 64, 4, "at most 32 groups"), (dict(groups=4, top_groups=5), 64, 4, "5 of 4"),
+    (dict(top=33), 64, 4, "top 33"), (dict(top=0), 64, 4, "top 0"), (dict(groups=8, top_groups=1, top=9), 64, 4, "top 9 of 8")])
+def test_route_refusals(kw, ld, T, text):
+    _refused("lt_dn_route", text, one, ld, one, one, T, router(**kw), None)
+    _refused("lt_dn_route", "null", None, 64, one, one, 4, router(), None)
+
+
+def test_experts_refusals():
+    e = P.epilogue(_lib.DN_GLU, glu=(0, 0.0, 0.0))
+    glu = lambda text, ldw=16, ldx=16, ldh=24, F=24, K=16, c=choice(), epi=e, W=one: _refused(
+        "lt_dn_experts_glu", text, W, ldw, one, ldx, one, ldh, 0, F, K, c, ctypes.byref(epi), None)
+    glu("null", W=None)
+    glu("multiples of 8", K=12)
+    glu("multiples of 8", ldw=8)
+    glu("ldh=23", ldh=23)
+    glu("aligned", W=ctypes.c_void_p(264))
+    glu("null choice", c=choice(ids=None))
+    glu("experts", c=choice(n=1025))
+    glu("top", c=choice(top=33))
+    glu("places", c=choice(T=1 << 28, top=8))
+    glu("LT_DN_GLU", epi=P.epilogue())
+    glu("LT_DN_GLU", epi=P.epilogue(_lib.DN_GLU, glu=(0, 0.0, 0.0), out_f32=True))
+    s = lambda text, ldy=24, ldh=16, c=choice(), w=one: _refused("lt_dn_experts_sum", text, one, 16, one, ldh, one, ldy, 0, 24, 16, c, w, None, None, None)
+    s("null", w=None)
+    s("ldy=23", ldy=23)
+    s("multiples of 8", ldh=12)
+    s("without an order", c=choice(T=65536))
+    _refused("lt_dn_experts_plan", "n=1025", one, 3, 2, 1025, one, None)
+    _refused("lt_dn_experts_plan", "null", None, 3, 2, 8, one, None)
+    assert _lib.dense().lt_dn_experts_plan_ints(5, 3, 8) == 24 and _lib.dense().lt_dn_experts_sum_ws(5, 3, 8) == 120
+
+
+def test_delta_refusals():
+    rows = lambda text, d=delta(), q=seqs((0, 5, 256)), ld=96, ldh=4, ldo=96: _refused(
+        "lt_dn_delta_rows", text, one, one, one, ld, one, one, ldh, one, ldo, 0, d, q, None)
+    rows("multiple of the key heads", delta(H=3))
+    rows("multiples of 8", delta(dp=12))
+    rows("above 512", delta(dp=520))
+    rows("eps", delta(eps=0.0))
+    rows("number of sequences", q=ctypes.byref(_lib.DnSeqs(n=0)))
+    rows("number of sequences", q=ctypes.byref(_lib.DnSeqs(n=9)))
+    rows("state is null", q=seqs((0, 5, None)))
+    rows("aligned", q=seqs((0, 5, 264)))
+    rows("rows of a sequence", q=seqs((0, -1, 256)))
+    rows("rows of a sequence", q=seqs((2 ** 31 - 2, 5, 256)))
+    rows("one state", q=seqs((0, 5, 256), (5, 5, 256)))
+    rows("share rows", q=seqs((0, 5, 256), (4, 5, 512)))
+    rows("ldh=3", ldh=3)
+    rows("ldo=95", ldo=95)
+    step = lambda text, d=delta(), S=one: _refused("lt_dn_delta_step", text, one, one, one, one, S, one, 0, one, one, d, None)
+    step("taps=0", delta(taps=0))
+    step("null constants", delta(conv=None))
+    step("aligned", S=ctypes.c_void_p(264))
+    step("null pointer", S=None)
+
+
+def test_no_rows_is_no_launch():
+    n = _lib.launch_count()
+    assert _lib.dense().lt_dn_delta_rows(one, one, one, 96, one, one, 4, one, 96, 0, delta(), seqs((0, 0, 256), (7, 0, 512)), None) == 0
+    assert _lib.launch_count() == n
+
+
+def test_objects_refuse():
+    with pytest.raises(ValueError, match="score"):
+        P.Router(8, 2, score="tanh")
+    with pytest.raises(ValueError, match="top 9"):
+        P.Router(8, 9)
+    with pytest.raises(ValueError, match="groups"):
+        P.Router(8, 2, groups=3)
+    with pytest.raises(ValueError, match="bias"):
+        P.Router(8, 2, bias=torch.zeros(7))
+    with pytest.raises(ValueError, match="matrices"):
+        P.Experts(torch.zeros(4, 4), gated=False)
+    with pytest.raises(ValueError, match="matrices"):
+        P.Experts(torch.zeros(2, 4, 8, dtype=torch.float16), gated=False)
+    with pytest.raises(ValueError, match="gate and up"):
+        P.Experts(torch.zeros(2, 5, 8), gated=True)
+    with pytest.raises(ValueError, match="key heads"):
+        P.DeltaRule(3, 2, 8, 8, torch.float32, 1.0, 1e-6)
