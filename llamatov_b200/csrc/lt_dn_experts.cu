@@ -2,10 +2,11 @@
 //   H[t][j]  = glu(gate and up rows of expert ids[t][j], x_t)                  (lt_dn_experts_glu)
 //   Y[t]    += ls * sum_j w[t][j] (W of expert ids[t][j]) H[t][j]              (lt_dn_experts_sum)
 //
-// Few places: each reads its expert's rows itself, so the time is that of the matrices' bytes.
+// With a plan: lt_dn_experts_group.cu.  Without one (few places) each place reads its expert's rows itself, and the time is that of
+// the matrices' bytes.
 //   k_few_glu   a warp per gate row and its up row
 //   k_few_sum   a CTA per rows of Y; its warps share the experts of the token, and their sums are added in order of j
-#include "lt_dn_common.cuh"
+#include "lt_dn_experts.cuh"
 
 namespace lt {
 namespace dn {
@@ -143,6 +144,11 @@ extern "C" int lt_dn_experts_glu(const void* W, int ldw, const void* X, int ldx,
     LT_REQUIRE(F > 0 && K > 0 && K % 8 == 0 && ldw >= K && ldw % 8 == 0 && ldx >= K && ldx % 8 == 0 && ldh >= F,
                "lt_dn_experts_glu: F=%d K=%d ldw=%d ldx=%d ldh=%d (multiples of 8)", F, K, ldw, ldx, ldh);
     LT_REQUIRE(aligned16(W) && aligned16(X), "lt_dn_experts_glu: W and X must be 16-byte aligned");
+    if (h_c->plan != nullptr) {
+        GroupP G = {W, X, H, device_status_ptr(), F, K, ldw, ldx, ldh, h_c->top, 0, *h_c, *h_epi};
+        LT_REQUIRE(G.status != nullptr, "lt_dn_experts_glu: status word unavailable");
+        return launch_group(G, true, f32, (cudaStream_t)stream);
+    }
     FewP P = {W, X, H, nullptr, nullptr, device_status_ptr(), ldw, ldx, ldh, F, K, *h_c, *h_epi};
     LT_REQUIRE(P.status != nullptr, "lt_dn_experts_glu: status word unavailable");
     const long need = ((long)h_c->T * h_c->top * F + FEW_THREADS / 32 - 1) / (FEW_THREADS / 32);
@@ -162,6 +168,13 @@ extern "C" int lt_dn_experts_sum(const void* W, int ldw, const void* H, int ldh,
     LT_REQUIRE(M > 0 && K > 0 && K % 8 == 0 && ldw >= K && ldw % 8 == 0 && ldh >= K && ldh % 8 == 0 && ldy >= M,
                "lt_dn_experts_sum: M=%d K=%d ldw=%d ldh=%d ldy=%d (multiples of 8)", M, K, ldw, ldh, ldy);
     LT_REQUIRE(aligned16(W) && aligned16(H), "lt_dn_experts_sum: W and H must be 16-byte aligned");
+    if (h_c->plan != nullptr) {
+        LT_REQUIRE(ws != nullptr, "lt_dn_experts_sum: a plan needs the workspace");
+        GroupP G = {W, H, ws, device_status_ptr(), M, K, ldw, ldh, M, 1, 0, *h_c, {}};
+        LT_REQUIRE(G.status != nullptr, "lt_dn_experts_sum: status word unavailable");
+        const int rc = launch_group(G, false, f32, (cudaStream_t)stream);
+        return rc != LT_OK ? rc : launch_combine(ws, w, ls, Y, ldy, M, *h_c, (cudaStream_t)stream);
+    }
     LT_REQUIRE(h_c->T <= 65535, "lt_dn_experts_sum: %d tokens without an order of the places (at most 65535)", h_c->T);
     FewP P = {W, H, Y, w, ls, device_status_ptr(), ldw, ldh, ldy, M, K, *h_c, {}};
     LT_REQUIRE(P.status != nullptr, "lt_dn_experts_sum: status word unavailable");

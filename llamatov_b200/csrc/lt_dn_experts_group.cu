@@ -1,0 +1,477 @@
+// The experts' products for many places: every expert's matrix is read once for all of its places, which the plan lists by
+// expert (lt_dn_route.cu).
+//
+// bf16 (k_group_tc): tcgen05.mma kind::f16, fp32 accumulators in tensor memory.  A tile is 128 gate rows with their 128 up rows (or
+// 256 output rows) of one expert, two MMAs of M = 128, by N places of it.  An expert's places are shared out evenly over as few tiles
+// as hold them, and N is the share rounded up to 16: rows of no place cost at most 15 columns of a tile, whatever the shares are.
+//   warp 8 : producer.  Weights by tiled TMA, the rows of X by gathering TMA (four rows an instruction, a lane each)
+//   warp 9 : one thread issues the MMAs
+//   warps 0-7 : epilogue, a thread per weight row
+// fp32 (k_group_f32): register-blocked tiles on the CUDA cores.
+#include "lt_dn_experts.cuh"
+#include "lt_tc.cuh"
+
+namespace lt {
+namespace dn {
+
+using namespace tc;
+
+constexpr int GK = 64;           // k elements of a stage (128 bytes)
+constexpr int MAX_EXPERTS = 1024;
+
+template <int NT>
+struct GroupCfg {
+    static constexpr int W_STAGE = 2 * 128 * 128, X_STAGE = NT * 128, STAGE = W_STAGE + X_STAGE;
+    static constexpr int NSTAGE = (206 * 1024) / STAGE > 8 ? 8 : (206 * 1024) / STAGE;
+    static constexpr int BUFS = NT <= 128 ? 2 : 1;          // sets of accumulators
+    static constexpr int TMEM = BUFS * 2 * NT;
+    static constexpr int EW = 8, THREADS = (EW + 2) * 32;
+    static constexpr int SMEM = 1024 + NSTAGE * STAGE + 512 + (MAX_EXPERTS + 1) * 4;
+    static_assert(TMEM <= 512 && (TMEM & (TMEM - 1)) == 0, "tensor memory columns");
+    static_assert(SMEM <= 227 * 1024, "shared memory");
+};
+
+struct GroupBars {
+    unsigned long long full[8], empty[8], tfull[2], tempty[2];
+    unsigned tmem_base;
+    int abort_flag;
+    int warp_tiles[10];
+};
+
+// D[tmem] (+)= A[smem] * B[smem], bf16 x bf16 -> fp32
+__device__ __forceinline__ void group_mma(unsigned d, unsigned long long a, unsigned long long b, unsigned idesc, bool acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((int)acc)
+        : "memory");
+}
+// rows y of a map whose box is one row high
+__device__ __forceinline__ void tma_gather4(unsigned dst, const CUtensorMap* map, int x, const int (&y)[4], unsigned bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]), "r"(bar)
+        : "memory");
+}
+
+// Tiles of places by expert: cum[e] tiles lie before expert e's.  Every role walks them with a cursor of its own.
+template <int NT>
+struct Cursor {
+    int e;
+    int from, count, n, rt;      // places of the tile in the plan's list, columns, row tile
+    __device__ __forceinline__ void seek(const GroupP& P, const int* cum, int tile) {
+        const int g = tile / P.row_tiles;
+        rt = tile - g * P.row_tiles;
+        while (cum[e + 1] <= g) e++;
+        const int at = P.c.plan[e], c = P.c.plan[e + 1] - at, tiles = cum[e + 1] - cum[e];
+        n = ((c + tiles - 1) / tiles + 15) & ~15;
+        from = at + (g - cum[e]) * n;
+        count = min(n, at + c - from);       // at least 1: the tiles before hold (tiles - 1) n <= (tiles - 1) NT < c places
+    }
+};
+
+template <int NT, bool GLU>
+__global__ void __launch_bounds__(GroupCfg<NT>::THREADS, 1)
+k_group_tc(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const __grid_constant__ GroupP P) {
+    using C = GroupCfg<NT>;
+    constexpr int NS = C::NSTAGE;
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    unsigned char* base = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    GroupBars* B = (GroupBars*)(base + NS * C::STAGE);
+    int* cum = (int*)(base + NS * C::STAGE + 512);
+    static_assert(sizeof(GroupBars) <= 512, "barriers");
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int nk = (P.K + GK - 1) / GK;
+    volatile int* abort_flag = &B->abort_flag;
+    const int* places = P.c.plan + P.c.n + 1;
+
+    if (tid == 0) {
+        for (int s = 0; s < NS; s++) {
+            mbar_init(&B->full[s], 1);
+            mbar_init(&B->empty[s], 1);
+        }
+        for (int s = 0; s < 2; s++) {
+            mbar_init(&B->tfull[s], 1);
+            mbar_init(&B->tempty[s], C::EW);
+        }
+        B->abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == C::EW + 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&B->tmem_base)),
+                     "r"((unsigned)C::TMEM)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    {   // sums of the experts' tiles: four experts a thread
+        int t[4], sum = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int e = tid * 4 + i;
+            t[i] = e < P.c.n ? (P.c.plan[e + 1] - P.c.plan[e] + NT - 1) / NT : 0;
+            sum += t[i];
+        }
+        int before = sum;
+#pragma unroll
+        for (int s = 1; s < 32; s <<= 1) {
+            const int o = __shfl_up_sync(0xffffffffu, before, s);
+            if (lane >= s) before += o;
+        }
+        if (lane == 31) B->warp_tiles[warp] = before;
+        __syncthreads();
+        before -= sum;
+        for (int w = 0; w < warp; w++) before += B->warp_tiles[w];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (tid * 4 + i <= P.c.n) cum[tid * 4 + i] = before;
+            before += t[i];
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const unsigned tmem = B->tmem_base;
+    const int tiles = cum[P.c.n] * P.row_tiles;
+    Cursor<NT> cur;
+    cur.e = 0;
+
+    if (warp == C::EW) {
+        unsigned it = 0;
+        bool go = true;
+        for (int tile = blockIdx.x; go && tile < tiles; tile += gridDim.x) {
+            cur.seek(P, cum, tile);
+            int y[NT / 128 > 0 ? NT / 128 : 1][4];
+#pragma unroll
+            for (int g = 0; g < (NT + 127) / 128; g++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) y[g][i] = places[cur.from + min((g * 32 + lane) * 4 + i, cur.count - 1)] / P.per;
+            const int row = GLU ? cur.e * 2 * P.M + cur.rt * 128 : cur.e * P.M + cur.rt * 256;
+            const int row2 = GLU ? row + P.M : row + 128;
+            for (int kb = 0; kb < nk; kb++, it++) {
+                const int s = it % NS;
+                const unsigned st = smem_u32(base) + s * C::STAGE, full = smem_u32(&B->full[s]);
+                if (!acquire(smem_u32(&B->empty[s]), ((it / NS) & 1) ^ 1, abort_flag, P.status)) {
+                    go = false;
+                    break;
+                }
+                if (lane == 0) {
+                    bar_expect_tx(full, C::W_STAGE + cur.n * 128);
+                    tma_load_2d(st, &tmW, kb * GK, row, full);
+                    tma_load_2d(st + 128 * 128, &tmW, kb * GK, row2, full);
+                }
+                __syncwarp();
+#pragma unroll
+                for (int g = 0; g < (NT + 127) / 128; g++)
+                    if ((g * 32 + lane) * 4 < cur.n) tma_gather4(st + C::W_STAGE + (g * 32 + lane) * 512, &tmX, kb * GK, y[g], full);
+            }
+        }
+    } else if (warp == C::EW + 1) {
+        if (lane == 0) {
+            const unsigned long long w0 = smem_desc<4>(smem_u32(base));
+            const unsigned long long x0 = smem_desc<4>(smem_u32(base) + C::W_STAGE);
+            unsigned it = 0, n = 0;
+            for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+                cur.seek(P, cum, tile);
+                    // D fp32, A and B bf16, both K-major, M = 128
+                const unsigned idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(cur.n >> 3) << 17) | ((unsigned)(128 >> 4) << 24);
+                const unsigned slot = n % C::BUFS;
+                mbar_wait<32>(&B->tempty[slot], ((n / C::BUFS) & 1) ^ 1, abort_flag, P.status);
+                tc_fence_after();
+                const unsigned d = tmem + slot * 2 * NT;
+                for (int kb = 0; kb < nk; kb++, it++) {
+                    const unsigned s = it % NS;
+                    mbar_wait<0>(&B->full[s], (it / NS) & 1, abort_flag, P.status);
+                    tc_fence_after();
+                    const unsigned long long wd = w0 + (unsigned long long)(s * (C::STAGE >> 4));
+                    const unsigned long long xd = x0 + (unsigned long long)(s * (C::STAGE >> 4));
+#pragma unroll
+                    for (int j = 0; j < GK / 16; j++)
+#pragma unroll
+                        for (int a = 0; a < 2; a++)
+                            group_mma(d + a * NT, wd + a * (128 * 128 >> 4) + 2 * j, xd + 2 * j, idesc, kb > 0 || j > 0);
+                    mma_commit(&B->empty[s]);
+                }
+                mma_commit(&B->tfull[slot]);
+                n++;
+            }
+        }
+    } else {
+        const int q = warp & 3, cg = warp >> 2;
+        unsigned n = 0;
+        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+            cur.seek(P, cum, tile);
+            const int row = cur.rt * (GLU ? 128 : 256) + q * 32 + lane;
+            const unsigned slot = n % C::BUFS;
+            mbar_wait<32>(&B->tfull[slot], (n / C::BUFS) & 1, abort_flag, P.status);
+            tc_fence_after();
+            const unsigned ta = tmem + ((unsigned)(q * 32) << 16) + slot * 2 * NT;
+#pragma unroll 1
+            for (int c0 = cg * 16; c0 < cur.count; c0 += 32) {
+                const int mine = places[cur.from + min(c0 + (lane & 15), cur.count - 1)];
+                int v[2][16];
+#pragma unroll
+                for (int a = 0; a < 2; a++) tmem_ld<16>(ta + a * NT + c0, v[a]);
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                for (int a = 0; a < 2; a++)
+#pragma unroll
+                    for (int c = 0; c < 16; c += 4) reg_fence4(&v[a][c]);
+                if (GLU) {
+                    float f[16];
+                    glu_bf16(P.epi, v[0], v[1], f);
+#pragma unroll
+                    for (int c = 0; c < 16; c++) {
+                        const int p = __shfl_sync(0xffffffffu, mine, c);
+                        if (row < P.M && c0 + c < cur.count) ((bf16*)P.Y)[(long)p * P.ldy + row] = from_f<bf16>(f[c]);
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 16; c++) {
+                        const int p = __shfl_sync(0xffffffffu, mine, c);
+                        float* y = (float*)P.Y + (long)p * P.ldy + row;
+                        if (c0 + c < cur.count) {
+                            if (row < P.M) y[0] = __int_as_float(v[0][c]);
+                            if (row + 128 < P.M) y[128] = __int_as_float(v[1][c]);
+                        }
+                    }
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&B->tempty[slot]);
+            n++;
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (*abort_flag && tid == 0) {     // a wait ran out: let copies in flight land before the CTA leaves
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000LL) {
+        }
+    }
+    __syncthreads();
+    if (warp == C::EW + 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((unsigned)C::TMEM) : "memory");
+    }
+}
+
+static int group_map(CUtensorMap* m, const void* ptr, long rows, int K, int ld, int box_rows) {
+    encode_fn_t fn = encode_fn();
+    LT_REQUIRE(fn != nullptr, "experts' products: cuTensorMapEncodeTiled is not available from this driver");
+    cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
+    cuuint32_t box[2] = {(cuuint32_t)GK, (cuuint32_t)box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        set_error("experts' products: cuTensorMapEncodeTiled failed (%d) for rows=%ld K=%d ld=%d", (int)r, rows, K, ld);
+        return LT_ERR_CUDA;
+    }
+    return LT_OK;
+}
+
+template <int NT, bool GLU>
+static int launch_group_tc(GroupP P, cudaStream_t s) {
+    using C = GroupCfg<NT>;
+    CUtensorMap tmW, tmX;
+    int rc = group_map(&tmW, P.W, (long)P.c.n * P.M * (GLU ? 2 : 1), P.K, P.ldw, 128);
+    if (rc != LT_OK) return rc;
+    rc = group_map(&tmX, P.X, (long)P.c.T * P.c.top / P.per, P.K, P.ldx, 1);
+    if (rc != LT_OK) return rc;
+    static PerDeviceOnce once;
+    if (once.first()) LT_CUDA(cudaFuncSetAttribute(k_group_tc<NT, GLU>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    P.row_tiles = (P.M + (GLU ? 127 : 255)) / (GLU ? 128 : 256);
+    k_group_tc<NT, GLU><<<sm_count(), C::THREADS, C::SMEM, s>>>(tmW, tmX, P);
+    return check_launch("experts' products");
+}
+template <bool GLU>
+static int pick_group_tc(const GroupP& P, cudaStream_t s) {
+    const long each = (long)P.c.T * P.c.top / P.c.n;        // places of an expert
+    if (each <= 24) return launch_group_tc<64, GLU>(P, s);
+    if (each <= 64) return launch_group_tc<128, GLU>(P, s);
+    return launch_group_tc<256, GLU>(P, s);
+}
+
+// ---------------------------------------------------------------------------- fp32
+
+// 64 weight rows (with GLU: and their 64 up rows) x 32 places of one expert per CTA of 128 threads; a thread owns 4 rows x 4
+// places, 16-byte reads of shared memory, three stages of 32 k filled by asynchronous copies.  k is added up 256 at a time, so that
+// chains of roundings stay short.
+constexpr int GF_THREADS = 128, GF_BM = 64, GF_BN = 32, GF_BK = 32, GF_ST = GF_BK + 4, GF_STAGES = 3, GF_PART = 8;
+
+template <bool GLU>
+__global__ void __launch_bounds__(GF_THREADS) k_group_f32(const __grid_constant__ GroupP P) {
+    constexpr int NG = GLU ? 2 : 1, ROWS = NG * GF_BM + GF_BN;
+    extern __shared__ __align__(16) float gf_smem[];
+    __shared__ int place[GF_BN];
+    __shared__ int found[3];                 // expert, first place in the list, places
+    const int tid = threadIdx.x, lane = tid & 31, n = tid & 15, m = tid >> 4;
+    const int n0 = blockIdx.x * GF_BM, g = blockIdx.y;
+    if (tid < 32) {                          // the expert whose tiles hold number g: 32 experts at a time
+        int before = 0;
+        bool done = false;
+        for (int e0 = 0; e0 < P.c.n && !done; e0 += 32) {
+            const int e = e0 + lane, at = e < P.c.n ? P.c.plan[e] : 0, c = e < P.c.n ? P.c.plan[e + 1] - at : 0;
+            const int tiles = (c + GF_BN - 1) / GF_BN;
+            int up = tiles;
+#pragma unroll
+            for (int s = 1; s < 32; s <<= 1) {
+                const int o = __shfl_up_sync(0xffffffffu, up, s);
+                if (lane >= s) up += o;
+            }
+            const int first = before + up - tiles;
+            if (g >= first && g < first + tiles) {
+                found[0] = e;
+                found[1] = at + (g - first) * GF_BN;
+                found[2] = min(GF_BN, c - (g - first) * GF_BN);
+            }
+            before += __shfl_sync(0xffffffffu, up, 31);
+            done = before > g;
+        }
+        if (!done && lane == 0) found[2] = 0;
+        __syncwarp();
+        const int count = found[2];
+        if (count > 0) place[lane] = P.c.plan[P.c.n + 1 + found[1] + min(lane, count - 1)];
+    }
+    __syncthreads();
+    const int count = found[2];
+    if (count == 0) return;
+    const float* W = (const float*)P.W + (long)found[0] * NG * P.M * P.ldw;
+    const int nk = (P.K + GF_BK - 1) / GF_BK;
+    auto copy = [&](int c, int stage) {
+        float* dst = gf_smem + stage * ROWS * GF_ST;
+        if (c < nk) {
+#pragma unroll
+            for (int e = tid; e < ROWS * (GF_BK / 4); e += GF_THREADS) {
+                const int r = e >> 3, k = c * GF_BK + (e & 7) * 4;          // K is a multiple of 8
+                const float* src;
+                bool ok = k < P.K;
+                if (r < NG * GF_BM) {
+                    const int row = n0 + (r & (GF_BM - 1));
+                    ok = ok && row < P.M;
+                    src = W + (long)((r / GF_BM) * P.M + row) * P.ldw + k;
+                } else {
+                    src = (const float*)P.X + (long)(place[r - NG * GF_BM] / P.per) * P.ldx + k;
+                }
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst + r * GF_ST + (e & 7) * 4)),
+                             "l"(ok ? src : (const float*)P.W), "r"(ok ? 16 : 0)
+                             : "memory");
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    float acc[NG][4][4], all[NG][4][4];
+#pragma unroll
+    for (int a = 0; a < NG; a++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) acc[a][i][j] = all[a][i][j] = 0.0f;
+#pragma unroll
+    for (int s = 0; s < GF_STAGES - 1; s++) copy(s, s);
+    int stage = 0;
+    for (int c = 0; c < nk; c++) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(GF_STAGES - 2) : "memory");
+        __syncthreads();                                   // chunk c is there, chunk c - 1 is used up
+        copy(c + GF_STAGES - 1, stage == 0 ? GF_STAGES - 1 : stage - 1);
+        const float4* w4 = (const float4*)(gf_smem + (stage * ROWS + n) * GF_ST);
+        const float4* x4 = (const float4*)(gf_smem + (stage * ROWS + NG * GF_BM + m * 4) * GF_ST);
+#pragma unroll 4
+        for (int k = 0; k < GF_BK / 4; k++) {
+            float4 x[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[i] = x4[i * (GF_ST / 4) + k];
+#pragma unroll
+            for (int a = 0; a < NG; a++) {
+                float4 w[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) w[j] = w4[(a * GF_BM + 16 * j) * (GF_ST / 4) + k];
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        acc[a][i][j] = fmaf(w[j].w, x[i].w, fmaf(w[j].z, x[i].z, fmaf(w[j].y, x[i].y, fmaf(w[j].x, x[i].x, acc[a][i][j]))));
+            }
+        }
+        stage = stage == GF_STAGES - 1 ? 0 : stage + 1;
+        if (c % GF_PART == GF_PART - 1 || c + 1 == nk) {
+#pragma unroll
+            for (int a = 0; a < NG; a++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        all[a][i][j] += acc[a][i][j];
+                        acc[a][i][j] = 0.0f;
+                    }
+        }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if (m * 4 + i >= count) break;
+        const long y = (long)place[m * 4 + i] * P.ldy;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int row = n0 + n + 16 * j;
+            if (row >= P.M) break;
+            if (GLU) glu_store<float>(P.epi, P.Y, y + row, all[0][i][j], all[NG - 1][i][j]);
+            else ((float*)P.Y)[y + row] = all[0][i][j];
+        }
+    }
+}
+
+template <bool GLU>
+static int launch_group_f32(const GroupP& P, cudaStream_t s) {
+    constexpr int SMEM = GF_STAGES * ((GLU ? 2 : 1) * GF_BM + GF_BN) * GF_ST * 4;
+    static PerDeviceOnce once;
+    if (once.first()) LT_CUDA(cudaFuncSetAttribute(k_group_f32<GLU>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+    const long places = (long)P.c.T * P.c.top;
+    const long tiles = places < P.c.n ? places : P.c.n + (places - P.c.n) / GF_BN;        // at most: one begun by every expert
+    LT_REQUIRE(tiles <= 65535, "experts' products: %ld places in fp32", places);
+    k_group_f32<GLU><<<dim3((P.M + GF_BM - 1) / GF_BM, (unsigned)tiles), GF_THREADS, SMEM, s>>>(P);
+    return check_launch("experts' products");
+}
+
+int launch_group(GroupP P, bool glu, bool f32, cudaStream_t s) {
+    if (f32) return glu ? launch_group_f32<true>(P, s) : launch_group_f32<false>(P, s);
+    return glu ? pick_group_tc<true>(P, s) : pick_group_tc<false>(P, s);
+}
+
+// ---------------------------------------------------------------------------- sum over a token's places
+
+__global__ void __launch_bounds__(256) k_combine(const float* __restrict__ ws, const float* __restrict__ w, const float* __restrict__ ls, float* Y,
+                                                 int ldy, int M, const __grid_constant__ lt_dn_choice c) {
+    __shared__ float sw[32];
+    __shared__ int on[32];
+    const int t = blockIdx.x, m = blockIdx.y * 256 + threadIdx.x;
+    if (threadIdx.x < c.top) {
+        const int e = c.ids[(long)t * c.top + threadIdx.x];
+        on[threadIdx.x] = e >= 0 && e < c.n;
+        sw[threadIdx.x] = w[(long)t * c.top + threadIdx.x];
+    }
+    __syncthreads();
+    if (m >= M) return;
+    float v = 0.0f;
+    bool any = false;
+    for (int j = 0; j < c.top; j++)
+        if (on[j]) {
+            v = fmaf(sw[j], ws[((long)t * c.top + j) * M + m], v);
+            any = true;
+        }
+    float* y = Y + (long)t * ldy + m;
+    if (any) *y = fmaf(ls != nullptr ? ls[m] : 1.0f, v, *y);
+}
+
+int launch_combine(const float* ws, const float* w, const float* ls, float* Y, int ldy, int M, const lt_dn_choice& c, cudaStream_t s) {
+    k_combine<<<dim3(c.T, (M + 255) / 256), 256, 0, s>>>(ws, w, ls, Y, ldy, M, c);
+    return check_launch("lt_dn_experts_sum");
+}
+
+}  // namespace dn
+}  // namespace lt

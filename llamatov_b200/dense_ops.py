@@ -129,6 +129,9 @@ def _here(t, what):
     return t
 
 
+GROUP_FROM = 64         # places from which on the products go expert by expert
+
+
 class Router:
     """Choice of `top` of n experts for rows of fp32 scores, and the weights of the chosen (lt_dn_route)."""
 
@@ -185,7 +188,12 @@ class Experts:
             raise ValueError(f"ids must be contiguous int32 [{T}, top], got {ids.dtype} {tuple(ids.shape)}")
         _here(ids, "ids")
         _here(self.W, "the experts' matrix")
-        return Places(ids, self.n)
+        top = ids.shape[1]
+        if T * top < GROUP_FROM:
+            return Places(ids, self.n)
+        buf = torch.empty(_lib.dense().lt_dn_experts_plan_ints(T, top, self.n), dtype=torch.int32, device="cuda")
+        _lib.call("lt_dn_experts_plan", ids.data_ptr(), T, top, self.n, buf.data_ptr(), dr._stream())
+        return Places(ids, self.n, buf)
 
     def hidden(self, x, ldx, places, h, ldh):
         """h[t*top + j] = glu of the gate and up rows of place (t, j)'s expert, for the rows of x."""
@@ -195,6 +203,9 @@ class Experts:
     def add_sum(self, h, ldh, places, w, y, ldy, ls=None):
         """y[t] += ls * sum over j of w[t][j] W h[t*top + j]."""
         ws = None
+        if places.buf is not None:
+            buf = torch.empty(_lib.dense().lt_dn_experts_sum_ws(places.T, places.top, self.M), dtype=torch.float32, device="cuda")
+            ws = buf.data_ptr()
         _lib.call("lt_dn_experts_sum", self.ptr, self.K, h, ldh, y, ldy, self.f32, self.M, self.K, places.ref, w, ls, ws, dr._stream())
 
 

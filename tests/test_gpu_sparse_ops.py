@@ -132,6 +132,13 @@ def _clamped(limit):
 GLU = {"gelu": ((0, 0.0, 0.0), lambda g, u: _gelu(g) * u), "clamped": ((1, 1.702, 1.2), _clamped(1.2))}
 
 
+@pytest.fixture(params=["few", "group"])
+def form(request, monkeypatch):
+    """Both forms of the products, whatever the number of places."""
+    monkeypatch.setattr(P, "GROUP_FROM", 1 if request.param == "group" else 10 ** 9)
+    return request.param
+
+
 def _ids(T, top, n, seed, how="spread"):
     g = torch.Generator().manual_seed(seed)
     if how == "one":                                   # everything to one expert (and its neighbours)
@@ -143,10 +150,11 @@ def _ids(T, top, n, seed, how="spread"):
 
 SIZES = [  # T, top, n, K, F or M
     (1, 1, 1, 8, 1), (1, 2, 4, 24, 9), (1, 8, 64, 264, 136), (2, 3, 5, 40, 130), (17, 2, 3, 72, 33), (37, 4, 16, 896, 616), (64, 4, 8, 64, 128),
-    (65, 1, 2, 128, 256), (200, 8, 16, 136, 264), (33, 32, 40, 16, 24), (300, 2, 70, 520, 136)]
+    (65, 1, 2, 128, 256), (200, 8, 16, 136, 264), (33, 32, 40, 16, 24), (300, 2, 70, 520, 136),
+    (600, 1, 2, 200, 40), (515, 2, 2, 64, 300)]
 
 
-def _check_glu(T, top, n, K, F, f32, how="spread", act="gelu", seed=1, ids=None, form=None):
+def _check_glu(T, top, n, K, F, f32, how="spread", act="gelu", seed=1, ids=None):
     W, X = _randn((n, 2 * F, K), seed, DT[f32], 1.5 * K ** -0.5), _randn((T, K + 8), seed + 1, DT[f32])
     ids = _ids(T, top, n, seed + 2, how) if ids is None else ids
     dids = ids.cuda()
@@ -171,13 +179,13 @@ def _check_glu(T, top, n, K, F, f32, how="spread", act="gelu", seed=1, ids=None,
 
 @pytest.mark.parametrize("f32", [0, 1])
 @pytest.mark.parametrize("T,top,n,K,F", SIZES)
-def test_experts_glu(f32, T, top, n, K, F):
+def test_experts_glu(form, f32, T, top, n, K, F):
     _check_glu(T, top, n, K, F, f32)
 
 
 @pytest.mark.parametrize("f32", [0, 1])
 @pytest.mark.parametrize("how", ["one", "same"])
-def test_experts_glu_crowded(f32, how):
+def test_experts_glu_crowded(form, f32, how):
     _check_glu(150, 3, 9, 72, 136, f32, how, "clamped")
     _check_glu(3, 3, 9, 72, 136, f32, how, "clamped")
 
@@ -207,20 +215,20 @@ def _check_sum(T, top, n, K, M, f32, how="spread", ls=True, seed=11, ids=None):
 
 @pytest.mark.parametrize("f32", [0, 1])
 @pytest.mark.parametrize("T,top,n,K,M", SIZES)
-def test_experts_sum(f32, T, top, n, K, M):
+def test_experts_sum(form, f32, T, top, n, K, M):
     _check_sum(T, top, n, K, M, f32)
 
 
 @pytest.mark.parametrize("f32", [0, 1])
 @pytest.mark.parametrize("how", ["one", "same"])
-def test_experts_sum_crowded(f32, how):
+def test_experts_sum_crowded(form, f32, how):
     _check_sum(150, 3, 9, 72, 136, f32, how, ls=False)
     _check_sum(3, 3, 9, 72, 136, f32, how, ls=False)
 
 
 @pytest.mark.parametrize("f32", [0, 1])
 @pytest.mark.parametrize("T", [2, 90])
-def test_experts_places_left_out(f32, T):
+def test_experts_places_left_out(form, f32, T):
     """Ids below zero leave a place out; a token all of whose places are left out keeps its row."""
     ids = _ids(T, 4, 8, 3)
     ids[0] = -1
@@ -233,7 +241,7 @@ def test_experts_places_left_out(f32, T):
 
 
 @pytest.mark.parametrize("T", [2, 90])
-def test_experts_ids_out_of_range_are_reported(T):
+def test_experts_ids_out_of_range_are_reported(form, T):
     ids = _ids(T, 4, 8, 3)
     ids[1, 1] = 8
     ids[T - 1, 3] = 2 ** 31 - 1
