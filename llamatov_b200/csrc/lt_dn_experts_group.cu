@@ -4,7 +4,9 @@
 // bf16 (k_group_tc): tcgen05.mma kind::f16, fp32 accumulators in tensor memory.  A tile is 128 gate rows with their 128 up rows (or
 // 256 output rows) of one expert, two MMAs of M = 128, by N places of it.  An expert's places are shared out evenly over as few tiles
 // as hold them, and N is the share rounded up to 16: rows of no place cost at most 15 columns of a tile, whatever the shares are.
-//   warp 8 : producer.  Weights by tiled TMA, the rows of X by gathering TMA (four rows an instruction, a lane each)
+//   warp 8 : weights, by tiled TMA
+//   warps 10-13 : the rows of X, by asynchronous copies of 16 bytes into the swizzled layout.  (Gathering TMA, four rows an
+//                 instruction, took 83 clocks each and 425 us where these copies take 121.)
 //   warp 9 : one thread issues the MMAs
 //   warps 0-7 : epilogue, a thread per weight row
 // fp32 (k_group_f32): register-blocked tiles on the CUDA cores.
@@ -25,7 +27,7 @@ struct GroupCfg {
     static constexpr int NSTAGE = (206 * 1024) / STAGE > 8 ? 8 : (206 * 1024) / STAGE;
     static constexpr int BUFS = NT <= 128 ? 2 : 1;          // sets of accumulators
     static constexpr int TMEM = BUFS * 2 * NT;
-    static constexpr int EW = 8, THREADS = (EW + 2) * 32;
+    static constexpr int EW = 8, XW = 4, THREADS = (EW + 2 + XW) * 32;
     static constexpr int SMEM = 1024 + NSTAGE * STAGE + 512 + (MAX_EXPERTS + 1) * 4;
     static_assert(TMEM <= 512 && (TMEM & (TMEM - 1)) == 0, "tensor memory columns");
     static_assert(SMEM <= 227 * 1024, "shared memory");
@@ -35,7 +37,7 @@ struct GroupBars {
     unsigned long long full[8], empty[8], tfull[2], tempty[2];
     unsigned tmem_base;
     int abort_flag;
-    int warp_tiles[10];
+    int warp_tiles[14];
 };
 
 // D[tmem] (+)= A[smem] * B[smem], bf16 x bf16 -> fp32
@@ -47,12 +49,9 @@ __device__ __forceinline__ void group_mma(unsigned d, unsigned long long a, unsi
         "l"(a), "l"(b), "r"(idesc), "r"((int)acc)
         : "memory");
 }
-// rows y of a map whose box is one row high
-__device__ __forceinline__ void tma_gather4(unsigned dst, const CUtensorMap* map, int x, const int (&y)[4], unsigned bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
-        "l"(map), "r"(x), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]), "r"(bar)
-        : "memory");
+// arrives when this thread's copies so far have landed
+__device__ __forceinline__ void cp_async_arrive(unsigned bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 
 // Tiles of places by expert: cum[e] tiles lie before expert e's.  Every role walks them with a cursor of its own.
@@ -73,7 +72,7 @@ struct Cursor {
 
 template <int NT, bool GLU>
 __global__ void __launch_bounds__(GroupCfg<NT>::THREADS, 1)
-k_group_tc(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const __grid_constant__ GroupP P) {
+k_group_tc(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ GroupP P) {
     using C = GroupCfg<NT>;
     constexpr int NS = C::NSTAGE;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -88,7 +87,7 @@ k_group_tc(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
 
     if (tid == 0) {
         for (int s = 0; s < NS; s++) {
-            mbar_init(&B->full[s], 1);
+            mbar_init(&B->full[s], 1 + C::XW * 32);
             mbar_init(&B->empty[s], 1);
         }
         for (int s = 0; s < 2; s++) {
@@ -142,11 +141,6 @@ k_group_tc(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
         bool go = true;
         for (int tile = blockIdx.x; go && tile < tiles; tile += gridDim.x) {
             cur.seek(P, cum, tile);
-            int y[NT / 128 > 0 ? NT / 128 : 1][4];
-#pragma unroll
-            for (int g = 0; g < (NT + 127) / 128; g++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) y[g][i] = places[cur.from + min((g * 32 + lane) * 4 + i, cur.count - 1)] / P.per;
             const int row = GLU ? cur.e * 2 * P.M + cur.rt * 128 : cur.e * P.M + cur.rt * 256;
             const int row2 = GLU ? row + P.M : row + 128;
             for (int kb = 0; kb < nk; kb++, it++) {
@@ -157,16 +151,42 @@ k_group_tc(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
                     break;
                 }
                 if (lane == 0) {
-                    bar_expect_tx(full, C::W_STAGE + cur.n * 128);
+                    bar_expect_tx(full, C::W_STAGE);
                     tma_load_2d(st, &tmW, kb * GK, row, full);
                     tma_load_2d(st + 128 * 128, &tmW, kb * GK, row2, full);
                 }
                 __syncwarp();
-#pragma unroll
-                for (int g = 0; g < (NT + 127) / 128; g++)
-                    if ((g * 32 + lane) * 4 < cur.n) tma_gather4(st + C::W_STAGE + (g * 32 + lane) * 512, &tmX, kb * GK, y[g], full);
             }
         }
+    } else if (warp >= C::EW + 2) {
+        // eight threads a row, 16 rows at a time; the row's 16-byte units stand where the 128-byte swizzle puts them
+        const int xt = tid - (C::EW + 2) * 32, r0 = xt >> 3, unit = xt & 7;
+        const unsigned dst0 = smem_u32(base) + C::W_STAGE + r0 * 128 + ((unit ^ (r0 & 7)) << 4);
+        unsigned it = 0;
+        bool go = true;
+        for (int tile = blockIdx.x; go && tile < tiles; tile += gridDim.x) {
+            cur.seek(P, cum, tile);
+            const bf16* src[NT / 16];
+#pragma unroll
+            for (int i = 0; i < NT / 16; i++)
+                src[i] = (const bf16*)P.X + (long)(places[cur.from + min(r0 + 16 * i, cur.count - 1)] / P.per) * P.ldx + unit * 8;
+            for (int kb = 0; kb < nk; kb++, it++) {
+                const int s = it % NS;
+                if (!acquire(smem_u32(&B->empty[s]), ((it / NS) & 1) ^ 1, abort_flag, P.status)) {
+                    go = false;
+                    break;
+                }
+                const int k = kb * GK, bytes = k + unit * 8 < P.K ? 16 : 0;
+                const unsigned dst = dst0 + s * C::STAGE;
+#pragma unroll
+                for (int i = 0; i < NT / 16; i++)
+                    if (16 * i < cur.n)
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + i * 2048), "l"(bytes ? src[i] + k : (const bf16*)P.X), "r"(bytes)
+                                     : "memory");
+                cp_async_arrive(smem_u32(&B->full[s]));
+            }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
     } else if (warp == C::EW + 1) {
         if (lane == 0) {
             const unsigned long long w0 = smem_desc<4>(smem_u32(base));
@@ -183,6 +203,7 @@ k_group_tc(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
                 for (int kb = 0; kb < nk; kb++, it++) {
                     const unsigned s = it % NS;
                     mbar_wait<0>(&B->full[s], (it / NS) & 1, abort_flag, P.status);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // X was copied through the generic proxy
                     tc_fence_after();
                     const unsigned long long wd = w0 + (unsigned long long)(s * (C::STAGE >> 4));
                     const unsigned long long xd = x0 + (unsigned long long)(s * (C::STAGE >> 4));
@@ -259,12 +280,12 @@ k_group_tc(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
     }
 }
 
-static int group_map(CUtensorMap* m, const void* ptr, long rows, int K, int ld, int box_rows) {
+static int group_map(CUtensorMap* m, const void* ptr, long rows, int K, int ld) {
     encode_fn_t fn = encode_fn();
     LT_REQUIRE(fn != nullptr, "experts' products: cuTensorMapEncodeTiled is not available from this driver");
     cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
     cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
-    cuuint32_t box[2] = {(cuuint32_t)GK, (cuuint32_t)box_rows};
+    cuuint32_t box[2] = {(cuuint32_t)GK, 128};
     cuuint32_t estr[2] = {1, 1};
     CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -278,15 +299,13 @@ static int group_map(CUtensorMap* m, const void* ptr, long rows, int K, int ld, 
 template <int NT, bool GLU>
 static int launch_group_tc(GroupP P, cudaStream_t s) {
     using C = GroupCfg<NT>;
-    CUtensorMap tmW, tmX;
-    int rc = group_map(&tmW, P.W, (long)P.c.n * P.M * (GLU ? 2 : 1), P.K, P.ldw, 128);
-    if (rc != LT_OK) return rc;
-    rc = group_map(&tmX, P.X, (long)P.c.T * P.c.top / P.per, P.K, P.ldx, 1);
+    CUtensorMap tmW;
+    const int rc = group_map(&tmW, P.W, (long)P.c.n * P.M * (GLU ? 2 : 1), P.K, P.ldw);
     if (rc != LT_OK) return rc;
     static PerDeviceOnce once;
     if (once.first()) LT_CUDA(cudaFuncSetAttribute(k_group_tc<NT, GLU>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
     P.row_tiles = (P.M + (GLU ? 127 : 255)) / (GLU ? 128 : 256);
-    k_group_tc<NT, GLU><<<sm_count(), C::THREADS, C::SMEM, s>>>(tmW, tmX, P);
+    k_group_tc<NT, GLU><<<sm_count(), C::THREADS, C::SMEM, s>>>(tmW, P);
     return check_launch("experts' products");
 }
 template <bool GLU>
