@@ -225,12 +225,16 @@ k_group_tc(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ Grou
             cur.seek(P, cum, tile);
             const int row = cur.rt * (GLU ? 128 : 256) + q * 32 + lane;
             const unsigned slot = n % C::BUFS;
+            int mine[NT / 32];                // places of this warp's columns, fetched under the products
+#pragma unroll
+            for (int i = 0; i < NT / 32; i++) mine[i] = places[cur.from + min(32 * i + cg * 16 + (lane & 15), cur.count - 1)];
             mbar_wait<32>(&B->tfull[slot], (n / C::BUFS) & 1, abort_flag, P.status);
             tc_fence_after();
             const unsigned ta = tmem + ((unsigned)(q * 32) << 16) + slot * 2 * NT;
-#pragma unroll 1
-            for (int c0 = cg * 16; c0 < cur.count; c0 += 32) {
-                const int mine = places[cur.from + min(c0 + (lane & 15), cur.count - 1)];
+#pragma unroll
+            for (int i = 0; i < NT / 32; i++) {
+                const int c0 = 32 * i + cg * 16, left = cur.count - c0;
+                if (left <= 0) break;
                 int v[2][16];
 #pragma unroll
                 for (int a = 0; a < 2; a++) tmem_ld<16>(ta + a * NT + c0, v[a]);
@@ -242,19 +246,20 @@ k_group_tc(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ Grou
                 if (GLU) {
                     float f[16];
                     glu_bf16(P.epi, v[0], v[1], f);
+                    bf16* y = (bf16*)P.Y + row;
 #pragma unroll
                     for (int c = 0; c < 16; c++) {
-                        const int p = __shfl_sync(0xffffffffu, mine, c);
-                        if (row < P.M && c0 + c < cur.count) ((bf16*)P.Y)[(long)p * P.ldy + row] = from_f<bf16>(f[c]);
+                        const int p = __shfl_sync(0xffffffffu, mine[i], c);
+                        if (row < P.M && c < left) y[(long)p * P.ldy] = from_f<bf16>(f[c]);
                     }
                 } else {
+                    float* y = (float*)P.Y + row;
 #pragma unroll
                     for (int c = 0; c < 16; c++) {
-                        const int p = __shfl_sync(0xffffffffu, mine, c);
-                        float* y = (float*)P.Y + (long)p * P.ldy + row;
-                        if (c0 + c < cur.count) {
-                            if (row < P.M) y[0] = __int_as_float(v[0][c]);
-                            if (row + 128 < P.M) y[128] = __int_as_float(v[1][c]);
+                        const long p = (long)__shfl_sync(0xffffffffu, mine[i], c) * P.ldy;
+                        if (c < left) {
+                            if (row < P.M) y[p] = __int_as_float(v[0][c]);
+                            if (row + 128 < P.M) y[p + 128] = __int_as_float(v[1][c]);
                         }
                     }
                 }
@@ -464,31 +469,63 @@ int launch_group(GroupP P, bool glu, bool f32, cudaStream_t s) {
 
 // ---------------------------------------------------------------------------- sum over a token's places
 
+// V columns a thread, four places' loads in flight
+template <int V>
 __global__ void __launch_bounds__(256) k_combine(const float* __restrict__ ws, const float* __restrict__ w, const float* __restrict__ ls, float* Y,
                                                  int ldy, int M, const __grid_constant__ lt_dn_choice c) {
     __shared__ float sw[32];
-    __shared__ int on[32];
-    const int t = blockIdx.x, m = blockIdx.y * 256 + threadIdx.x;
-    if (threadIdx.x < c.top) {
-        const int e = c.ids[(long)t * c.top + threadIdx.x];
-        on[threadIdx.x] = e >= 0 && e < c.n;
-        sw[threadIdx.x] = w[(long)t * c.top + threadIdx.x];
+    __shared__ int from[32];             // the places that count, in order
+    __shared__ int used;
+    const int t = blockIdx.x, m = (blockIdx.y * 256 + threadIdx.x) * V;
+    if (threadIdx.x < 32) {
+        const int j = threadIdx.x, e = j < c.top ? c.ids[(long)t * c.top + j] : -1;
+        const bool on = e >= 0 && e < c.n;
+        const unsigned all = __ballot_sync(0xffffffffu, on);
+        if (on) {
+            const int at = __popc(all & ((1u << j) - 1));
+            from[at] = j;
+            sw[at] = w[(long)t * c.top + j];
+        }
+        if (j == 0) used = __popc(all);
     }
     __syncthreads();
-    if (m >= M) return;
-    float v = 0.0f;
-    bool any = false;
-    for (int j = 0; j < c.top; j++)
-        if (on[j]) {
-            v = fmaf(sw[j], ws[((long)t * c.top + j) * M + m], v);
-            any = true;
+    if (m >= M || used == 0) return;
+    const float* in = ws + (long)t * c.top * M + m;
+    float v[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) v[i] = 0.0f;
+    for (int j = 0; j < used; j += 4) {
+        float x[4][V];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            if (j + u >= used) break;
+            const float* p = in + (long)from[j + u] * M;
+            if (V == 4) *(float4*)x[u] = __ldcs((const float4*)p);
+            else x[u][0] = __ldcs(p);
         }
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            if (j + u >= used) break;
+#pragma unroll
+            for (int i = 0; i < V; i++) v[i] = fmaf(sw[j + u], x[u][i], v[i]);
+        }
+    }
     float* y = Y + (long)t * ldy + m;
-    if (any) *y = fmaf(ls != nullptr ? ls[m] : 1.0f, v, *y);
+#pragma unroll
+    for (int i = 0; i < V; i++) v[i] = ls != nullptr ? ls[m + i] * v[i] : v[i];
+    if (V == 4) {
+        const float4 o = *(const float4*)y;
+        *(float4*)y = make_float4(o.x + v[0], o.y + v[V > 1 ? 1 : 0], o.z + v[V > 1 ? 2 : 0], o.w + v[V > 1 ? 3 : 0]);
+    } else {
+        y[0] += v[0];
+    }
 }
 
 int launch_combine(const float* ws, const float* w, const float* ls, float* Y, int ldy, int M, const lt_dn_choice& c, cudaStream_t s) {
-    k_combine<<<dim3(c.T, (M + 255) / 256), 256, 0, s>>>(ws, w, ls, Y, ldy, M, c);
+    if (M % 4 == 0 && ldy % 4 == 0 && aligned16(ws) && aligned16(Y))
+        k_combine<4><<<dim3(c.T, (M + 1023) / 1024), 256, 0, s>>>(ws, w, ls, Y, ldy, M, c);
+    else
+        k_combine<1><<<dim3(c.T, (M + 255) / 256), 256, 0, s>>>(ws, w, ls, Y, ldy, M, c);
     return check_launch("lt_dn_experts_sum");
 }
 
