@@ -246,6 +246,12 @@ typedef struct {
 int lt_dn_delta_rows(const void* q, const void* k, const void* v, int ld, const float* la, const float* beta, int ldh, float* o, int ldo,
                      int f32, const lt_dn_delta* h_d, const lt_dn_seqs* h_q, void* stream);
 
+/* The same in chunks of 64 tokens on the tensor cores (bf16 only; dp <= 256, dvp <= 512; sums as exact as in token order).  ws: fp32
+ * workspace of lt_dn_delta_chunked_ws elements. */
+long lt_dn_delta_chunked_ws(const lt_dn_delta* h_d, const lt_dn_seqs* h_q);
+int lt_dn_delta_chunked(const void* q, const void* k, const void* v, int ld, const float* la, const float* beta, int ldh, float* o, int ldo,
+                        const lt_dn_delta* h_d, const lt_dn_seqs* h_q, float* ws, void* stream);
+
 /* One token at position *len (then *len += 1): convolution, silu, step size la = A softplus(dt + dt_bias) and recurrence in one
  * launch.  vkq: one row, values (H*dvp), keys (G*dp), queries (G*dp), ahead of the convolution, whose last inputs are in the ring
  * as in lt_dn_ssd_rows.  dt, beta [H]; o [H*dvp] fp32.  ticket: one int of the sequence, zero between launches. */

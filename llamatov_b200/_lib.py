@@ -173,6 +173,7 @@ DENSE_SIGNATURES = {
     "lt_dn_gqa_rows": [_vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, ctypes.POINTER(DnGqa), _vp],
     "lt_dn_gqa_attn": [_vp, _i, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, ctypes.POINTER(DnGqa), _vp],
     "lt_dn_delta_rows": [_vp, _vp, _vp, _i, _vp, _vp, _i, _vp, _i, _i, ctypes.POINTER(DnDelta), ctypes.POINTER(DnSeqs), _vp],
+    "lt_dn_delta_chunked": [_vp, _vp, _vp, _i, _vp, _vp, _i, _vp, _i, ctypes.POINTER(DnDelta), ctypes.POINTER(DnSeqs), _vp, _vp],
     "lt_dn_delta_step": [_vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, ctypes.POINTER(DnDelta), _vp],
     "lt_dn_route": [_vp, _i, _vp, _vp, _i, ctypes.POINTER(DnRouter), _vp],
     "lt_dn_experts_plan": [_vp, _i, _i, _i, _vp, _vp],
@@ -183,6 +184,7 @@ DENSE_SIGNATURES = {
 _DENSE_QUERIES = {"lt_dn_gqa_step_ws": ([_i, _i, _i], ctypes.c_long),
                   "lt_dn_gqa_step_tickets": ([_i, _i], _i),
                   "lt_dn_latent_step_ws": ([_i, _i, _i, _i], ctypes.c_long),
+                  "lt_dn_delta_chunked_ws": ([ctypes.POINTER(DnDelta), ctypes.POINTER(DnSeqs)], ctypes.c_long),
                   "lt_dn_experts_plan_ints": ([_i, _i, _i], ctypes.c_long),
                   "lt_dn_experts_sum_ws": ([_i, _i, _i], ctypes.c_long),
                   "lt_dn_recurrence_chunked_ws": ([_i, _i, _i, _i], ctypes.c_long)}

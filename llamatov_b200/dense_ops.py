@@ -211,6 +211,9 @@ class Experts:
 
 # --------------------------------------------------------------------------- delta rule
 
+DELTA_CHUNKED_FROM = 64         # tokens of the longest sequence from which on bf16 rows are walked in chunks
+
+
 class DeltaRule:
     """Gated delta rule of H heads on G key heads: rows() over the rows of sequences, step() for one token with its convolution
     (taps, conv, conv_b, dt_bias and A as in lt_dn_delta, on the device).  dim and vdim are the padded sizes."""
@@ -236,7 +239,12 @@ class DeltaRule:
             for j, r in enumerate(part):
                 seqs.start[j], seqs.rows[j], seqs.S[j] = at, r, states[i + j]
                 at += r
-            _lib.call("lt_dn_delta_rows", q, k, v, ld, la, beta, ldh, o, ldo, self.f32, self._ref, ctypes.byref(seqs), dr._stream())
+            args = (q, k, v, ld, la, beta, ldh, o, ldo)
+            if self.f32 or max(part) < DELTA_CHUNKED_FROM or self.dim > 256 or self.vdim > 512:
+                _lib.call("lt_dn_delta_rows", *args, self.f32, self._ref, ctypes.byref(seqs), dr._stream())
+                continue
+            ws = torch.empty(_lib.dense().lt_dn_delta_chunked_ws(self._ref, ctypes.byref(seqs)), dtype=torch.float32, device="cuda")
+            _lib.call("lt_dn_delta_chunked", *args, self._ref, ctypes.byref(seqs), ws.data_ptr(), dr._stream())
 
     def step(self, row, dt, beta, ring, S, o, len_, ticket):
         _lib.call("lt_dn_delta_step", row, dt, beta, ring, S, o, self.f32, len_, ticket, self._ref, dr._stream())

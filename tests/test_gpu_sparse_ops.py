@@ -4,6 +4,8 @@ can go wrong.
 Tolerances.  fp32 sums of n products of unit variance are off by at most n 2^-24 of their absolute values and by about sqrt(n) 2^-24
 as a rule; tests allow 8 sqrt(n) 2^-24 of the outputs' size, and half a step (2^-9 of the power of two below, so 2^-8 of the value at
 most) for a result that is rounded to bf16."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -350,33 +352,45 @@ DELTA = [  # lengths, H, G, d, dv
     ([200], 2, 1, 136, 8), ([7] * 8, 2, 2, 8, 136), ([3] * 11, 1, 1, 32, 32), ([130, 1], 2, 2, 264, 16), ([5, 40], 1, 1, 512, 24), ([333], 3, 3, 72, 48)]
 
 
-@pytest.mark.parametrize("f32", [0, 1])
+@pytest.fixture(params=["order", "order-f32", "chunks"])
+def walk(request, monkeypatch):
+    """Token order in both types, and chunks, whatever the number of rows: the value is f32."""
+    monkeypatch.setattr(P, "DELTA_CHUNKED_FROM", 1 if request.param == "chunks" else 10 ** 9)
+    return int(request.param == "order-f32")
+
+
 @pytest.mark.parametrize("lengths,H,G,d,dv", DELTA)
-def test_delta_rows(f32, lengths, H, G, d, dv):
+def test_delta_rows(walk, lengths, H, G, d, dv):
+    f32 = walk
     for strong in (False, True):
         rows, la, beta, S = _delta_case(lengths, H, G, d, dv, f32, seed=len(lengths) + d, strong=strong)
         eo, eS = _delta_run(rows, la, beta, S, lengths, H, G, d, dv, f32)
         assert eo <= _delta_tol(max(lengths)) and eS <= _delta_tol(max(lengths)), (eo, eS)
 
 
-@pytest.mark.parametrize("f32", [0, 1])
-def test_delta_rows_between_other_rows(f32):
+@pytest.mark.parametrize("chunks,f32", [(0, 0), (0, 1), (1, 0)])
+def test_delta_rows_between_other_rows(chunks, f32):
     lengths, H, G, d, dv = [5, 0, 70], 4, 2, 24, 40
 
     def call(op, q, k, v, ld, la, beta, o, seqs):
-        import ctypes
-        _lib.call("lt_dn_delta_rows", q, k, v, ld, la.data_ptr(), beta.data_ptr(), H, o.data_ptr(), H * dv + 2, f32, op._ref, ctypes.byref(seqs), stream())
+        args = (q, k, v, ld, la.data_ptr(), beta.data_ptr(), H, o.data_ptr(), H * dv + 2)
+        if not chunks:
+            _lib.call("lt_dn_delta_rows", *args, f32, op._ref, ctypes.byref(seqs), stream())
+            return
+        n = _lib.dense().lt_dn_delta_chunked_ws(op._ref, ctypes.byref(seqs))
+        ws = torch.full((n + 4,), float("nan"), device="cuda")
+        _lib.call("lt_dn_delta_chunked", *args, op._ref, ctypes.byref(seqs), ws.data_ptr(), stream())
+        assert torch.isnan(ws[n:]).all()
     rows, la, beta, S = _delta_case(lengths, H, G, d, dv, f32, seed=4, gap=3)
     eo, eS = _delta_run(rows, la, beta, S, lengths, H, G, d, dv, f32, gap=3, call=call)
     assert eo <= _delta_tol(70) and eS <= _delta_tol(70)
 
 
-@pytest.mark.parametrize("f32", [0, 1])
 @pytest.mark.parametrize("T", [3, 150])
-def test_delta_extremes(f32, T):
+def test_delta_extremes(walk, T):
     """Nothing written (beta 0), everything forgotten (la minus infinity), no decay, zero keys and queries, full corrections with
     keys that repeat, a growing state."""
-    H, G, d, dv = 6, 6, 32, 24
+    f32, H, G, d, dv = walk, 6, 6, 32, 24
     rows, la, beta, S = _delta_case([T], H, G, d, dv, f32, seed=9)
     la[:, 1:] = 0.0
     la[:, 0] = -float("inf")

@@ -91,6 +91,16 @@ def test_delta_refusals():
     rows("share rows", q=seqs((0, 5, 256), (4, 5, 512)))
     rows("ldh=3", ldh=3)
     rows("ldo=95", ldo=95)
+    chunked = lambda text, d=delta(), q=seqs((0, 5, 256)), k=one, ld=96, ldo=96, ws=one: _refused(
+        "lt_dn_delta_chunked", text, one, k, one, ld, one, one, 4, one, ldo, d, q, ws, None)
+    chunked("above 256", delta(dp=264))
+    chunked("above 256", delta(dvp=520))
+    chunked("alignment", k=ctypes.c_void_p(258))
+    chunked("alignment", ld=100)
+    chunked("alignment", ldo=97)
+    chunked("null pointer", ws=None)
+    chunked("one state", q=seqs((0, 5, 256), (5, 5, 256)))
+    assert _lib.dense().lt_dn_delta_chunked_ws(delta(), seqs((0, 65, 256), (65, 0, 512))) == 2 * 4 * (3 * 64 * 64 // 2 + 132 + 24 * 16 + 24 * 64)
     step = lambda text, d=delta(), S=one: _refused("lt_dn_delta_step", text, one, one, one, one, S, one, 0, one, one, d, None)
     step("taps=0", delta(taps=0))
     step("null constants", delta(conv=None))
