@@ -90,33 +90,39 @@ __device__ __forceinline__ void load_rows(bf16* dst, int stride, int units, cons
         cp16(dst + t * stride + x, src + (ok ? (c.row0 + t) * ld + col + x : 0), ok);
     }
 }
-// 1 / |row| of 64 rows, a warp per row
-__device__ __forceinline__ void row_norms(const bf16* s, int stride, int width, float eps, float scale, float* out) {
-    const int lane = threadIdx.x & 31;
-    for (int t = threadIdx.x >> 5; t < DC; t += blockDim.x >> 5) {
+// scale / |row| of 64 rows, eight lanes per row
+__device__ __forceinline__ void row_norms(const bf16* s, int stride, int units, float eps, float scale, float* out) {
+    const int sub = threadIdx.x & 7;
+    for (int t = threadIdx.x >> 3; t < DC; t += blockDim.x >> 3) {
         float a = 0.0f;
-        for (int x = 2 * lane; x < width; x += 64) {
-            const unsigned w = *(const unsigned*)(s + t * stride + x);
-            a = fmaf(lo_f(w), lo_f(w), fmaf(hi_f(w), hi_f(w), a));
+        for (int x = sub; x < units; x += 8) {
+            float f[8];
+            Vec<bf16>::unpack(*(const uint4*)(s + t * stride + x * 8), f);
+#pragma unroll
+            for (int i = 0; i < 8; i++) a = fmaf(f[i], f[i], a);
         }
-        a = warp_sum(a);
-        if (lane == 0) out[t] = scale / sqrtf(a + eps);
+        a += __shfl_xor_sync(0xffffffffu, a, 1);
+        a += __shfl_xor_sync(0xffffffffu, a, 2);
+        a += __shfl_xor_sync(0xffffffffu, a, 4);
+        if (sub == 0) out[t] = scale / sqrtf(a + eps);
     }
 }
 
 // ---------------------------------------------------------------------------- T of every chunk
 
 constexpr int MS = DC + 4;       // row stride of fp32 tiles
+constexpr int PREP_THREADS = 256;
 
-__global__ void __launch_bounds__(128) k_delta_prep(const __grid_constant__ DeltaChunkP P) {
+// I + A is inverted in place: diagonal blocks of 16 by forward substitution, a column per lane, then the blocks below them,
+// X21 = -X22 (A21 X11), first of 16, then of 32.
+__global__ void __launch_bounds__(PREP_THREADS) k_delta_prep(const __grid_constant__ DeltaChunkP P) {
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ __align__(16) double sb[DC];
-    __shared__ float sr[DC], sbeta[DC];
+    __shared__ __align__(16) float sr[DC], sbeta[DC];
     const int dpr = (P.D.dp + 31) & ~31, KS = dpr + 8;
-    float* sA = (float*)smem;                 // A, strictly below the diagonal
-    float* sX = sA + DC * MS;                 // its inverse
-    float* sT = sX + DC * MS;                 // [32][32 + 4]
-    bf16* sk = (bf16*)(sT + 32 * 36);
+    float* sA = (float*)smem;                 // [64][MS]
+    bf16* sk = (bf16*)(sA + DC * MS);
+    float* sT = (float*)sk;                   // [32][36], once the keys are used
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tg = lane & 3;
     const int h = blockIdx.y, hq = h / (P.D.H / P.D.G);
     const Chunk c = chunk_of(P, blockIdx.x);
@@ -124,35 +130,38 @@ __global__ void __launch_bounds__(128) k_delta_prep(const __grid_constant__ Delt
     load_rows(sk, KS, dpr / 8, P.k, c, P.ld, hq * P.D.dp, P.D.dp);
     asm volatile("cp.async.commit_group;" ::: "memory");
     if (warp == 0) log_sums(P, c, h, lane, sb);
-    if (tid >= 64) sbeta[tid - 64] = tid - 64 < c.rows ? P.beta[(c.row0 + tid - 64) * P.ldh + h] : 0.0f;
+    if (tid >= 64 && tid < 128) sbeta[tid - 64] = tid - 64 < c.rows ? P.beta[(c.row0 + tid - 64) * P.ldh + h] : 0.0f;
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
-    row_norms(sk, KS, dpr, P.D.eps, 1.0f, sr);
-    __syncthreads();
-    {   // k_i . k_j: rows 16 warp + g (+ 8), columns 8 n + 2 tg (+ 1) up to the diagonal
-        float a[8][4];
+    row_norms(sk, KS, dpr / 8, P.D.eps, 1.0f, sr);
+    const int m = warp & 3;      // k_i . k_j: rows 16 m + g (+ 8), columns 16 n + 2 tg (+ 1, + 8, + 9) of every other n up to m
+    float a[2][2][4];
 #pragma unroll
-        for (int n = 0; n < 8; n++) a[n][0] = a[n][1] = a[n][2] = a[n][3] = 0.0f;
-        for (int kk = 0; kk < dpr / 16; kk++) {
-            unsigned x[4];
-            ldsm4(x, sk + (warp * 16 + (lane & 15)) * KS + kk * 16 + (lane >> 4) * 8);
+    for (int n = 0; n < 2; n++)
 #pragma unroll
-            for (int n = 0; n < 8; n += 2) {
-                if (n > 2 * warp) break;
-                unsigned r[4];
-                ldsm4(r, sk + (n * 8 + (lane & 7) + ((lane >> 4) << 3)) * KS + kk * 16 + ((lane >> 3) & 1) * 8);
-                mma16816(a[n], x, r[0], r[1]);
-                mma16816(a[n + 1], x, r[2], r[3]);
-            }
+        for (int e = 0; e < 4; e++) a[n][0][e] = a[n][1][e] = 0.0f;
+    for (int kk = 0; kk < dpr / 16; kk++) {
+        unsigned x[4];
+        ldsm4(x, sk + (m * 16 + (lane & 15)) * KS + kk * 16 + (lane >> 4) * 8);
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
+            const int col = 2 * n + (warp >> 2);
+            if (col > m) break;
+            unsigned r[4];
+            ldsm4(r, sk + (col * 16 + (lane & 7) + ((lane >> 4) << 3)) * KS + kk * 16 + ((lane >> 3) & 1) * 8);
+            mma16816(a[n][0], x, r[0], r[1]);
+            mma16816(a[n][1], x, r[2], r[3]);
         }
+    }
+    __syncthreads();
 #pragma unroll
-        for (int n = 0; n < 8; n++) {
-            if (n > 2 * warp + 1) break;
+    for (int n = 0; n < 2; n++) {
+        const int col = 2 * n + (warp >> 2);
+        if (col > m) break;
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int i = warp * 16 + g + (e >> 1) * 8, j = n * 8 + 2 * tg + (e & 1);
-                sA[i * MS + j] = j < i ? a[n][e] * sbeta[i] * sr[i] * sr[j] * exp2f((float)(sb[i] - sb[j])) : 0.0f;
-            }
+        for (int e = 0; e < 8; e++) {
+            const int i = m * 16 + g + ((e >> 1) & 1) * 8, j = col * 16 + (e >> 2) * 8 + 2 * tg + (e & 1);
+            sA[i * MS + j] = j < i ? a[n][e >> 2][e & 3] * sbeta[i] * sr[i] * sr[j] * exp2f((float)(sb[i] - sb[j])) : 0.0f;
         }
     }
     if (tid < DC) {
@@ -162,88 +171,82 @@ __global__ void __launch_bounds__(128) k_delta_prep(const __grid_constant__ Delt
         if (tid == 0) vec[2 * DC] = exp2f((float)sb[DC - 1]);
     }
     __syncthreads();
-    if (lane < 16) {         // inverse of a diagonal block of 16, a column per lane
-        const float* a = sA + warp * 16 * MS + warp * 16;
+    if (warp < 4 && lane < 16) {
+        float* d = sA + warp * 16 * MS + warp * 16;
         float x[16];
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            float s = i == lane ? 1.0f : 0.0f;
+        for (int i = 0; i < 16; i++) x[i] = i == lane ? 1.0f : 0.0f;
 #pragma unroll
-            for (int k = 0; k < 16; k++)
-                if (k < i) s = fmaf(-a[i * MS + k], x[k], s);
-            x[i] = s;
-            sX[(warp * 16 + i) * MS + warp * 16 + lane] = s;
+        for (int k = 0; k < 15; k++)
+#pragma unroll
+            for (int i = k + 1; i < 16; i++) x[i] = fmaf(-d[i * MS + k], x[k], x[i]);
+        __syncwarp(0xffffu);
+#pragma unroll
+        for (int i = 0; i < 16; i++) d[i * MS + lane] = x[i];
+    }
+    __syncthreads();
+    {
+        const int p = tid >> 7, i = (tid >> 3) & 15, j = (tid & 7) * 2, r = 32 * p + 16 + i, q = 32 * p;
+        float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 16; k++) {
+            const float x = sA[r * MS + q + k];
+            const float2 y = *(const float2*)(sA + (q + k) * MS + q + j);
+            s0 = fmaf(x, y.x, s0);
+            s1 = fmaf(x, y.y, s1);
         }
-    }
-    __syncthreads();
-    // blocks below: X21 = -X22 (A21 X11), first of 16, then of 32
+        *(float2*)(sT + (p * 16 + i) * 36 + j) = make_float2(s0, s1);
+        __syncthreads();
+        s0 = s1 = 0.0f;
 #pragma unroll
-    for (int e = tid; e < 512; e += 128) {
-        const int p = e >> 8, i = (e >> 4) & 15, j = e & 15, r = 32 * p + 16 + i, q = 32 * p;
-        float s = 0.0f;
-#pragma unroll
-        for (int k = 0; k < 16; k++) s = fmaf(sA[r * MS + q + k], sX[(q + k) * MS + q + j], s);       // X11 is zero above its diagonal
-        sT[(p * 16 + i) * 36 + j] = s;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int e = tid; e < 512; e += 128) {
-        const int p = e >> 8, i = (e >> 4) & 15, j = e & 15, r = 32 * p + 16 + i, q = 32 * p;
-        float s = 0.0f;
-#pragma unroll
-        for (int k = 0; k < 16; k++) s = fmaf(-sX[r * MS + q + 16 + k], sT[(p * 16 + k) * 36 + j], s);
-        sX[r * MS + q + j] = s;
-        sX[(q + i) * MS + q + 16 + j] = 0.0f;
-    }
-    __syncthreads();
-    const int i0 = (tid >> 3) * 2, j0 = (tid & 7) * 4;       // 2 x 4 of 32 x 32
-    float s[2][4];
-#pragma unroll
-    for (int i = 0; i < 2; i++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) s[i][j] = 0.0f;
-#pragma unroll 8
-    for (int k = 0; k < 32; k++) {
-        const float4 x = *(const float4*)(sX + k * MS + j0);
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const float a = sA[(32 + i0 + i) * MS + k];
-            s[i][0] = fmaf(a, x.x, s[i][0]); s[i][1] = fmaf(a, x.y, s[i][1]); s[i][2] = fmaf(a, x.z, s[i][2]); s[i][3] = fmaf(a, x.w, s[i][3]);
+        for (int k = 0; k < 16; k++) {
+            const float x = -sA[r * MS + q + 16 + k];
+            const float2 y = *(const float2*)(sT + (p * 16 + k) * 36 + j);
+            s0 = fmaf(x, y.x, s0);
+            s1 = fmaf(x, y.y, s1);
         }
+        *(float2*)(sA + r * MS + q + j) = make_float2(s0, s1);
+        *(float2*)(sA + (q + i) * MS + q + 16 + j) = make_float2(0, 0);
     }
-#pragma unroll
-    for (int i = 0; i < 2; i++) *(float4*)(sT + (i0 + i) * 36 + j0) = make_float4(s[i][0], s[i][1], s[i][2], s[i][3]);
     __syncthreads();
+    {
+        const int i = tid >> 3, j = (tid & 7) * 4;
+        float4 s = make_float4(0, 0, 0, 0);
 #pragma unroll
-    for (int i = 0; i < 2; i++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) s[i][j] = 0.0f;
-#pragma unroll 8
-    for (int k = 0; k < 32; k++) {
-        const float4 x = *(const float4*)(sT + k * 36 + j0);
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const float a = -sX[(32 + i0 + i) * MS + 32 + k];
-            s[i][0] = fmaf(a, x.x, s[i][0]); s[i][1] = fmaf(a, x.y, s[i][1]); s[i][2] = fmaf(a, x.z, s[i][2]); s[i][3] = fmaf(a, x.w, s[i][3]);
+        for (int k = 0; k < 32; k++) {
+            const float x = sA[(32 + i) * MS + k];
+            const float4 y = *(const float4*)(sA + k * MS + j);
+            s.x = fmaf(x, y.x, s.x); s.y = fmaf(x, y.y, s.y); s.z = fmaf(x, y.z, s.z); s.w = fmaf(x, y.w, s.w);
         }
-    }
+        *(float4*)(sT + i * 36 + j) = s;
+        __syncthreads();
+        s = make_float4(0, 0, 0, 0);
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-        *(float4*)(sX + (32 + i0 + i) * MS + j0) = make_float4(s[i][0], s[i][1], s[i][2], s[i][3]);
-        *(float4*)(sX + (i0 + i) * MS + 32 + j0) = make_float4(0, 0, 0, 0);
+        for (int k = 0; k < 32; k++) {
+            const float x = -sA[(32 + i) * MS + 32 + k];
+            const float4 y = *(const float4*)(sT + k * 36 + j);
+            s.x = fmaf(x, y.x, s.x); s.y = fmaf(x, y.y, s.y); s.z = fmaf(x, y.z, s.z); s.w = fmaf(x, y.w, s.w);
+        }
+        *(float4*)(sA + (32 + i) * MS + j) = s;
+        *(float4*)(sA + i * MS + 32 + j) = make_float4(0, 0, 0, 0);
     }
     __syncthreads();
     bf16* out = P.T3 + at * 3 * DC * DC;
-    for (int e = tid; e < DC * DC / 4; e += 128) {
+#pragma unroll
+    for (int e = tid; e < DC * DC / 4; e += PREP_THREADS) {
         const int i = e >> 4, j = (e & 15) * 4;
-        const float4 x = *(const float4*)(sX + i * MS + j), be = *(const float4*)(sbeta + j);
-        uint2 a, b, d;
-        split3(x.x * be.x, x.y * be.y, a.x, b.x, d.x);
-        split3(x.z * be.z, x.w * be.w, a.y, b.y, d.y);
-        *(uint2*)(out + i * DC + j) = a;
-        *(uint2*)(out + DC * DC + i * DC + j) = b;
-        *(uint2*)(out + 2 * DC * DC + i * DC + j) = d;
+        const float4 x = *(const float4*)(sA + i * MS + j), be = *(const float4*)(sbeta + j);
+        uint2 t0, t1, t2;
+        split3(x.x * be.x, x.y * be.y, t0.x, t1.x, t2.x);
+        split3(x.z * be.z, x.w * be.w, t0.y, t1.y, t2.y);
+        *(uint2*)(out + i * DC + j) = t0;
+        *(uint2*)(out + DC * DC + i * DC + j) = t1;
+        *(uint2*)(out + 2 * DC * DC + i * DC + j) = t2;
     }
+}
+static size_t prep_smem(int dp) {
+    const size_t keys = (size_t)DC * (((dp + 31) & ~31) + 8) * 2, T = 32 * 36 * 4;
+    return (size_t)DC * MS * 4 + (keys > T ? keys : T);
 }
 
 // ---------------------------------------------------------------------------- states
@@ -275,65 +278,83 @@ __global__ void __launch_bounds__(NW * 32) k_delta_states(const __grid_constant_
     const int cw = warp * 16 * KT;
     const int va = v0 + g, vb = va + 8;
 
-    auto load = [&](int chunk) {
-        if (chunk < nchunk) {
-            unsigned char* st = smem + (chunk % L::STAGES) * L::STAGE;
-            bf16* sk = (bf16*)st;
-            bf16* sT = (bf16*)(st + L::K_B);
-            bf16* sv = (bf16*)(st + L::K_B + L::T_B);
-            float* sc = (float*)(st + L::K_B + L::T_B + L::V_B);
-            const int rows = P.Q.rows[b] - chunk * DC;
-            const long r0 = (long)P.Q.start[b] + chunk * DC;
-            const long at = (long)(P.first[b] + chunk) * P.D.H + h;
+    // this thread's 16-byte units of a stage: one column of the keys, one of T, one of the values; pointers go on by chunks
+    constexpr int KU = L::DPR / 8, KR = THREADS / KU;        // units of a row of keys, rows of them at a time
+    const int kt_ = tid / KU, kx = (tid % KU) * 8, tt = tid >> 3, tx = (tid & 7) * 8, vt = tid >> 1, vx = (tid & 1) * 8;
+    const bool k_ok = kx < dp, v_ok = tid < 2 * DC && v0 + vx < dvp;
+    const bf16* kp = P.k + ((long)P.Q.start[b] + kt_) * P.ld + (long)hq * dp + kx;
+    const bf16* vp = P.v + ((long)P.Q.start[b] + vt) * P.ld + (long)h * dvp + v0 + vx;
+    const long at0 = (long)P.first[b] * P.D.H + h;
+    const bf16* tp = P.T3 + at0 * 3 * DC * DC + tid * 8;
+    const float* cp = P.vec + at0 * DVEC + tid * 4;
+    int left = P.Q.rows[b], next = 0;         // rows not yet asked for, chunk that is asked for next
+    auto load = [&]() {
+        if (next < nchunk) {
+            unsigned char* st = smem + (next % L::STAGES) * L::STAGE;
+            bf16* sk = (bf16*)st + kt_ * KS + kx;
+            bf16* sT = (bf16*)(st + L::K_B) + tt * TS + tx;
 #pragma unroll
-            for (int e = tid; e < DC * (L::DPR / 8); e += THREADS) {
-                const int t = e / (L::DPR / 8), x = (e - t * (L::DPR / 8)) * 8;
-                const bool ok = t < rows && x < dp;
-                cp16(sk + t * KS + x, P.k + (ok ? (r0 + t) * P.ld + (long)hq * dp + x : 0), ok);
+            for (int i = 0; i < DC / KR; i++) {
+                const bool ok = k_ok && kt_ + i * KR < left;
+                cp16(sk + i * KR * KS, ok ? kp + (long)i * KR * P.ld : P.k, ok);
             }
-            const bf16* T3 = P.T3 + at * 3 * DC * DC;
 #pragma unroll
-            for (int e = tid; e < 3 * DC * 8; e += THREADS) cp16(sT + (e >> 3) * TS + (e & 7) * 8, T3 + e * 8, true);
-            for (int e = tid; e < DC * 2; e += THREADS) {
-                const int t = e >> 1, x = (e & 1) * 8;
-                const bool ok = t < rows && v0 + x < dvp;
-                cp16(sv + t * L::VS + x, P.v + (ok ? (r0 + t) * P.ld + (long)h * dvp + v0 + x : 0), ok);
+            for (int i = 0; i < 3 * DC * 8 / THREADS; i++) cp16(sT + i * (THREADS / 8) * TS, tp + i * THREADS * 8, true);
+            if (tid < 2 * DC) {
+                const bool ok = v_ok && vt < left;
+                cp16((bf16*)(st + L::K_B + L::T_B) + vt * L::VS + vx, ok ? vp : P.v, ok);
             }
-            if (tid < DVEC / 4) cp16(sc + tid * 4, P.vec + at * DVEC + tid * 4, true);
+            if (tid < DVEC / 4) cp16((float*)(st + L::K_B + L::T_B + L::V_B) + tid * 4, cp, true);
+            kp += (long)DC * P.ld;
+            vp += (long)DC * P.ld;
+            tp += (long)P.D.H * 3 * DC * DC;
+            cp += (long)P.D.H * DVEC;
+            left -= DC;
+            next++;
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
 
     float s[2 * KT][4];              // S[va or vb][cw + 8 i + 2 tg + (0, 1)]
+    const long sa = (long)va * dp + cw + 2 * tg, sd = (long)vb * dp + cw + 2 * tg;
+    const bool a_ok = va < dvp, b_ok = vb < dvp;
     float* S = P.Q.S[b] + (long)h * dvp * dp;
 #pragma unroll
     for (int i = 0; i < 2 * KT; i++) {
-        const int c = cw + i * 8 + tg * 2;
         float2 a = make_float2(0, 0), d = a;
-        if (c < dp && va < dvp) a = *(const float2*)(S + (long)va * dp + c);
-        if (c < dp && vb < dvp) d = *(const float2*)(S + (long)vb * dp + c);
+        if (cw + 8 * i < dp && a_ok) a = *(const float2*)(S + sa + 8 * i);
+        if (cw + 8 * i < dp && b_ok) d = *(const float2*)(S + sd + 8 * i);
         s[i][0] = a.x; s[i][1] = a.y; s[i][2] = d.x; s[i][3] = d.y;
     }
     auto keep = [&](float* to) {
 #pragma unroll
         for (int i = 0; i < 2 * KT; i++) {
-            const int c = cw + i * 8 + tg * 2;
-            if (c < dp && va < dvp) *(float2*)(to + (long)va * dp + c) = make_float2(s[i][0], s[i][1]);
-            if (c < dp && vb < dvp) *(float2*)(to + (long)vb * dp + c) = make_float2(s[i][2], s[i][3]);
+            if (cw + 8 * i < dp && a_ok) *(float2*)(to + sa + 8 * i) = make_float2(s[i][0], s[i][1]);
+            if (cw + 8 * i < dp && b_ok) *(float2*)(to + sd + 8 * i) = make_float2(s[i][2], s[i][3]);
         }
     };
+    // operands that do not wait for the state are read ahead of the barrier that the state's own share waits at
+    auto keys = [&](unsigned (&r)[KT][4][4], const bf16* sk) {
 #pragma unroll
-    for (int i = 0; i < L::STAGES - 1; i++) load(i);
+        for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+            for (int n = 0; n < 4; n++)
+                ldsm4(r[kt][n], sk + (n * 16 + (lane & 7) + ((lane >> 4) << 3)) * KS + cw + kt * 16 + ((lane >> 3) & 1) * 8);
+    };
+#pragma unroll
+    for (int i = 0; i < L::STAGES - 1; i++) load();
     asm volatile("cp.async.wait_group %0;" ::"n"(L::STAGES - 2) : "memory");
     __syncthreads();
+    unsigned kf[KT][4][4];
+    keys(kf, (const bf16*)smem);
+    float* S0 = P.S0 + at0 * dvp * dp;
+    float* U = P.U + at0 * dvp * DC;
     for (int chunk = 0; chunk < nchunk; chunk++) {
         const unsigned char* st = smem + (chunk % L::STAGES) * L::STAGE;
         const bf16* sk = (const bf16*)st;
         const bf16* sT = (const bf16*)(st + L::K_B);
         const bf16* sv = (const bf16*)(st + L::K_B + L::T_B);
         const float* sc = (const float*)(st + L::K_B + L::T_B + L::V_B);
-        const long at = (long)(P.first[b] + chunk) * P.D.H + h;
-        keep(P.S0 + at * dvp * dp);
         if (warp < active) {         // this warp's share of (K S^T)^T
             float y[8][4];
 #pragma unroll
@@ -346,15 +367,12 @@ __global__ void __launch_bounds__(NW * 32) k_delta_states(const __grid_constant_
                 split3(s[2 * kt + 1][0], s[2 * kt + 1][1], a[0][2], a[1][2], a[2][2]);
                 split3(s[2 * kt + 1][2], s[2 * kt + 1][3], a[0][3], a[1][3], a[2][3]);
 #pragma unroll
-                for (int n = 0; n < 8; n += 2) {
-                    unsigned r[4];
-                    ldsm4(r, sk + (n * 8 + (lane & 7) + ((lane >> 4) << 3)) * KS + cw + kt * 16 + ((lane >> 3) & 1) * 8);
+                for (int p = 2; p >= 0; p--)
 #pragma unroll
-                    for (int p = 2; p >= 0; p--) {
-                        mma16816(y[n], a[p], r[0], r[1]);
-                        mma16816(y[n + 1], a[p], r[2], r[3]);
+                    for (int n = 0; n < 4; n++) {
+                        mma16816(y[2 * n], a[p], kf[kt][n][0], kf[kt][n][1]);
+                        mma16816(y[2 * n + 1], a[p], kf[kt][n][2], kf[kt][n][3]);
                     }
-                }
             }
             float* o = sY + (warp * 16 + g) * L::YS + 2 * tg;
 #pragma unroll
@@ -363,16 +381,20 @@ __global__ void __launch_bounds__(NW * 32) k_delta_states(const __grid_constant_
                 *(float2*)(o + 8 * L::YS + 8 * n) = make_float2(y[n][2], y[n][3]);
             }
         }
+        keep(S0);
+        S0 += (long)P.D.H * dvp * dp;
         __syncthreads();             // shares are there; nobody works on the chunk before
-        load(chunk + L::STAGES - 1);
+        load();
 #pragma unroll
         for (int e = tid; e < 256; e += THREADS) {       // X = V - e^b r (K S^T), transposed
             const int v = e >> 4, t = (e & 15) * 4;
             float4 y = *(const float4*)(sY + v * L::YS + t);
-            for (int w = 1; w < active; w++) {
-                const float4 z = *(const float4*)(sY + (w * 16 + v) * L::YS + t);
-                y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
-            }
+#pragma unroll
+            for (int w = 1; w < NW; w++)
+                if (w < active) {
+                    const float4 z = *(const float4*)(sY + (w * 16 + v) * L::YS + t);
+                    y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
+                }
             const float4 f = *(const float4*)(sc + t);
             uint2 a, d, l;
             split3(fmaf(-f.x, y.x, to_f(sv[t * L::VS + v])), fmaf(-f.y, y.y, to_f(sv[(t + 1) * L::VS + v])), a.x, d.x, l.x);
@@ -381,42 +403,43 @@ __global__ void __launch_bounds__(NW * 32) k_delta_states(const __grid_constant_
             *(uint2*)(sXp + (16 + v) * TS + t) = d;
             *(uint2*)(sXp + (32 + v) * TS + t) = l;
         }
-        __syncthreads();
+        unsigned kb[4][KT][4];       // the keys again, as rows of tokens
 #pragma unroll
-        for (int u = 0; u < 8 / NW; u++) {       // U^T = X^T T^T: tokens 8 i ..
-            const int i = u == 0 ? warp : 7 - warp;
-            float d[3][4];
+        for (int kk = 0; kk < 4; kk++)
 #pragma unroll
-            for (int p = 0; p < 3; p++) d[p][0] = d[p][1] = d[p][2] = d[p][3] = 0.0f;
+            for (int i = 0; i < KT; i++) ldsm4t(kb[kk][i], sk + (kk * 16 + (lane & 15)) * KS + cw + i * 16 + (lane >> 4) * 8);
 #pragma unroll
-            for (int k2 = 0; k2 < 2; k2++) {     // 32 tokens of X at a time
-                if (4 * k2 > i) break;
-                unsigned tb[3][4];
+        for (int u = 0; u < 8 / NW; u++) {       // U^T = X^T T^T: tokens 8 i ..; warps that share a scheduler have as much together
+            const int i = NW == 8 ? (warp < 4 ? warp : 11 - warp) : (u == 0 ? warp : 7 - warp);
+            unsigned tb[3][2][4];
 #pragma unroll
-                for (int p = 0; p < 3; p++) ldsm4(tb[p], sT + (p * DC + i * 8 + (lane & 7)) * TS + k2 * 32 + (lane >> 3) * 8);
+            for (int p = 0; p < 3; p++)
 #pragma unroll
-                for (int k1 = 0; k1 < 2; k1++) {
-                    const int kt = 2 * k2 + k1;
-                    if (2 * kt > i) break;
-                    unsigned xa[3][4];
+                for (int k2 = 0; k2 < 2; k2++)
+                    if (4 * k2 <= i) ldsm4(tb[p][k2], sT + (p * DC + i * 8 + (lane & 7)) * TS + k2 * 32 + (lane >> 3) * 8);
+            if (u == 0) __syncthreads();         // X is there
+            float d[6][4];
 #pragma unroll
-                    for (int p = 0; p < 3; p++) ldsm4(xa[p], sXp + (p * 16 + (lane & 15)) * TS + kt * 16 + (lane >> 4) * 8);
-                    mma16816(d[2], xa[2], tb[0][2 * k1], tb[0][2 * k1 + 1]);
-                    mma16816(d[1], xa[1], tb[0][2 * k1], tb[0][2 * k1 + 1]);
-                    mma16816(d[0], xa[0], tb[0][2 * k1], tb[0][2 * k1 + 1]);
-                    mma16816(d[2], xa[0], tb[2][2 * k1], tb[2][2 * k1 + 1]);
-                    mma16816(d[1], xa[0], tb[1][2 * k1], tb[1][2 * k1 + 1]);
-                    mma16816(d[2], xa[1], tb[1][2 * k1], tb[1][2 * k1 + 1]);
-                }
+            for (int p = 0; p < 6; p++) d[p][0] = d[p][1] = d[p][2] = d[p][3] = 0.0f;
+#pragma unroll
+            for (int kt = 0; kt < 4; kt++) {
+                if (2 * kt > i) break;
+                unsigned xa[3][4];
+#pragma unroll
+                for (int p = 0; p < 3; p++) ldsm4(xa[p], sXp + (p * 16 + (lane & 15)) * TS + kt * 16 + (lane >> 4) * 8);
+                const int lo = 2 * (kt & 1);
+                mma16816(d[0], xa[0], tb[0][kt >> 1][lo], tb[0][kt >> 1][lo + 1]);
+                mma16816(d[1], xa[0], tb[1][kt >> 1][lo], tb[1][kt >> 1][lo + 1]);
+                mma16816(d[2], xa[1], tb[0][kt >> 1][lo], tb[0][kt >> 1][lo + 1]);
+                mma16816(d[3], xa[0], tb[2][kt >> 1][lo], tb[2][kt >> 1][lo + 1]);
+                mma16816(d[4], xa[1], tb[1][kt >> 1][lo], tb[1][kt >> 1][lo + 1]);
+                mma16816(d[5], xa[2], tb[0][kt >> 1][lo], tb[0][kt >> 1][lo + 1]);
             }
             const int t = i * 8 + 2 * tg;
+            const float2 z = *(const float2*)(sc + DC + t);
             float x[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) x[e] = d[0][e] + (d[1][e] + d[2][e]);
-            float* U = P.U + at * dvp * DC;
-            if (va < dvp) *(float2*)(U + (long)va * DC + t) = make_float2(x[0], x[1]);
-            if (vb < dvp) *(float2*)(U + (long)vb * DC + t) = make_float2(x[2], x[3]);
-            const float2 z = *(const float2*)(sc + DC + t);
+            for (int e = 0; e < 4; e++) x[e] = d[0][e] + ((d[1][e] + d[2][e]) + (d[3][e] + (d[4][e] + d[5][e])));
             unsigned a, m, l;
             split3(x[0] * z.x, x[1] * z.y, a, m, l);
             *(unsigned*)(sZp + g * TS + t) = a;
@@ -426,11 +449,15 @@ __global__ void __launch_bounds__(NW * 32) k_delta_states(const __grid_constant_
             *(unsigned*)(sZp + (8 + g) * TS + t) = a;
             *(unsigned*)(sZp + (24 + g) * TS + t) = m;
             *(unsigned*)(sZp + (40 + g) * TS + t) = l;
+            if (a_ok) *(float2*)(U + (long)va * DC + t) = make_float2(x[0], x[1]);
+            if (b_ok) *(float2*)(U + (long)vb * DC + t) = make_float2(x[2], x[3]);
         }
+        U += (long)P.D.H * dvp * DC;
+        const float end = sc[2 * DC];
         asm volatile("cp.async.wait_group %0;" ::"n"(L::STAGES - 2) : "memory");
         __syncthreads();             // Z is there, and the next chunk
+        if (chunk + 1 < nchunk) keys(kf, (const bf16*)(smem + ((chunk + 1) % L::STAGES) * L::STAGE));
         if (warp < active) {
-            const float end = sc[2 * DC];
             float d[3][2 * KT][4];
 #pragma unroll
             for (int p = 0; p < 3; p++)
@@ -442,15 +469,12 @@ __global__ void __launch_bounds__(NW * 32) k_delta_states(const __grid_constant_
 #pragma unroll
                 for (int p = 0; p < 3; p++) ldsm4(za[p], sZp + (p * 16 + (lane & 15)) * TS + kk * 16 + (lane >> 4) * 8);
 #pragma unroll
-                for (int i = 0; i < 2 * KT; i += 2) {
-                    unsigned r[4];
-                    ldsm4t(r, sk + (kk * 16 + (lane & 15)) * KS + cw + i * 8 + (lane >> 4) * 8);
+                for (int i = 0; i < KT; i++)
 #pragma unroll
                     for (int p = 0; p < 3; p++) {
-                        mma16816(d[p][i], za[p], r[0], r[1]);
-                        mma16816(d[p][i + 1], za[p], r[2], r[3]);
+                        mma16816(d[p][2 * i], za[p], kb[kk][i][0], kb[kk][i][1]);
+                        mma16816(d[p][2 * i + 1], za[p], kb[kk][i][2], kb[kk][i][3]);
                     }
-                }
             }
 #pragma unroll
             for (int i = 0; i < 2 * KT; i++)
@@ -473,16 +497,17 @@ static int launch_states(const DeltaChunkP& P, cudaStream_t s) {
 
 // ---------------------------------------------------------------------------- outputs
 
-// NK: blocks of 16 key channels at most; NW warps of 16 value columns each
+// NK: blocks of 16 key channels at most; a warp owns 8 value columns at a time
 template <int NK, int NW>
 struct DeltaOut {
     static constexpr int QS = NK * 16 + 8;
     static constexpr int SMEM = 2 * DC * QS * 2 + 3 * DC * TS * 2;
+    static constexpr int CTAS = NW == 4 ? 4 : NK <= 8 ? 2 : 1;      // of an SM
 };
 
 template <int NK, int NW>
-__global__ void __launch_bounds__(NW * 32) k_delta_out(const __grid_constant__ DeltaChunkP P) {
-    constexpr int QS = DeltaOut<NK, NW>::QS;
+__global__ void __launch_bounds__(NW * 32, DeltaOut<NK, NW>::CTAS) k_delta_out(const __grid_constant__ DeltaChunkP P) {
+    constexpr int QS = DeltaOut<NK, NW>::QS, KB = NK < 8 ? NK : 8;      // blocks of channels whose state is fetched together
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ __align__(16) double sb[DC];
     __shared__ float sr[DC], srq[DC];
@@ -496,15 +521,36 @@ __global__ void __launch_bounds__(NW * 32) k_delta_out(const __grid_constant__ D
     load_rows(sq, QS, NK * 2, P.q, c, P.ld, hq * dp, dp);
     load_rows(sk, QS, NK * 2, P.k, c, P.ld, hq * dp, dp);
     asm volatile("cp.async.commit_group;" ::: "memory");
+    const float* S0 = P.S0 + at * dvp * dp + 2 * tg;
+    const float* U = P.U + at * dvp * DC + 2 * tg;
+    float2 fS[KB][2], fU[4][2];
+    auto fetch_state = [&](int v, int kb) {
+#pragma unroll
+        for (int k = 0; k < KB; k++) {
+            const int x = (kb + k) * 16;
+            const float* p = S0 + (long)(v + g) * dp + x;
+            fS[k][0] = v < dvp && x < dp ? __ldcs((const float2*)p) : make_float2(0, 0);
+            fS[k][1] = v < dvp && x + 8 < dp ? __ldcs((const float2*)(p + 8)) : make_float2(0, 0);
+        }
+    };
+    auto fetch_u = [&](int v) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float* p = U + (long)(v + g) * DC + k * 16;
+            fU[k][0] = v < dvp ? __ldcs((const float2*)p) : make_float2(0, 0);
+            fU[k][1] = v < dvp ? __ldcs((const float2*)(p + 8)) : make_float2(0, 0);
+        }
+    };
+    fetch_state(warp * 8, 0);
     if (warp == 0) log_sums(P, c, h, lane, sb);
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
-    row_norms(sk, QS, NK * 16, P.D.eps, 1.0f, sr);
-    row_norms(sq, QS, NK * 16, P.D.eps, P.D.q_scale, srq);
+    row_norms(sk, QS, NK * 2, P.D.eps, 1.0f, sr);
+    row_norms(sq, QS, NK * 2, P.D.eps, P.D.q_scale, srq);
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < 8 / NW; u++) {           // q_t . k_j: columns 8 i .. of all rows that see them
-        const int i = u == 0 ? warp : 7 - warp;
+        const int i = NW == 8 ? (warp < 4 ? warp : 11 - warp) : (u == 0 ? warp : 7 - warp);
         float a[4][4];
 #pragma unroll
         for (int m = 0; m < 4; m++) a[m][0] = a[m][1] = a[m][2] = a[m][3] = 0.0f;
@@ -545,81 +591,56 @@ __global__ void __launch_bounds__(NW * 32) k_delta_out(const __grid_constant__ D
         }
     }
     __syncthreads();
-    for (int v0 = warp * 16; v0 < dvp; v0 += NW * 16) {
-        const float* S0 = P.S0 + at * dvp * dp;
-        const float* U = P.U + at * dvp * DC;
-        const bool ok[2] = {v0 + g < dvp, v0 + 8 + g < dvp};
-        float acc[4][2][4], low[4][2][4];
+    for (int v0 = warp * 8; v0 < dvp; v0 += NW * 8) {
+        if (v0 != warp * 8) fetch_state(v0, 0);
+        float acc[4][4], low[4][4];
 #pragma unroll
         for (int m = 0; m < 4; m++)
 #pragma unroll
-            for (int n = 0; n < 2; n++)
+            for (int e = 0; e < 4; e++) acc[m][e] = low[m][e] = 0.0f;
 #pragma unroll
-                for (int e = 0; e < 4; e++) acc[m][n][e] = low[m][n][e] = 0.0f;
+        for (int kb = 0; kb < NK; kb += KB) {
+            if (kb >= nk) break;
+            if (kb > 0) fetch_state(v0, kb);
 #pragma unroll
-        for (int kk = 0; kk < NK; kk++) {
-            if (kk >= nk) break;
-            unsigned bS[2][3][2];
+            for (int k = 0; k < KB; k++) {
+                if (kb + k >= nk) break;
+                unsigned b0[3], b1[3];
+                split3(fS[k][0].x, fS[k][0].y, b0[0], b0[1], b0[2]);
+                split3(fS[k][1].x, fS[k][1].y, b1[0], b1[1], b1[2]);
+                if (k == 0 && kb == 0) fetch_u(v0);
 #pragma unroll
-            for (int n = 0; n < 2; n++) {
-                const float* p = S0 + (long)(v0 + 8 * n + g) * dp + kk * 16 + 2 * tg;
-                float2 x = make_float2(0, 0), y = x;
-                if (ok[n]) {
-                    x = *(const float2*)p;
-                    if (kk * 16 + 8 < dp) y = *(const float2*)(p + 8);
-                }
-                split3(x.x, x.y, bS[n][0][0], bS[n][1][0], bS[n][2][0]);
-                split3(y.x, y.y, bS[n][0][1], bS[n][1][1], bS[n][2][1]);
-            }
-#pragma unroll
-            for (int m = 0; m < 4; m++) {
-                unsigned x[4];
-                ldsm4(x, sq + (m * 16 + (lane & 15)) * QS + kk * 16 + (lane >> 4) * 8);
-#pragma unroll
-                for (int n = 0; n < 2; n++) {
-                    mma16816(acc[m][n], x, bS[n][0][0], bS[n][0][1]);
-                    mma16816(low[m][n], x, bS[n][2][0], bS[n][2][1]);
-                    mma16816(low[m][n], x, bS[n][1][0], bS[n][1][1]);
+                for (int m = 0; m < 4; m++) {
+                    unsigned x[4];
+                    ldsm4(x, sq + (m * 16 + (lane & 15)) * QS + (kb + k) * 16 + (lane >> 4) * 8);
+                    mma16816(acc[m], x, b0[0], b1[0]);
+                    mma16816(low[m], x, b0[2], b1[2]);
+                    mma16816(low[m], x, b0[1], b1[1]);
                 }
             }
         }
 #pragma unroll
         for (int m = 0; m < 4; m++) {
             const float fa = exp2f((float)sb[m * 16 + g]), fb = exp2f((float)sb[m * 16 + g + 8]);
-#pragma unroll
-            for (int n = 0; n < 2; n++) {
-                acc[m][n][0] *= fa; acc[m][n][1] *= fa; acc[m][n][2] *= fb; acc[m][n][3] *= fb;
-                low[m][n][0] *= fa; low[m][n][1] *= fa; low[m][n][2] *= fb; low[m][n][3] *= fb;
-            }
+            acc[m][0] *= fa; acc[m][1] *= fa; acc[m][2] *= fb; acc[m][3] *= fb;
+            low[m][0] *= fa; low[m][1] *= fa; low[m][2] *= fb; low[m][3] *= fb;
         }
 #pragma unroll
         for (int kt = 0; kt < 4; kt++) {
-            unsigned bU[2][3][2];
-#pragma unroll
-            for (int n = 0; n < 2; n++) {
-                const float* p = U + (long)(v0 + 8 * n + g) * DC + kt * 16 + 2 * tg;
-                float2 x = make_float2(0, 0), y = x;
-                if (ok[n]) {
-                    x = *(const float2*)p;
-                    y = *(const float2*)(p + 8);
-                }
-                split3(x.x, x.y, bU[n][0][0], bU[n][1][0], bU[n][2][0]);
-                split3(y.x, y.y, bU[n][0][1], bU[n][1][1], bU[n][2][1]);
-            }
+            unsigned b0[3], b1[3];
+            split3(fU[kt][0].x, fU[kt][0].y, b0[0], b0[1], b0[2]);
+            split3(fU[kt][1].x, fU[kt][1].y, b1[0], b1[1], b1[2]);
 #pragma unroll
             for (int m = kt; m < 4; m++) {
                 unsigned x[3][4];
 #pragma unroll
                 for (int p = 0; p < 3; p++) ldsm4(x[p], sP + (p * DC + m * 16 + (lane & 15)) * TS + kt * 16 + (lane >> 4) * 8);
-#pragma unroll
-                for (int n = 0; n < 2; n++) {
-                    mma16816(acc[m][n], x[0], bU[n][0][0], bU[n][0][1]);
-                    mma16816(low[m][n], x[0], bU[n][2][0], bU[n][2][1]);
-                    mma16816(low[m][n], x[2], bU[n][0][0], bU[n][0][1]);
-                    mma16816(low[m][n], x[1], bU[n][1][0], bU[n][1][1]);
-                    mma16816(low[m][n], x[0], bU[n][1][0], bU[n][1][1]);
-                    mma16816(low[m][n], x[1], bU[n][0][0], bU[n][0][1]);
-                }
+                mma16816(acc[m], x[0], b0[0], b1[0]);
+                mma16816(low[m], x[0], b0[2], b1[2]);
+                mma16816(low[m], x[2], b0[0], b1[0]);
+                mma16816(low[m], x[1], b0[1], b1[1]);
+                mma16816(low[m], x[0], b0[1], b1[1]);
+                mma16816(low[m], x[1], b0[0], b1[0]);
             }
         }
 #pragma unroll
@@ -629,11 +650,8 @@ __global__ void __launch_bounds__(NW * 32) k_delta_out(const __grid_constant__ D
                 const int t = m * 16 + g + 8 * e;
                 if (t >= c.rows) continue;
                 const float f = srq[t];
-                float* o = P.o + (c.row0 + t) * P.ldo + (long)h * dvp + v0 + 2 * tg;
-#pragma unroll
-                for (int n = 0; n < 2; n++)
-                    if (v0 + 8 * n < dvp)
-                        *(float2*)(o + 8 * n) = make_float2(f * (acc[m][n][2 * e] + low[m][n][2 * e]), f * (acc[m][n][2 * e + 1] + low[m][n][2 * e + 1]));
+                *(float2*)(P.o + (c.row0 + t) * P.ldo + (long)h * dvp + v0 + 2 * tg) =
+                    make_float2(f * (acc[m][2 * e] + low[m][2 * e]), f * (acc[m][2 * e + 1] + low[m][2 * e + 1]));
             }
     }
 }
@@ -688,11 +706,10 @@ extern "C" int lt_dn_delta_chunked(const void* q, const void* k, const void* v, 
     P.S0 = P.vec + n * DVEC;
     P.U = P.S0 + n * P.D.dvp * P.D.dp;
     cudaStream_t s = (cudaStream_t)stream;
-    const int dp = P.D.dp, dpr = (dp + 31) & ~31;
-    const size_t sm = (size_t)(2 * DC * MS + 32 * 36) * 4 + (size_t)DC * (dpr + 8) * 2;
+    const int dp = P.D.dp;
     static PerDeviceOnce once;
-    if (once.first()) LT_CUDA(cudaFuncSetAttribute(k_delta_prep, cudaFuncAttributeMaxDynamicSharedMemorySize, (2 * DC * MS + 32 * 36) * 4 + DC * 264 * 2));
-    k_delta_prep<<<dim3(chunks, P.D.H), 128, sm, s>>>(P);
+    if (once.first()) LT_CUDA(cudaFuncSetAttribute(k_delta_prep, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)prep_smem(256)));
+    k_delta_prep<<<dim3(chunks, P.D.H), PREP_THREADS, prep_smem(dp), s>>>(P);
     int rc = check_launch("lt_dn_delta_chunked (prepare)");
     if (rc != LT_OK) return rc;
     rc = dp <= 64 ? launch_states<4, 1, 2>(P, s) : dp <= 128 ? launch_states<8, 1, 3>(P, s) : launch_states<8, 2, 2>(P, s);
