@@ -156,6 +156,14 @@ __device__ __forceinline__ float warp_sum(float v) {
     for (int s = 16; s > 0; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
     return v;
 }
+// N sums at once: step by step, so that one's shuffle runs under another's
+template <int N>
+__device__ __forceinline__ void warp_sums(float (&v)[N]) {
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1)
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] += __shfl_xor_sync(0xffffffffu, v[i], s);
+}
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
     for (int s = 16; s > 0; s >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, s));

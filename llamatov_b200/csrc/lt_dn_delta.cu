@@ -1,150 +1,373 @@
 // Gated delta rule in token order, state in fp32:
 //   k^ = k / sqrt(sum k^2 + eps),  q^ = q_scale q / sqrt(sum q^2 + eps)
 //   u_t = beta_t (v_t - a_t S k^_t),  S <- a_t S + u_t k^_t^T,  o_t = S q^_t
-// The output needs no second pass over the new state: S_new q^ = a (S q^) + u (k^ . q^), so both products are taken of the old
-// state together and a token is one dependent chain: products, their sum over the lanes of a column, u, the update.
+// Tokens are taken four at a time.  With g_i the product of the block's decays up to token i, everything that needs the state is a
+// product with the state before the block, S k^_i and S q^_i, and the rest is numbers of the keys and queries alone:
+//   u_i = beta_i (v_i - g_i S k^_i - sum_(j < i) (g_i / g_j) (k^_i . k^_j) u_j)
+//   o_i = g_i S q^_i + sum_(j <= i) (g_i / g_j) (q^_i . k^_j) u_j,   S <- g_3 S + sum_j (g_3 / g_j) u_j k^_j^T
+// so that the dependent chain (products, their sum over the lanes of a column, u, the update) is gone through once for four tokens.
+// (The ratios are products of the decays between, no quotients.)
 //
-// k_delta_scan walks rows (fp32, short portions): a CTA owns 32 value columns of one head of one sequence, eight lanes share a
-// column (dp/8 key channels each, in registers); normed q and k and k^ . q^ are made 16 tokens at a time, a warp per token.
+// k_delta_scan walks rows (fp32, short portions): a CTA owns 16 value columns of one head of one sequence.  Four warps hold the state,
+// eight lanes a column, dp/8 key channels each in registers, and read keys and queries as they are in memory: the norms are part of
+// the blocks' numbers.  Four warps make those numbers for the next batch, a warp per block, from rows that bulk copies have brought a
+// batch earlier.  What bounds it is how many instructions a block is for one warp (four to five clocks each, as its scheduler has
+// little else): products are of pairs (fma.rn.f32x2), and of S q^ a lane gets the one sum that it stores.
+// (14 heads of 64 in fp32, 300 rows: 94 us token by token, staged without overlap; 47 in blocks with two columns a lane; 33 now.)
 // k_delta_step is one token with its convolution and step size.
 #include "lt_dn_delta.cuh"
+#include "lt_tc.cuh"
 
 namespace lt {
 namespace dn {
+
+using namespace tc;
 
 struct DeltaScanP {
     const void *q, *k, *v;
     const float *la, *beta;
     float* o;
+    int* status;
     int ld, ldh, ldo;
     lt_dn_delta D;
     lt_dn_seqs Q;
 };
-constexpr int DT = 16;    // tokens staged at a time
 
-__device__ __forceinline__ float sum8(float v) {       // over the eight lanes of a column
-    v += __shfl_xor_sync(0xffffffffu, v, 1);
-    v += __shfl_xor_sync(0xffffffffu, v, 2);
-    return v + __shfl_xor_sync(0xffffffffu, v, 4);
+// two fp32 in a register pair, as the packed instructions take them
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 pack2(float x, float y) {
+    f2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void unpack2(f2 v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+    f2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+    f2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
 }
 
-template <int KPT>
+// a state row's share of a lane: VEC channels at a time, LN lanes side by side
+template <int KPT, int VEC = 4, int LN = 8>
 __device__ __forceinline__ void load_state(float (&s)[KPT], const float* row, int dp, int g) {
 #pragma unroll
     for (int i = 0; i < KPT / 4; i++) {
-        const int c = i * 32 + g * 4;
+        const int c = (i * 4 / VEC * LN + g) * VEC + i * 4 % VEC;
         float4 x = make_float4(0, 0, 0, 0);
         if (c < dp) x = *(const float4*)(row + c);
         s[4 * i] = x.x; s[4 * i + 1] = x.y; s[4 * i + 2] = x.z; s[4 * i + 3] = x.w;
     }
 }
-template <int KPT>
+template <int KPT, int VEC = 4, int LN = 8>
 __device__ __forceinline__ void store_state(const float (&s)[KPT], float* row, int dp, int g) {
 #pragma unroll
     for (int i = 0; i < KPT / 4; i++) {
-        const int c = i * 32 + g * 4;
+        const int c = (i * 4 / VEC * LN + g) * VEC + i * 4 % VEC;
         if (c < dp) *(float4*)(row + c) = make_float4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
     }
 }
 
-template <typename T, int KPT>
-__global__ void __launch_bounds__(256) k_delta_scan(const __grid_constant__ DeltaScanP P) {
-    constexpr int DP = 8 * KPT;
-    extern __shared__ __align__(16) float dsm[];
-    float* sq = dsm;                   // [DT][DP]
-    float* sk = sq + DT * DP;
-    float* sv = sk + DT * DP;          // [DT][32]
-    float* sc = sv + DT * 32;          // [DT][4]: decay, beta, k . q
-    const lt_dn_delta& D = P.D;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = tid & 7, cl = tid >> 3;
-    const int h = blockIdx.y, b = blockIdx.z, hq = h / (D.H / D.G), col = blockIdx.x * 32 + cl;
-    const bool col_ok = col < D.dvp;
-    const int T_ = P.Q.rows[b];
-    const long first = P.Q.start[b];
-    if (T_ == 0) return;
-    float s[KPT];
-    float* Srow = P.Q.S[b] + ((long)h * D.dvp + (col_ok ? col : 0)) * D.dp;
-    load_state<KPT>(s, Srow, D.dp, g);
+// The numbers of a block of four tokens, with r_i = 1 / |k_i| and rq_i = q_scale / |q_i|
+struct __align__(16) DeltaBlock {
+    float kk[4][4];      // beta_i (g_i / g_j) r_i r_j k_i . k_j, below the diagonal
+    float qk[4][4];      // (g_i / g_j) rq_i r_j q_i . k_j, up to it
+    float beta[4], bg[4], gq[4], z[4];      // beta_i; beta_i g_i r_i; g_i rq_i; (g_3 / g_i) r_i
+    float end[4];        // g_3
+};
+constexpr int SCAN_COLS = 16;
 
-    for (int t0 = 0; t0 < T_; t0 += DT) {
-        const int nt = min(DT, T_ - t0);
-        for (int t = warp; t < nt; t += 8) {
-            const long r = first + t0 + t;
-            const T* q = (const T*)P.q + r * P.ld + (long)hq * D.dp;
-            const T* k = (const T*)P.k + r * P.ld + (long)hq * D.dp;
-            float fq[DP / 32], fk[DP / 32], qq = 0.0f, kk = 0.0f, kq = 0.0f;
-#pragma unroll
-            for (int i = 0; i < DP / 32; i++) {
-                const int c = lane + 32 * i;
-                fq[i] = c < D.dp ? to_f(q[c]) : 0.0f;
-                fk[i] = c < D.dp ? to_f(k[c]) : 0.0f;
-                qq = fmaf(fq[i], fq[i], qq);
-                kk = fmaf(fk[i], fk[i], kk);
-                kq = fmaf(fk[i], fq[i], kq);
-            }
-            qq = warp_sum(qq);
-            kk = warp_sum(kk);
-            kq = warp_sum(kq);
-            const float rq = D.q_scale / sqrtf(qq + D.eps), rk = 1.0f / sqrtf(kk + D.eps);
-#pragma unroll
-            for (int i = 0; i < DP / 32; i++) {
-                sq[t * DP + lane + 32 * i] = fq[i] * rq;
-                sk[t * DP + lane + 32 * i] = fk[i] * rk;
-            }
-            const int c = blockIdx.x * 32 + lane;
-            sv[t * 32 + lane] = c < D.dvp ? to_f(((const T*)P.v)[r * P.ld + (long)h * D.dvp + c]) : 0.0f;
-            if (lane == 0) {
-                sc[4 * t] = expf(P.la[r * P.ldh + h]);
-                sc[4 * t + 1] = P.beta[r * P.ldh + h];
-                sc[4 * t + 2] = kq * rq * rk;
-            }
-        }
-        __syncthreads();
-        for (int t = 0; t < nt; t++) {
-            const float a = sc[4 * t], be = sc[4 * t + 1], kq = sc[4 * t + 2], v = sv[t * 32 + cl];
-            float4 k[KPT / 4];
-            float p[4] = {0, 0, 0, 0}, r[4] = {0, 0, 0, 0};
-#pragma unroll
-            for (int i = 0; i < KPT / 4; i++) {
-                const int c = t * DP + i * 32 + g * 4;
-                k[i] = *(const float4*)(sk + c);
-                const float4 q = *(const float4*)(sq + c);
-                p[0] = fmaf(k[i].x, s[4 * i], p[0]); p[1] = fmaf(k[i].y, s[4 * i + 1], p[1]);
-                p[2] = fmaf(k[i].z, s[4 * i + 2], p[2]); p[3] = fmaf(k[i].w, s[4 * i + 3], p[3]);
-                r[0] = fmaf(q.x, s[4 * i], r[0]); r[1] = fmaf(q.y, s[4 * i + 1], r[1]);
-                r[2] = fmaf(q.z, s[4 * i + 2], r[2]); r[3] = fmaf(q.w, s[4 * i + 3], r[3]);
-            }
-            const float Sk = sum8((p[0] + p[1]) + (p[2] + p[3])), Sq = sum8((r[0] + r[1]) + (r[2] + r[3]));
-            const float u = be * fmaf(-a, Sk, v);
-#pragma unroll
-            for (int i = 0; i < KPT / 4; i++) {
-                s[4 * i] = fmaf(a, s[4 * i], u * k[i].x);
-                s[4 * i + 1] = fmaf(a, s[4 * i + 1], u * k[i].y);
-                s[4 * i + 2] = fmaf(a, s[4 * i + 2], u * k[i].z);
-                s[4 * i + 3] = fmaf(a, s[4 * i + 3], u * k[i].w);
-            }
-            if (g == 0 && col_ok) P.o[(first + t0 + t) * P.ldo + (long)h * D.dvp + col] = fmaf(a, Sq, u * kq);
-        }
-        __syncthreads();
-    }
-    if (col_ok) store_state<KPT>(s, Srow, D.dp, g);
+__device__ __forceinline__ void bulk_load(unsigned dst, const void* src, unsigned bytes, unsigned bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
 }
 
-template <typename T, int KPT>
+// LN lanes a column, KPT channels a lane
+template <typename T, int KPT, int LN>
+struct DeltaScan {
+    static constexpr int DP = LN * KPT, BT = DP <= 128 ? 16 : 8, NB = BT / 4;     // tokens and blocks of a batch
+    static constexpr int CW = LN / 2, THREADS = (CW + 4) * 32;                    // warps that hold the state
+    static constexpr int RAW = 2 * DP + SCAN_COLS;                                // elements of a row: q, k, v
+    static constexpr int VEC = sizeof(T) == 2 && KPT >= 8 ? 8 : 4;                // channels of a load
+    static constexpr int RAW_B = BT * RAW * (int)sizeof(T);
+    static constexpr int SMEM = 3 * RAW_B + 2 * NB * (int)sizeof(DeltaBlock);
+    static_assert(SMEM <= 227 * 1024 && RAW_B % 16 == 0, "shared memory");
+};
+template <typename T, int VEC>
+__device__ __forceinline__ void load_pairs(f2 (&f)[VEC / 2], const T* p) {
+    if (sizeof(T) == 4) {
+        const float4 x = *(const float4*)p;
+        f[0] = pack2(x.x, x.y);
+        f[1] = pack2(x.z, x.w);
+    } else {
+        unsigned w[4];
+        if (VEC == 8) *(uint4*)w = *(const uint4*)p;
+        else *(uint2*)w = *(const uint2*)p;
+#pragma unroll
+        for (int i = 0; i < VEC / 2; i++) f[i] = pack2(lo_f(w[i]), hi_f(w[i]));
+    }
+}
+
+template <typename T, int KPT, int LN>
+__global__ void __launch_bounds__(DeltaScan<T, KPT, LN>::THREADS) k_delta_scan(const __grid_constant__ DeltaScanP P) {
+    using L = DeltaScan<T, KPT, LN>;
+    constexpr int DP = L::DP, BT = L::BT, NB = L::NB, VEC = L::VEC, ES = (int)sizeof(T);
+    extern __shared__ __align__(128) unsigned char dsm[];
+    __shared__ unsigned long long full[3];
+    __shared__ int abort_word;
+    const lt_dn_delta& D = P.D;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int h = blockIdx.y, b = blockIdx.z, hq = h / (D.H / D.G), v0 = blockIdx.x * SCAN_COLS;
+    const int rows = P.Q.rows[b], batches = (rows + BT - 1) / BT;
+    const long first = P.Q.start[b];
+    if (rows == 0) return;
+    volatile int* abort_flag = &abort_word;
+    auto raw = [&](int n) { return (T*)(dsm + (n % 3) * L::RAW_B); };
+    auto ready = [&](int n) { return (DeltaBlock*)(dsm + 3 * L::RAW_B) + (n & 1) * NB; };
+    auto wait = [&](int n) {
+        const unsigned bar = smem_u32(&full[n % 3]);
+        bar_wait(bar_test(bar, (n / 3) & 1), bar, (n / 3) & 1, abort_flag, P.status);
+    };
+    // what no copy writes is zero: channels behind dp, columns behind dvp, tokens behind the last (or an earlier token's, whose beta is
+    // taken for 0)
+    for (int e = tid; e < 3 * L::RAW_B / 16; e += L::THREADS) ((uint4*)dsm)[e] = make_uint4(0, 0, 0, 0);
+    if (tid == 0) {
+        abort_word = 0;
+        for (int i = 0; i < 3; i++) mbar_init(&full[i], NB);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncthreads();
+
+    if (warp >= L::CW) {
+        const int blk = warp - L::CW;
+        // rows of the block: a lane copies a token's q, k or v
+        const int cols = min(SCAN_COLS, D.dvp - v0), what = lane >> 2, tok = blk * 4 + (lane & 3);
+        const T* src = what == 0 ? (const T*)P.q + (long)hq * D.dp : what == 1 ? (const T*)P.k + (long)hq * D.dp : (const T*)P.v + (long)h * D.dvp + v0;
+        src += (first + tok) * P.ld;
+        const unsigned to_place = (unsigned)((tok * L::RAW + what * DP) * ES), bytes = (unsigned)((what < 2 ? D.dp : cols) * ES);
+        auto fetch = [&](int n) {
+            if (blk >= NB || n >= batches || *abort_flag) return;
+            const int count = max(0, min(4, rows - n * BT - blk * 4));
+            const unsigned bar = smem_u32(&full[n % 3]);
+            if (lane == 0) bar_expect_tx(bar, (unsigned)(count * (2 * D.dp + cols) * ES));
+            __syncwarp();
+            if (what < 3 && (lane & 3) < count) bulk_load(smem_u32(raw(n)) + to_place, src + (long)n * BT * P.ld, bytes, bar);
+        };
+        // decay and beta of the block's tokens in lanes 0 - 3, asked for a batch ahead
+        float la = 0.0f, be = 0.0f, la_next = 0.0f, be_next = 0.0f;
+        auto numbers = [&](int n) {
+            const int t = n * BT + blk * 4 + (lane & 3);
+            const bool ok = n < batches && blk < NB && t < rows;
+            la = la_next;
+            be = be_next;
+            la_next = ok ? P.la[(first + t) * P.ldh + h] : 0.0f;
+            be_next = ok ? P.beta[(first + t) * P.ldh + h] : 0.0f;
+        };
+        auto make = [&](int n) {
+            if (blk >= NB) return;
+            const float decay = expf(la);
+            const T* in = raw(n) + blk * 4 * L::RAW;
+            float x[32];             // k_i . k_j (j < i), q_i . k_j (j <= i), q_i . q_i, k_i . k_i
+#pragma unroll
+            for (int i = 0; i < 32; i++) x[i] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < DP / 32; c++) {
+                float q[4], k[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    q[i] = to_f(in[i * L::RAW + lane + 32 * c]);
+                    k[i] = to_f(in[i * L::RAW + DP + lane + 32 * c]);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+#pragma unroll
+                    for (int j = 0; j <= i; j++) {
+                        if (j < i) x[i * (i - 1) / 2 + j] = fmaf(k[i], k[j], x[i * (i - 1) / 2 + j]);
+                        x[6 + i * (i + 1) / 2 + j] = fmaf(q[i], k[j], x[6 + i * (i + 1) / 2 + j]);
+                    }
+                    x[16 + i] = fmaf(q[i], q[i], x[16 + i]);
+                    x[20 + i] = fmaf(k[i], k[i], x[20 + i]);
+                }
+            }
+            // sums over the lanes: at every step a lane hands on one half of its values and keeps the other, and ends with number `lane`
+#pragma unroll
+            for (int s = 16; s > 0; s >>= 1)
+#pragma unroll
+                for (int i = 0; i < s; i++) {
+                    const bool up = (lane & s) != 0;
+                    const float give = up ? x[i] : x[i + s], have = up ? x[i + s] : x[i];
+                    x[i] = have + __shfl_xor_sync(0xffffffffu, give, s);
+                }
+            const float dot = x[0];
+            const float norm = (lane < 20 ? D.q_scale : 1.0f) / sqrtf(dot + D.eps);      // of lanes 16 - 23
+            const int i = (lane >> 2) & 3, j = lane & 3;
+            float a[4];
+#pragma unroll
+            for (int m = 0; m < 4; m++) a[m] = __shfl_sync(0xffffffffu, decay, m);
+            float ratio = 1.0f, to = 1.0f, rest = 1.0f;      // g_i / g_j, g_j, g_3 / g_j
+#pragma unroll
+            for (int m = 0; m < 4; m++) {
+                if (m > j && m <= i) ratio *= a[m];
+                if (m <= j) to *= a[m];
+                if (m > j) rest *= a[m];
+            }
+            const bool kk = lane < 16;
+            const int at = kk ? (j < i ? i * (i - 1) / 2 + j : 0) : 6 + (j <= i ? i * (i + 1) / 2 + j : 0);
+            const float d = __shfl_sync(0xffffffffu, dot, at);
+            const float ni = __shfl_sync(0xffffffffu, norm, (kk ? 20 : 16) + i), rj = __shfl_sync(0xffffffffu, norm, 20 + j);
+            const float qj = __shfl_sync(0xffffffffu, norm, 16 + j);
+            const float bi = __shfl_sync(0xffffffffu, be, i), bj = __shfl_sync(0xffffffffu, be, j);
+            float* o = (float*)(ready(n) + blk);
+            o[lane] = (kk ? j < i : j <= i) ? ratio * (d * ni * rj) * (kk ? bi : 1.0f) : 0.0f;
+            if (lane < 16) o[32 + lane] = i == 0 ? bj : i == 1 ? bj * to * rj : i == 2 ? to * qj : rest * rj;
+            if (lane == 19) o[48] = to;
+        };
+        fetch(0);
+        fetch(1);
+        numbers(0);
+        numbers(1);
+        wait(0);
+        make(0);
+        __syncthreads();
+        for (int n = 0; n < batches; n++) {      // while the others walk batch n
+            fetch(n + 2);
+            numbers(n + 2);
+            if (n + 1 < batches) {
+                wait(n + 1);
+                make(n + 1);
+            }
+            __syncthreads();
+        }
+    } else {
+        const int g = tid & (LN - 1), cl = tid / LN, col = v0 + cl, mine = g & 3;      // mine: the token whose output this lane has
+        const bool col_ok = col < D.dvp;
+        float* Srow = P.Q.S[b] + ((long)h * D.dvp + (col_ok ? col : 0)) * D.dp;
+        f2 s[KPT / 2];
+        {
+            float t[KPT];
+            load_state<KPT, VEC, LN>(t, Srow, D.dp, g);
+#pragma unroll
+            for (int i = 0; i < KPT / 2; i++) s[i] = pack2(t[2 * i], t[2 * i + 1]);
+        }
+        float* o = P.o + (first + mine) * P.ldo + (long)h * D.dvp + col;
+        __syncthreads();
+        for (int n = 0; n < batches; n++) {
+            wait(n);
+            const T* qb = raw(n) + g * VEC;
+            const T* vb = raw(n) + 2 * DP + cl;
+            const DeltaBlock* R = ready(n);
+            int left = rows - n * BT;
+#pragma unroll 1
+            for (int blk = 0; blk < NB && left > 0; blk++) {
+                f2 x[8];             // S k_i, then S q_i, in halves
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[i] = 0ull;
+#pragma unroll
+                for (int c = 0; c < KPT / VEC; c++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        f2 k[VEC / 2], q[VEC / 2];
+                        load_pairs<T, VEC>(k, qb + i * L::RAW + DP + c * LN * VEC);
+                        load_pairs<T, VEC>(q, qb + i * L::RAW + c * LN * VEC);
+#pragma unroll
+                        for (int e = 0; e < VEC / 2; e++) {
+                            x[i] = fma2(k[e], s[c * VEC / 2 + e], x[i]);
+                            x[4 + i] = fma2(q[e], s[c * VEC / 2 + e], x[4 + i]);
+                        }
+                    }
+                // the block's numbers, read ahead of the shuffles, which nothing is moved across
+                const float4 be = *(const float4*)R->beta, bg = *(const float4*)R->bg, z = *(const float4*)R->z, qk = *(const float4*)R->qk[mine];
+                const float4 k1 = *(const float4*)R->kk[1], k2 = *(const float4*)R->kk[2], k3 = *(const float4*)R->kk[3];
+                const float end = R->end[0], gq = R->gq[mine];
+                const float v0_ = be.x * to_f(vb[0]), v1 = be.y * to_f(vb[L::RAW]), v2 = be.z * to_f(vb[2 * L::RAW]), v3 = be.w * to_f(vb[3 * L::RAW]);
+                float p[4], r[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    float a, c;
+                    unpack2(x[i], a, c);
+                    p[i] = a + c;
+                    unpack2(x[4 + i], a, c);
+                    r[i] = a + c;
+                }
+#pragma unroll
+                for (int m = LN / 2; m > 0; m >>= 1) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) p[i] += __shfl_xor_sync(0xffffffffu, p[i], m);
+                    if (m >= 4) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) r[i] += __shfl_xor_sync(0xffffffffu, r[i], m);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < m; i++) {    // a lane ends with the sum of its own number
+                            const bool up = (g & m) != 0;
+                            const float give = up ? r[i] : r[i + m], have = up ? r[i + m] : r[i];
+                            r[i] = have + __shfl_xor_sync(0xffffffffu, give, m);
+                        }
+                    }
+                }
+                const float u0 = fmaf(-bg.x, p[0], v0_);
+                const float u1 = fmaf(-k1.x, u0, fmaf(-bg.y, p[1], v1));
+                const float u2 = fmaf(-k2.y, u1, fmaf(-k2.x, u0, fmaf(-bg.z, p[2], v2)));
+                const float u3 = fmaf(-k3.z, u2, fmaf(-k3.y, u1, fmaf(-k3.x, u0, fmaf(-bg.w, p[3], v3))));
+                // above the diagonal the numbers are zero
+                const float y = fmaf(qk.w, u3, fmaf(qk.z, u2, fmaf(qk.y, u1, fmaf(qk.x, u0, gq * r[0]))));
+                if (col_ok && g < 4 && mine < left) *o = y;
+                const float w0 = z.x * u0, w1 = z.y * u1, w2 = z.z * u2, w3 = z.w * u3;
+                const f2 w[4] = {pack2(w0, w0), pack2(w1, w1), pack2(w2, w2), pack2(w3, w3)}, end2 = pack2(end, end);
+#pragma unroll
+                for (int c = 0; c < KPT / VEC; c++) {
+#pragma unroll
+                    for (int e = c * VEC / 2; e < (c + 1) * VEC / 2; e++) s[e] = mul2(s[e], end2);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        f2 k[VEC / 2];
+                        load_pairs<T, VEC>(k, qb + i * L::RAW + DP + c * LN * VEC);
+#pragma unroll
+                        for (int e = 0; e < VEC / 2; e++) s[c * VEC / 2 + e] = fma2(w[i], k[e], s[c * VEC / 2 + e]);
+                    }
+                }
+                qb += 4 * L::RAW;
+                vb += 4 * L::RAW;
+                o += 4L * P.ldo;
+                left -= 4;
+                R++;
+            }
+            __syncthreads();
+        }
+        if (col_ok) {
+            float t[KPT];
+#pragma unroll
+            for (int i = 0; i < KPT / 2; i++) unpack2(s[i], t[2 * i], t[2 * i + 1]);
+            store_state<KPT, VEC, LN>(t, Srow, D.dp, g);
+        }
+    }
+    if (*abort_flag) {               // a wait ran out: let copies in flight land before the CTA leaves
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000LL) {
+        }
+    }
+}
+
+template <typename T, int KPT, int LN>
 static int launch_delta_scan(const DeltaScanP& P, cudaStream_t s) {
-    const size_t smem = ((size_t)DT * 8 * KPT * 2 + (size_t)DT * 36) * 4;
+    using L = DeltaScan<T, KPT, LN>;
     static PerDeviceOnce once;
-    if (once.first()) LT_CUDA(cudaFuncSetAttribute(k_delta_scan<T, KPT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    k_delta_scan<T, KPT><<<dim3((P.D.dvp + 31) / 32, P.D.H, P.Q.n), 256, smem, s>>>(P);
-    return check_launch("lt_dn_delta");
+    if (once.first()) LT_CUDA(cudaFuncSetAttribute(k_delta_scan<T, KPT, LN>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM));
+    k_delta_scan<T, KPT, LN><<<dim3((P.D.dvp + SCAN_COLS - 1) / SCAN_COLS, P.D.H, P.Q.n), L::THREADS, L::SMEM, s>>>(P);
+    return check_launch("lt_dn_delta_rows");
 }
 template <typename T>
 static int delta_scan_size(const DeltaScanP& P, cudaStream_t s) {
-    if (P.D.dp <= 32) return launch_delta_scan<T, 4>(P, s);
-    if (P.D.dp <= 64) return launch_delta_scan<T, 8>(P, s);
-    if (P.D.dp <= 128) return launch_delta_scan<T, 16>(P, s);
-    if (P.D.dp <= 256) return launch_delta_scan<T, 32>(P, s);
-    return launch_delta_scan<T, 64>(P, s);
+    if (P.D.dp <= 32) return launch_delta_scan<T, 4, 8>(P, s);
+    if (P.D.dp <= 64) return launch_delta_scan<T, 8, 8>(P, s);
+    if (P.D.dp <= 128) return launch_delta_scan<T, 16, 8>(P, s);
+    if (P.D.dp <= 256) return launch_delta_scan<T, 16, 16>(P, s);
+    return launch_delta_scan<T, 32, 16>(P, s);
 }
 
 // ---------------------------------------------------------------------------- one token
@@ -211,11 +434,14 @@ __global__ void __launch_bounds__(256) k_delta_step(const __grid_constant__ Delt
         qq = fmaf(q.x, q.x, fmaf(q.y, q.y, fmaf(q.z, q.z, fmaf(q.w, q.w, qq))));
         kq = fmaf(k.x, q.x, fmaf(k.y, q.y, fmaf(k.z, q.z, fmaf(k.w, q.w, kq))));
     }
-    Sk = sum8(Sk);
-    Sq = sum8(Sq);
-    kk = sum8(kk);
-    qq = sum8(qq);
-    kq = sum8(kq);
+#pragma unroll
+    for (int x = 1; x < 8; x <<= 1) {            // over the eight lanes of a column, the five sums side by side
+        Sk += __shfl_xor_sync(0xffffffffu, Sk, x);
+        Sq += __shfl_xor_sync(0xffffffffu, Sq, x);
+        kk += __shfl_xor_sync(0xffffffffu, kk, x);
+        qq += __shfl_xor_sync(0xffffffffu, qq, x);
+        kq += __shfl_xor_sync(0xffffffffu, kq, x);
+    }
     const float rk = 1.0f / sqrtf(kk + D.eps), rq = D.q_scale / sqrtf(qq + D.eps);
     const float u = be * fmaf(-a, Sk * rk, sv[cl]), uk = u * rk;
 #pragma unroll
@@ -290,8 +516,10 @@ extern "C" int lt_dn_delta_rows(const void* q, const void* k, const void* v, int
     LT_REQUIRE(q && k && v && la && beta && o, "lt_dn_delta_rows: null pointer");
     LT_REQUIRE(ld >= h_d->G * h_d->dp && ld >= h_d->H * h_d->dvp && ldh >= h_d->H && ldo >= h_d->H * h_d->dvp,
                "lt_dn_delta_rows: ld=%d ldh=%d ldo=%d", ld, ldh, ldo);
+    LT_REQUIRE(ld % 8 == 0 && ldo % 2 == 0 && aligned16(q) && aligned16(k) && aligned16(v) && aligned16(o), "lt_dn_delta_rows: alignment");
     if (rows == 0) return LT_OK;
-    DeltaScanP P = {q, k, v, la, beta, o, ld, ldh, ldo, *h_d, *h_q};
+    DeltaScanP P = {q, k, v, la, beta, o, device_status_ptr(), ld, ldh, ldo, *h_d, *h_q};
+    LT_REQUIRE(P.status != nullptr, "lt_dn_delta_rows: status word unavailable");
     if (f32) return delta_scan_size<float>(P, (cudaStream_t)stream);
     return delta_scan_size<bf16>(P, (cudaStream_t)stream);
 }

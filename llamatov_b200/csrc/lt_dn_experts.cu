@@ -22,7 +22,11 @@ struct FewP {
     lt_dn_epilogue epi;
 };
 
-constexpr int FEW_THREADS = 256, FEW_U = 4;
+// An SM has four CTAs of 64 registers a thread, each lane with two rows x 4 loads of 16 bytes under way.  (8 of 64 experts for one
+// token in bf16: gate|up 2 x 1024 x 2048 14.2 us, 4.7 TB/s, down 2048 x 1024 10.5; with two CTAs that also hold their part of x
+// ahead 15.1 and 13.3; twice the loads a lane 16.0 and 14.0; rows through rings of bulk copies in shared memory, 192 KB under way,
+// 20.1 and 15.9.)
+constexpr int FEW_THREADS = 256, FEW_U = 4, FEW_CTAS = 4;
 
 // products of two rows with x: this lane's share
 template <typename T>
@@ -30,14 +34,12 @@ __device__ __forceinline__ void two_dots(const T* a, const T* b, const T* x, int
     constexpr int N = Vec<T>::N;
     for (int base = lane; base < nvec; base += 32 * FEW_U) {
         int4 va[FEW_U], vb[FEW_U];
-        uint4 vx[FEW_U];
 #pragma unroll
         for (int u = 0; u < FEW_U; u++) {
             const int i = base + u * 32;
             if (i < nvec) {
                 va[u] = ld_stream_v4((const uint4*)a + i);
                 vb[u] = ld_stream_v4((const uint4*)b + i);
-                vx[u] = ((const uint4*)x)[i];
             }
         }
 #pragma unroll
@@ -46,7 +48,7 @@ __device__ __forceinline__ void two_dots(const T* a, const T* b, const T* x, int
             float fa[N], fb[N], fx[N];
             Vec<T>::unpack(make_uint4(va[u].x, va[u].y, va[u].z, va[u].w), fa);
             Vec<T>::unpack(make_uint4(vb[u].x, vb[u].y, vb[u].z, vb[u].w), fb);
-            Vec<T>::unpack(vx[u], fx);
+            Vec<T>::unpack(((const uint4*)x)[base + u * 32], fx);
 #pragma unroll
             for (int j = 0; j < N; j++) {
                 s0 = fmaf(fa[j], fx[j], s0);
@@ -57,7 +59,7 @@ __device__ __forceinline__ void two_dots(const T* a, const T* b, const T* x, int
 }
 
 template <typename T>
-__global__ void __launch_bounds__(FEW_THREADS, 2) k_few_glu(const __grid_constant__ FewP P) {
+__global__ void __launch_bounds__(FEW_THREADS, FEW_CTAS) k_few_glu(const __grid_constant__ FewP P) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nvec = P.K / Vec<T>::N;
     const long tasks = (long)P.c.T * P.c.top * P.M, nw = (long)gridDim.x * (FEW_THREADS / 32);
     for (long i = (long)blockIdx.x * (FEW_THREADS / 32) + warp; i < tasks; i += nw) {
@@ -70,15 +72,15 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) k_few_glu(const __grid_constan
         const T* a = (const T*)P.W + ((long)e * 2 * P.M + f) * P.ldw;
         float g = 0.0f, u = 0.0f;
         two_dots(a, a + (long)P.M * P.ldw, (const T*)P.X + p / P.c.top * P.ldx, nvec, lane, g, u);
-        g = warp_sum(g);
-        u = warp_sum(u);
-        if (lane == 0) glu_store<T>(P.epi, P.Y, p * P.ldy + f, g, u);
+        float v[2] = {g, u};
+        warp_sums(v);
+        if (lane == 0) glu_store<T>(P.epi, P.Y, p * P.ldy + f, v[0], v[1]);
     }
 }
 
 // wj warps share a pair of rows: warp s of them has the experts s, s + wj, ...
 template <typename T>
-__global__ void __launch_bounds__(FEW_THREADS, 2) k_few_sum(const __grid_constant__ FewP P, int wj) {
+__global__ void __launch_bounds__(FEW_THREADS, FEW_CTAS) k_few_sum(const __grid_constant__ FewP P, int wj) {
     __shared__ float part[2][FEW_THREADS / 32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nvec = P.K / Vec<T>::N;
     const int sub = warp & (wj - 1), pairs = FEW_THREADS / 32 / wj, t = blockIdx.y;
@@ -100,8 +102,10 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) k_few_sum(const __grid_constan
                 s0 = fmaf(P.w[p], a, s0);
                 s1 = fmaf(P.w[p], c, s1);
             }
-            s0 = warp_sum(s0);
-            s1 = warp_sum(s1);
+            float v[2] = {s0, s1};
+            warp_sums(v);
+            s0 = v[0];
+            s1 = v[1];
         }
         if (lane == 0) {
             part[0][warp] = s0;
@@ -151,8 +155,8 @@ extern "C" int lt_dn_experts_glu(const void* W, int ldw, const void* X, int ldx,
     }
     FewP P = {W, X, H, nullptr, nullptr, device_status_ptr(), ldw, ldx, ldh, F, K, *h_c, *h_epi};
     LT_REQUIRE(P.status != nullptr, "lt_dn_experts_glu: status word unavailable");
-    const long need = ((long)h_c->T * h_c->top * F + FEW_THREADS / 32 - 1) / (FEW_THREADS / 32);
-    const int grid = (int)(need < 2L * sm_count() ? need : 2L * sm_count());
+    const long need = ((long)h_c->T * h_c->top * F + FEW_THREADS / 32 - 1) / (FEW_THREADS / 32), most = (long)FEW_CTAS * sm_count();
+    const int grid = (int)(need < most ? need : most);
     if (f32) k_few_glu<float><<<grid, FEW_THREADS, 0, (cudaStream_t)stream>>>(P);
     else k_few_glu<bf16><<<grid, FEW_THREADS, 0, (cudaStream_t)stream>>>(P);
     return check_launch("lt_dn_experts_glu");
@@ -181,7 +185,7 @@ extern "C" int lt_dn_experts_sum(const void* W, int ldw, const void* H, int ldh,
     int wj = 1;
     while (wj < h_c->top && wj < FEW_THREADS / 32) wj *= 2;
     const int pairs = FEW_THREADS / 32 / wj, need = ((M + 1) / 2 + pairs - 1) / pairs;
-    const int most = (2 * sm_count() + h_c->T - 1) / h_c->T;
+    const int most = (FEW_CTAS * sm_count() + h_c->T - 1) / h_c->T;
     const dim3 grid(need < most ? need : most, h_c->T);
     if (f32) k_few_sum<float><<<grid, FEW_THREADS, 0, (cudaStream_t)stream>>>(P, wj);
     else k_few_sum<bf16><<<grid, FEW_THREADS, 0, (cudaStream_t)stream>>>(P, wj);

@@ -323,14 +323,14 @@ static int pick_group_tc(const GroupP& P, cudaStream_t s) {
 
 // ---------------------------------------------------------------------------- fp32
 
-// 64 weight rows (with GLU: and their 64 up rows) x 32 places of one expert per CTA of 128 threads; a thread owns 4 rows x 4
+// 64 weight rows (with GLU: and their 64 up rows) x 8 MQ places of one expert per CTA of 128 threads; a thread owns 4 rows x MQ
 // places, 16-byte reads of shared memory, three stages of 32 k filled by asynchronous copies.  k is added up 256 at a time, so that
-// chains of roundings stay short.
-constexpr int GF_THREADS = 128, GF_BM = 64, GF_BN = 32, GF_BK = 32, GF_ST = GF_BK + 4, GF_STAGES = 3, GF_PART = 8;
+// chains of roundings stay short.  Instructions bound it, and places that a tile has no use for cost as many as the others.
+constexpr int GF_THREADS = 128, GF_BM = 64, GF_BK = 32, GF_ST = GF_BK + 4, GF_STAGES = 3, GF_PART = 8;
 
-template <bool GLU>
+template <bool GLU, int MQ>
 __global__ void __launch_bounds__(GF_THREADS) k_group_f32(const __grid_constant__ GroupP P) {
-    constexpr int NG = GLU ? 2 : 1, ROWS = NG * GF_BM + GF_BN;
+    constexpr int GF_BN = 8 * MQ, NG = GLU ? 2 : 1, ROWS = NG * GF_BM + GF_BN;
     extern __shared__ __align__(16) float gf_smem[];
     __shared__ int place[GF_BN];
     __shared__ int found[3];                 // expert, first place in the list, places
@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(GF_THREADS) k_group_f32(const __grid_constant_
         if (!done && lane == 0) found[2] = 0;
         __syncwarp();
         const int count = found[2];
-        if (count > 0) place[lane] = P.c.plan[P.c.n + 1 + found[1] + min(lane, count - 1)];
+        if (count > 0 && lane < GF_BN) place[lane] = P.c.plan[P.c.n + 1 + found[1] + min(lane, count - 1)];
     }
     __syncthreads();
     const int count = found[2];
@@ -389,11 +389,11 @@ __global__ void __launch_bounds__(GF_THREADS) k_group_f32(const __grid_constant_
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    float acc[NG][4][4], all[NG][4][4];
+    float acc[NG][MQ][4], all[NG][MQ][4];
 #pragma unroll
     for (int a = 0; a < NG; a++)
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int i = 0; i < MQ; i++)
 #pragma unroll
             for (int j = 0; j < 4; j++) acc[a][i][j] = all[a][i][j] = 0.0f;
 #pragma unroll
@@ -404,19 +404,19 @@ __global__ void __launch_bounds__(GF_THREADS) k_group_f32(const __grid_constant_
         __syncthreads();                                   // chunk c is there, chunk c - 1 is used up
         copy(c + GF_STAGES - 1, stage == 0 ? GF_STAGES - 1 : stage - 1);
         const float4* w4 = (const float4*)(gf_smem + (stage * ROWS + n) * GF_ST);
-        const float4* x4 = (const float4*)(gf_smem + (stage * ROWS + NG * GF_BM + m * 4) * GF_ST);
+        const float4* x4 = (const float4*)(gf_smem + (stage * ROWS + NG * GF_BM + m * MQ) * GF_ST);
 #pragma unroll 4
         for (int k = 0; k < GF_BK / 4; k++) {
-            float4 x[4];
+            float4 x[MQ];
 #pragma unroll
-            for (int i = 0; i < 4; i++) x[i] = x4[i * (GF_ST / 4) + k];
+            for (int i = 0; i < MQ; i++) x[i] = x4[i * (GF_ST / 4) + k];
 #pragma unroll
             for (int a = 0; a < NG; a++) {
                 float4 w[4];
 #pragma unroll
                 for (int j = 0; j < 4; j++) w[j] = w4[(a * GF_BM + 16 * j) * (GF_ST / 4) + k];
 #pragma unroll
-                for (int i = 0; i < 4; i++)
+                for (int i = 0; i < MQ; i++)
 #pragma unroll
                     for (int j = 0; j < 4; j++)
                         acc[a][i][j] = fmaf(w[j].w, x[i].w, fmaf(w[j].z, x[i].z, fmaf(w[j].y, x[i].y, fmaf(w[j].x, x[i].x, acc[a][i][j]))));
@@ -427,7 +427,7 @@ __global__ void __launch_bounds__(GF_THREADS) k_group_f32(const __grid_constant_
 #pragma unroll
             for (int a = 0; a < NG; a++)
 #pragma unroll
-                for (int i = 0; i < 4; i++)
+                for (int i = 0; i < MQ; i++)
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
                         all[a][i][j] += acc[a][i][j];
@@ -437,9 +437,9 @@ __global__ void __launch_bounds__(GF_THREADS) k_group_f32(const __grid_constant_
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        if (m * 4 + i >= count) break;
-        const long y = (long)place[m * 4 + i] * P.ldy;
+    for (int i = 0; i < MQ; i++) {
+        if (m * MQ + i >= count) break;
+        const long y = (long)place[m * MQ + i] * P.ldy;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const int row = n0 + n + 16 * j;
@@ -450,20 +450,27 @@ __global__ void __launch_bounds__(GF_THREADS) k_group_f32(const __grid_constant_
     }
 }
 
-template <bool GLU>
+template <bool GLU, int MQ>
 static int launch_group_f32(const GroupP& P, cudaStream_t s) {
-    constexpr int SMEM = GF_STAGES * ((GLU ? 2 : 1) * GF_BM + GF_BN) * GF_ST * 4;
+    constexpr int BN = 8 * MQ, SMEM = GF_STAGES * ((GLU ? 2 : 1) * GF_BM + BN) * GF_ST * 4;
     static PerDeviceOnce once;
-    if (once.first()) LT_CUDA(cudaFuncSetAttribute(k_group_f32<GLU>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+    if (once.first()) LT_CUDA(cudaFuncSetAttribute(k_group_f32<GLU, MQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
     const long places = (long)P.c.T * P.c.top;
-    const long tiles = places < P.c.n ? places : P.c.n + (places - P.c.n) / GF_BN;        // at most: one begun by every expert
+    const long tiles = places < P.c.n ? places : P.c.n + (places - P.c.n) / BN;        // at most: one begun by every expert
     LT_REQUIRE(tiles <= 65535, "experts' products: %ld places in fp32", places);
-    k_group_f32<GLU><<<dim3((P.M + GF_BM - 1) / GF_BM, (unsigned)tiles), GF_THREADS, SMEM, s>>>(P);
+    k_group_f32<GLU, MQ><<<dim3((P.M + GF_BM - 1) / GF_BM, (unsigned)tiles), GF_THREADS, SMEM, s>>>(P);
     return check_launch("experts' products");
+}
+template <bool GLU>
+static int pick_group_f32(const GroupP& P, cudaStream_t s) {
+    const long each = (long)P.c.T * P.c.top / P.c.n;        // places of an expert
+    if (each <= 6) return launch_group_f32<GLU, 1>(P, s);
+    if (each <= 14) return launch_group_f32<GLU, 2>(P, s);
+    return launch_group_f32<GLU, 4>(P, s);
 }
 
 int launch_group(GroupP P, bool glu, bool f32, cudaStream_t s) {
-    if (f32) return glu ? launch_group_f32<true>(P, s) : launch_group_f32<false>(P, s);
+    if (f32) return glu ? pick_group_f32<true>(P, s) : pick_group_f32<false>(P, s);
     return glu ? pick_group_tc<true>(P, s) : pick_group_tc<false>(P, s);
 }
 

@@ -3,9 +3,11 @@
 //
 //   s = softmax(l) or sigmoid(l),  c = s + bias,  the top of c inside the best groups,  w = s / sum of the chosen s * scale
 //
-// k_route: a warp per token, scores in registers.  Scores and choice values are doubles: whether an expert is among the top
-// depends on the last bits of values that lie close together, and 64 bits make the choice the same whatever order a sum is
-// taken in.  The choice is made on the bits of c, which order like the numbers, by integer reductions over the warp.
+// k_route: a warp per token.  Scores and choice values are doubles: whether an expert is among the top depends on the last bits of
+// values that lie close together, and 64 bits make the choice the same whatever order a sum is taken in.  The choice is made on the
+// bits of c, which order like the numbers, by integer reductions over the warp; the scores of the chosen are made once more at the
+// end, a lane each, instead of being carried along.  A group's experts are shared by consecutive lanes, so that a lane is kept or
+// dropped as a whole.  (2048 tokens, top 8 of 256 in 4 of 8 groups: instructions bound it, half of them in the picks.)
 // k_plan: a CTA per expert counts the places of lower experts and lists its own in order.  Every CTA reads all ids, so no CTA
 // waits for another and the order does not depend on timing.
 #include "lt_dn_common.cuh"
@@ -44,84 +46,75 @@ __device__ __forceinline__ int warp_best(unsigned long long key, int index) {
     return (int)__reduce_min_sync(0xffffffffu, hi == mh && lo == ml ? (unsigned)index : 0xffffffffu);
 }
 
-// VPL: experts of a lane, lane + 32 i
+__device__ __forceinline__ float clean_logit(float x) { return x != x ? -INFINITY : fminf(x, 3.402823466e38f); }
+__device__ __forceinline__ double key_value(unsigned long long k) {
+    return __longlong_as_double((long long)((k >> 63) ? k & 0x7fffffffffffffffull : ~k));
+}
+
+// VPL: experts of a lane at most; `each` lanes share a group, `own` experts a lane
 template <int VPL>
-__global__ void __launch_bounds__(32 * ROUTE_WARPS) k_route(const __grid_constant__ RouteP P) {
-    extern __shared__ __align__(16) unsigned char route_smem[];
+__global__ void __launch_bounds__(32 * ROUTE_WARPS) k_route(const __grid_constant__ RouteP P, int each, int own) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int t = blockIdx.x * ROUTE_WARPS + warp;
     if (t >= P.T) return;
     const lt_dn_router& R = P.R;
     const float* l = P.logits + (long)t * P.ld;
-    double s[VPL];
+    const int group = lane / each, size = R.n / R.groups, in = (lane - group * each) * own;      // first expert, inside the group
+    const int first = group * size + in, mine = group < R.groups ? max(0, min(own, size - in)) : 0;
     unsigned long long key[VPL];
     float x[VPL], m = -INFINITY;
 #pragma unroll
     for (int i = 0; i < VPL; i++) {
-        const int e = lane + 32 * i;
-        x[i] = e < R.n ? l[e] : -INFINITY;
-        if (x[i] != x[i]) x[i] = -INFINITY;
-        x[i] = fminf(x[i], 3.402823466e38f);
+        x[i] = i < mine ? clean_logit(l[first + i]) : -INFINITY;
         m = fmaxf(m, x[i]);
     }
-    if (R.score == LT_DN_SCORE_SOFTMAX) {
-        m = warp_max(m);
-        double sum = 0.0;
-#pragma unroll
-        for (int i = 0; i < VPL; i++) {
-            s[i] = x[i] == -INFINITY ? 0.0 : exp((double)x[i] - (double)m);
-            sum += s[i];
-        }
-        sum = warp_add(sum);
-#pragma unroll
-        for (int i = 0; i < VPL; i++) s[i] = sum > 0.0 ? s[i] / sum : 0.0;
-    } else {
-#pragma unroll
-        for (int i = 0; i < VPL; i++) s[i] = x[i] == -INFINITY ? 0.0 : 1.0 / (1.0 + exp(-(double)x[i]));
-    }
+    double sum = 0.0;
+    const bool softmax = R.score == LT_DN_SCORE_SOFTMAX;
+    if (softmax) m = warp_max(m);
 #pragma unroll
     for (int i = 0; i < VPL; i++) {
-        const int e = lane + 32 * i;
-        double c = s[i];
-        if (R.bias != nullptr && e < R.n) c += (double)R.bias[e];
-        key[i] = e < R.n ? order_key(x[i] == -INFINITY ? -INFINITY : c) : 0ull;
+        double e = 0.0;
+        if (x[i] != -INFINITY) e = exp(softmax ? (double)x[i] - (double)m : -(double)x[i]);
+        sum += e;
+        key[i] = (unsigned long long)__double_as_longlong(e);
+    }
+    if (softmax) sum = warp_add(sum);
+    const double inv = sum > 0.0 ? 1.0 / sum : 0.0;
+#pragma unroll
+    for (int i = 0; i < VPL; i++) {
+        const double e = __longlong_as_double((long long)key[i]);
+        double c = softmax ? e * inv : 1.0 / (1.0 + e);
+        if (R.bias != nullptr && i < mine) c += (double)R.bias[first + i];
+        key[i] = i < mine ? order_key(x[i] == -INFINITY ? -INFINITY : c) : 0ull;
     }
     if (R.groups > 1) {
-        double* c = (double*)route_smem + warp * (R.n + R.groups);    // a word between the groups: no bank conflicts
-        const int size = R.n / R.groups;
+        unsigned long long a = 0ull, b = 0ull;           // the two best of the lane, then of the group
 #pragma unroll
         for (int i = 0; i < VPL; i++) {
-            const int e = lane + 32 * i;
-            if (e < R.n) {
-                const unsigned long long k = key[i];
-                c[e + e / size] = __longlong_as_double((long long)((k >> 63) ? k & 0x7fffffffffffffffull : ~k));
-            }
+            const unsigned long long low = min(a, key[i]);
+            a = max(a, key[i]);
+            b = max(b, low);
         }
-        __syncwarp();
+        for (int s = 1; s < each; s <<= 1) {
+            const unsigned long long oa = __shfl_xor_sync(0xffffffffu, a, s), ob = __shfl_xor_sync(0xffffffffu, b, s);
+            b = max(min(a, oa), max(b, ob));
+            a = max(a, oa);
+        }
         unsigned long long gkey = 0ull;
-        if (lane < R.groups) {
-            double a = -INFINITY, b = -INFINITY;
-            for (int i = 0; i < size; i++) {
-                const double v = c[lane * (size + 1) + i];
-                b = fmax(b, fmin(a, v));
-                a = fmax(a, v);
-            }
-            gkey = order_key(size > 1 ? a + b : a);
-        }
+        if (lane - group * each == 0 && group < R.groups) gkey = order_key(size > 1 ? key_value(a) + key_value(b) : key_value(a));
         unsigned kept = 0;
         for (int i = 0; i < R.top_groups; i++) {
-            const int g = warp_best(gkey, lane);
+            const int g = warp_best(gkey, group);
             kept |= 1u << g;
-            if (lane == g) gkey = 0ull;
+            if (group == g) gkey = 0ull;
         }
+        if (!((kept >> group) & 1)) {
 #pragma unroll
-        for (int i = 0; i < VPL; i++) {
-            const int e = lane + 32 * i;
-            if (e < R.n && !((kept >> (e / size)) & 1)) key[i] = KEY_DROPPED;
+            for (int i = 0; i < VPL; i++)
+                if (i < mine) key[i] = KEY_DROPPED;
         }
     }
-    double total = 0.0, mine = 0.0;      // lane j keeps the score of choice j (and j + 32 is never needed: top <= 32)
-    int chosen = 0;
+    int chosen = 0;                      // of place `lane`
     for (int j = 0; j < R.top; j++) {
         unsigned long long best = key[0];
         int at = 0;
@@ -131,32 +124,34 @@ __global__ void __launch_bounds__(32 * ROUTE_WARPS) k_route(const __grid_constan
                 best = key[i];
                 at = i;
             }
-        const int e = warp_best(best, lane + 32 * at);
-        double v = 0.0;
+        const int e = warp_best(best, first + at);
+        if (lane == j) chosen = e;
+        const bool here = e >= first && e < first + mine;
 #pragma unroll
         for (int i = 0; i < VPL; i++)
-            if (lane + 32 * i == e) {
-                v = s[i];
-                key[i] = 0ull;
-            }
-        v = __shfl_sync(0xffffffffu, v, e & 31);
-        total += v;
-        if (lane == j) {
-            mine = v;
-            chosen = e;
+            if (here && i == at) key[i] = 0ull;
+    }
+    double s = 0.0;
+    if (lane < R.top) {
+        const float v = clean_logit(l[chosen]);
+        if (v != -INFINITY) {
+            const double e = exp(softmax ? (double)v - (double)m : -(double)v);
+            s = softmax ? e * inv : 1.0 / (1.0 + e);
         }
     }
+    if (R.renorm) {
+        const double total = warp_add(s);
+        s = total > 0.0 ? s / total : 0.0;
+    }
     if (lane < R.top) {
-        if (R.renorm) mine = total > 0.0 ? mine / total : 0.0;
         P.ids[(long)t * R.top + lane] = chosen;
-        P.w[(long)t * R.top + lane] = (float)(mine * (double)R.scale);
+        P.w[(long)t * R.top + lane] = (float)(s * (double)R.scale);
     }
 }
 
 template <int VPL>
-static int launch_route(const RouteP& P, cudaStream_t s) {
-    const size_t smem = P.R.groups > 1 ? (size_t)ROUTE_WARPS * (P.R.n + P.R.groups) * 8 : 0;
-    k_route<VPL><<<(P.T + ROUTE_WARPS - 1) / ROUTE_WARPS, 32 * ROUTE_WARPS, smem, s>>>(P);
+static int launch_route(const RouteP& P, int each, int own, cudaStream_t s) {
+    k_route<VPL><<<(P.T + ROUTE_WARPS - 1) / ROUTE_WARPS, 32 * ROUTE_WARPS, 0, s>>>(P, each, own);
     return check_launch("lt_dn_route");
 }
 
@@ -236,11 +231,15 @@ extern "C" int lt_dn_route(const float* logits, int ld, int* ids, float* w, int 
                R.n / R.groups * R.top_groups);
     RouteP P = {logits, ids, w, ld, T, R};
     cudaStream_t s = (cudaStream_t)stream;
-    if (R.n <= 64) return launch_route<2>(P, s);
-    if (R.n <= 128) return launch_route<4>(P, s);
-    if (R.n <= 256) return launch_route<8>(P, s);
-    if (R.n <= 512) return launch_route<16>(P, s);
-    return launch_route<32>(P, s);
+    int each = 32;
+    while (each * R.groups > 32) each /= 2;
+    const int size = R.n / R.groups, own = (size + each - 1) / each;
+    if (own <= 2) return launch_route<2>(P, each, own, s);
+    if (own <= 4) return launch_route<4>(P, each, own, s);
+    if (own <= 8) return launch_route<8>(P, each, own, s);
+    if (own <= 16) return launch_route<16>(P, each, own, s);
+    if (own <= 32) return launch_route<32>(P, each, own, s);
+    return launch_route<64>(P, each, own, s);       // more than 16 groups that are no power of two
 }
 
 extern "C" long lt_dn_experts_plan_ints(int T, int top, int n) { return (long)T * top + n + 1; }

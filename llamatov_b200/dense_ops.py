@@ -122,6 +122,11 @@ def cast_input(x, n1, x2=None):
 
 # --------------------------------------------------------------------------- sparse feed-forwards
 
+def _stream():
+    """The current stream's handle, as dev_residency._stream, without the Stream object that it makes (3 us of a call's 8)."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+
+
 def _here(t, what):
     """Launches go to the current device: an operand of another one is refused."""
     if t.device.type != "cuda" or t.device.index != torch.cuda.current_device():
@@ -151,7 +156,7 @@ class Router:
 
     def rows(self, logits, ld, ids, w, T):
         """ids int32 [T][top] and w fp32 [T][top] of T rows of logits."""
-        _lib.call("lt_dn_route", logits, ld, ids, w, T, self._ref, dr._stream())
+        _lib.call("lt_dn_route", logits, ld, ids, w, T, self._ref, _stream())
 
 
 class Places:
@@ -192,13 +197,13 @@ class Experts:
         if T * top < GROUP_FROM:
             return Places(ids, self.n)
         buf = torch.empty(_lib.dense().lt_dn_experts_plan_ints(T, top, self.n), dtype=torch.int32, device="cuda")
-        _lib.call("lt_dn_experts_plan", ids.data_ptr(), T, top, self.n, buf.data_ptr(), dr._stream())
+        _lib.call("lt_dn_experts_plan", ids.data_ptr(), T, top, self.n, buf.data_ptr(), _stream())
         return Places(ids, self.n, buf)
 
     def hidden(self, x, ldx, places, h, ldh):
         """h[t*top + j] = glu of the gate and up rows of place (t, j)'s expert, for the rows of x."""
         _lib.call("lt_dn_experts_glu", self.ptr, self.K, x, ldx, h, ldh, self.f32, self.M, self.K, places.ref, ctypes.byref(self.epi),
-                  dr._stream())
+                  _stream())
 
     def add_sum(self, h, ldh, places, w, y, ldy, ls=None):
         """y[t] += ls * sum over j of w[t][j] W h[t*top + j]."""
@@ -206,7 +211,7 @@ class Experts:
         if places.buf is not None:
             buf = torch.empty(_lib.dense().lt_dn_experts_sum_ws(places.T, places.top, self.M), dtype=torch.float32, device="cuda")
             ws = buf.data_ptr()
-        _lib.call("lt_dn_experts_sum", self.ptr, self.K, h, ldh, y, ldy, self.f32, self.M, self.K, places.ref, w, ls, ws, dr._stream())
+        _lib.call("lt_dn_experts_sum", self.ptr, self.K, h, ldh, y, ldy, self.f32, self.M, self.K, places.ref, w, ls, ws, _stream())
 
 
 # --------------------------------------------------------------------------- delta rule
@@ -241,10 +246,10 @@ class DeltaRule:
                 at += r
             args = (q, k, v, ld, la, beta, ldh, o, ldo)
             if self.f32 or max(part) < DELTA_CHUNKED_FROM or self.dim > 256 or self.vdim > 512:
-                _lib.call("lt_dn_delta_rows", *args, self.f32, self._ref, ctypes.byref(seqs), dr._stream())
+                _lib.call("lt_dn_delta_rows", *args, self.f32, self._ref, ctypes.byref(seqs), _stream())
                 continue
             ws = torch.empty(_lib.dense().lt_dn_delta_chunked_ws(self._ref, ctypes.byref(seqs)), dtype=torch.float32, device="cuda")
-            _lib.call("lt_dn_delta_chunked", *args, self._ref, ctypes.byref(seqs), ws.data_ptr(), dr._stream())
+            _lib.call("lt_dn_delta_chunked", *args, self._ref, ctypes.byref(seqs), ws.data_ptr(), _stream())
 
     def step(self, row, dt, beta, ring, S, o, len_, ticket):
-        _lib.call("lt_dn_delta_step", row, dt, beta, ring, S, o, self.f32, len_, ticket, self._ref, dr._stream())
+        _lib.call("lt_dn_delta_step", row, dt, beta, ring, S, o, self.f32, len_, ticket, self._ref, _stream())

@@ -91,6 +91,8 @@ def test_delta_refusals():
     rows("share rows", q=seqs((0, 5, 256), (4, 5, 512)))
     rows("ldh=3", ldh=3)
     rows("ldo=95", ldo=95)
+    rows("alignment", ld=100)
+    rows("alignment", ldo=97)
     chunked = lambda text, d=delta(), q=seqs((0, 5, 256)), k=one, ld=96, ldo=96, ws=one: _refused(
         "lt_dn_delta_chunked", text, one, k, one, ld, one, one, 4, one, ldo, d, q, ws, None)
     chunked("above 256", delta(dp=264))
