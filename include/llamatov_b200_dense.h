@@ -221,7 +221,7 @@ int lt_dn_gqa_step(const void* y, void* kc, void* vc, void* vfirst, int vmix_sto
 /* Gated delta rule.  Per head, with k and q of its group (H a multiple of G) brought to unit length,
  *   k <- k / sqrt(sum k^2 + eps),  q <- q_scale * q / sqrt(sum q^2 + eps):
  *   S <- e^la_t S,  u = beta_t (v_t - S k_t),  S <- S + u k_t^T,  o_t = S q_t      (S fp32, stored [H][dvp][dp])
- * la (logarithms of the decays, <= 0 in a decaying memory; minus infinity forgets) and beta are fp32 [row][ldh]. */
+ * la (logarithms of the decays, <= 0 in a decaying memory; minus infinity forgets) and beta are fp32 [row][ldla], [row][ldb]. */
 typedef struct {
     int H, G, dp, dvp;       /* heads, key heads, padded key and value sizes */
     float q_scale, eps;      /* eps > 0 */
@@ -243,14 +243,14 @@ typedef struct {
 
 /* Rows of up to LT_DN_SEQS sequences, in token order.  q, k: element type, key head g at columns g*dp; v: head h at h*dvp; row
  * stride ld for all three.  o: fp32, row stride ldo. */
-int lt_dn_delta_rows(const void* q, const void* k, const void* v, int ld, const float* la, const float* beta, int ldh, float* o, int ldo,
-                     int f32, const lt_dn_delta* h_d, const lt_dn_seqs* h_q, void* stream);
+int lt_dn_delta_rows(const void* q, const void* k, const void* v, int ld, const float* la, int ldla, const float* beta, int ldb, float* o,
+                     int ldo, int f32, const lt_dn_delta* h_d, const lt_dn_seqs* h_q, void* stream);
 
 /* The same in chunks of 64 tokens on the tensor cores (bf16 only; dp <= 256, dvp <= 512; sums as exact as in token order).  ws: fp32
  * workspace of lt_dn_delta_chunked_ws elements. */
 long lt_dn_delta_chunked_ws(const lt_dn_delta* h_d, const lt_dn_seqs* h_q);
-int lt_dn_delta_chunked(const void* q, const void* k, const void* v, int ld, const float* la, const float* beta, int ldh, float* o, int ldo,
-                        const lt_dn_delta* h_d, const lt_dn_seqs* h_q, float* ws, void* stream);
+int lt_dn_delta_chunked(const void* q, const void* k, const void* v, int ld, const float* la, int ldla, const float* beta, int ldb, float* o,
+                        int ldo, const lt_dn_delta* h_d, const lt_dn_seqs* h_q, float* ws, void* stream);
 
 /* One token at position *len (then *len += 1): convolution, silu, step size la = A softplus(dt + dt_bias) and recurrence in one
  * launch.  vkq: one row, values (H*dvp), keys (G*dp), queries (G*dp), ahead of the convolution, whose last inputs are in the ring

@@ -172,8 +172,8 @@ DENSE_SIGNATURES = {
     "lt_dn_ssd_step": [_vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, ctypes.POINTER(DnSsd), _vp],
     "lt_dn_gqa_rows": [_vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, ctypes.POINTER(DnGqa), _vp],
     "lt_dn_gqa_attn": [_vp, _i, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, ctypes.POINTER(DnGqa), _vp],
-    "lt_dn_delta_rows": [_vp, _vp, _vp, _i, _vp, _vp, _i, _vp, _i, _i, ctypes.POINTER(DnDelta), ctypes.POINTER(DnSeqs), _vp],
-    "lt_dn_delta_chunked": [_vp, _vp, _vp, _i, _vp, _vp, _i, _vp, _i, ctypes.POINTER(DnDelta), ctypes.POINTER(DnSeqs), _vp, _vp],
+    "lt_dn_delta_rows": [_vp, _vp, _vp, _i, _vp, _i, _vp, _i, _vp, _i, _i, ctypes.POINTER(DnDelta), ctypes.POINTER(DnSeqs), _vp],
+    "lt_dn_delta_chunked": [_vp, _vp, _vp, _i, _vp, _i, _vp, _i, _vp, _i, ctypes.POINTER(DnDelta), ctypes.POINTER(DnSeqs), _vp, _vp],
     "lt_dn_delta_step": [_vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, ctypes.POINTER(DnDelta), _vp],
     "lt_dn_route": [_vp, _i, _vp, _vp, _i, ctypes.POINTER(DnRouter), _vp],
     "lt_dn_experts_plan": [_vp, _i, _i, _i, _vp, _vp],

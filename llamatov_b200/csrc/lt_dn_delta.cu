@@ -28,7 +28,7 @@ struct DeltaScanP {
     const float *la, *beta;
     float* o;
     int* status;
-    int ld, ldh, ldo;
+    int ld, ldla, ldb, ldo;
     lt_dn_delta D;
     lt_dn_seqs Q;
 };
@@ -165,8 +165,8 @@ __global__ void __launch_bounds__(DeltaScan<T, KPT, LN>::THREADS) k_delta_scan(c
             const bool ok = n < batches && blk < NB && t < rows;
             la = la_next;
             be = be_next;
-            la_next = ok ? P.la[(first + t) * P.ldh + h] : 0.0f;
-            be_next = ok ? P.beta[(first + t) * P.ldh + h] : 0.0f;
+            la_next = ok ? P.la[(first + t) * P.ldla + h] : 0.0f;
+            be_next = ok ? P.beta[(first + t) * P.ldb + h] : 0.0f;
         };
         auto make = [&](int n) {
             if (blk >= NB) return;
@@ -507,18 +507,18 @@ const char* delta_seqs_error(const lt_dn_seqs* Q, int* rows) {
 using namespace lt;
 using namespace lt::dn;
 
-extern "C" int lt_dn_delta_rows(const void* q, const void* k, const void* v, int ld, const float* la, const float* beta, int ldh, float* o,
+extern "C" int lt_dn_delta_rows(const void* q, const void* k, const void* v, int ld, const float* la, int ldla, const float* beta, int ldb, float* o,
                                 int ldo, int f32, const lt_dn_delta* h_d, const lt_dn_seqs* h_q, void* stream) {
     int rows = 0;
     const char* bad = delta_error(h_d);
     if (bad == nullptr) bad = delta_seqs_error(h_q, &rows);
     LT_REQUIRE(bad == nullptr, "lt_dn_delta_rows: %s", bad);
     LT_REQUIRE(q && k && v && la && beta && o, "lt_dn_delta_rows: null pointer");
-    LT_REQUIRE(ld >= h_d->G * h_d->dp && ld >= h_d->H * h_d->dvp && ldh >= h_d->H && ldo >= h_d->H * h_d->dvp,
-               "lt_dn_delta_rows: ld=%d ldh=%d ldo=%d", ld, ldh, ldo);
+    LT_REQUIRE(ld >= h_d->G * h_d->dp && ld >= h_d->H * h_d->dvp && ldla >= h_d->H && ldb >= h_d->H && ldo >= h_d->H * h_d->dvp,
+               "lt_dn_delta_rows: ld=%d ldla=%d ldb=%d ldo=%d", ld, ldla, ldb, ldo);
     LT_REQUIRE(ld % 8 == 0 && ldo % 2 == 0 && aligned16(q) && aligned16(k) && aligned16(v) && aligned16(o), "lt_dn_delta_rows: alignment");
     if (rows == 0) return LT_OK;
-    DeltaScanP P = {q, k, v, la, beta, o, device_status_ptr(), ld, ldh, ldo, *h_d, *h_q};
+    DeltaScanP P = {q, k, v, la, beta, o, device_status_ptr(), ld, ldla, ldb, ldo, *h_d, *h_q};
     LT_REQUIRE(P.status != nullptr, "lt_dn_delta_rows: status word unavailable");
     if (f32) return delta_scan_size<float>(P, (cudaStream_t)stream);
     return delta_scan_size<bf16>(P, (cudaStream_t)stream);

@@ -33,7 +33,7 @@ struct DeltaChunkP {
     float* o;
     bf16* T3;                // [chunk][H][3][64][64]
     float *vec, *S0, *U;     // [chunk][H]: [DVEC], [dvp][dp], [dvp][64]
-    int ld, ldh, ldo;
+    int ld, ldla, ldb, ldo;
     int first[LT_DN_SEQS + 1];    // chunks before a sequence's
     lt_dn_delta D;
     lt_dn_seqs Q;
@@ -68,8 +68,8 @@ __device__ __forceinline__ Chunk chunk_of(const DeltaChunkP& P, int c) {
 // sums of a chunk's log decays (base 2), by one warp: doubles, so that differences are exact
 __device__ __forceinline__ void log_sums(const DeltaChunkP& P, const Chunk& c, int h, int lane, double* sb) {
     const int t = 2 * lane;
-    const double l0 = t < c.rows ? (double)(delta_log(P.la[(c.row0 + t) * P.ldh + h]) * DLOG2E) : 0.0;
-    const double l1 = t + 1 < c.rows ? (double)(delta_log(P.la[(c.row0 + t + 1) * P.ldh + h]) * DLOG2E) : 0.0;
+    const double l0 = t < c.rows ? (double)(delta_log(P.la[(c.row0 + t) * P.ldla + h]) * DLOG2E) : 0.0;
+    const double l1 = t + 1 < c.rows ? (double)(delta_log(P.la[(c.row0 + t + 1) * P.ldla + h]) * DLOG2E) : 0.0;
     double p = l0 + l1;
 #pragma unroll
     for (int s = 1; s < 32; s <<= 1) {
@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(PREP_THREADS) k_delta_prep(const __grid_consta
     load_rows(sk, KS, dpr / 8, P.k, c, P.ld, hq * P.D.dp, P.D.dp);
     asm volatile("cp.async.commit_group;" ::: "memory");
     if (warp == 0) log_sums(P, c, h, lane, sb);
-    if (tid >= 64 && tid < 128) sbeta[tid - 64] = tid - 64 < c.rows ? P.beta[(c.row0 + tid - 64) * P.ldh + h] : 0.0f;
+    if (tid >= 64 && tid < 128) sbeta[tid - 64] = tid - 64 < c.rows ? P.beta[(c.row0 + tid - 64) * P.ldb + h] : 0.0f;
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
     row_norms(sk, KS, dpr / 8, P.D.eps, 1.0f, sr);
@@ -682,7 +682,7 @@ extern "C" long lt_dn_delta_chunked_ws(const lt_dn_delta* h_d, const lt_dn_seqs*
     return delta_chunks(h_q) * h_d->H * delta_chunk_floats(h_d);
 }
 
-extern "C" int lt_dn_delta_chunked(const void* q, const void* k, const void* v, int ld, const float* la, const float* beta, int ldh, float* o,
+extern "C" int lt_dn_delta_chunked(const void* q, const void* k, const void* v, int ld, const float* la, int ldla, const float* beta, int ldb, float* o,
                                    int ldo, const lt_dn_delta* h_d, const lt_dn_seqs* h_q, float* ws, void* stream) {
     int rows = 0;
     const char* bad = delta_error(h_d);
@@ -690,13 +690,13 @@ extern "C" int lt_dn_delta_chunked(const void* q, const void* k, const void* v, 
     LT_REQUIRE(bad == nullptr, "lt_dn_delta_chunked: %s", bad);
     LT_REQUIRE(q && k && v && la && beta && o && ws, "lt_dn_delta_chunked: null pointer");
     LT_REQUIRE(h_d->dp <= 256 && h_d->dvp <= 512, "lt_dn_delta_chunked: head sizes %d and %d are above 256 and 512", h_d->dp, h_d->dvp);
-    LT_REQUIRE(ld >= h_d->G * h_d->dp && ld >= h_d->H * h_d->dvp && ldh >= h_d->H && ldo >= h_d->H * h_d->dvp, "lt_dn_delta_chunked: ld=%d ldh=%d ldo=%d",
-               ld, ldh, ldo);
+    LT_REQUIRE(ld >= h_d->G * h_d->dp && ld >= h_d->H * h_d->dvp && ldla >= h_d->H && ldb >= h_d->H && ldo >= h_d->H * h_d->dvp, "lt_dn_delta_chunked: ld=%d ldla=%d ldb=%d ldo=%d",
+               ld, ldla, ldb, ldo);
     LT_REQUIRE(ld % 8 == 0 && ldo % 2 == 0 && aligned16(q) && aligned16(k) && aligned16(v) && aligned16(o) && aligned16(ws), "lt_dn_delta_chunked: alignment");
     if (rows == 0) return LT_OK;
     DeltaChunkP P = {};
     P.q = (const bf16*)q; P.k = (const bf16*)k; P.v = (const bf16*)v; P.la = la; P.beta = beta; P.o = o;
-    P.ld = ld; P.ldh = ldh; P.ldo = ldo; P.D = *h_d; P.Q = *h_q;
+    P.ld = ld; P.ldla = ldla; P.ldb = ldb; P.ldo = ldo; P.D = *h_d; P.Q = *h_q;
     for (int i = 0; i < P.Q.n; i++) P.first[i + 1] = P.first[i] + (P.Q.rows[i] + DC - 1) / DC;
     for (int i = P.Q.n; i < LT_DN_SEQS; i++) P.first[i + 1] = P.first[P.Q.n];
     const int chunks = P.first[P.Q.n];

@@ -233,8 +233,10 @@ class DeltaRule:
                                                                                    for t in self.keep])
         self._ref = ctypes.byref(self.desc)
 
-    def rows(self, q, k, v, ld, la, beta, ldh, o, ldo, states, rows):
-        """Consecutive rows of sequences: rows[i] of them with the state at states[i], from row 0 on."""
+    def rows(self, q, k, v, ld, la, beta, ldh, o, ldo, states, rows, ldb=None):
+        """Consecutive rows of sequences: rows[i] of them with the state at states[i], from row 0 on.  la and beta have row stride
+        ldh, or beta ldb of its own."""
+        ldb = ldh if ldb is None else ldb
         if len(states) != len(rows):
             raise ValueError(f"{len(states)} states for {len(rows)} sequences")
         at = 0
@@ -244,7 +246,7 @@ class DeltaRule:
             for j, r in enumerate(part):
                 seqs.start[j], seqs.rows[j], seqs.S[j] = at, r, states[i + j]
                 at += r
-            args = (q, k, v, ld, la, beta, ldh, o, ldo)
+            args = (q, k, v, ld, la, ldh, beta, ldb, o, ldo)
             if self.f32 or max(part) < DELTA_CHUNKED_FROM or self.dim > 256 or self.vdim > 512:
                 _lib.call("lt_dn_delta_rows", *args, self.f32, self._ref, ctypes.byref(seqs), _stream())
                 continue

@@ -389,6 +389,19 @@ class DeviceSsdState(DeviceRecurrentState):
         self.ring = None
 
 
+class DeviceDeltaState(DeviceSsdState):
+    """State of a delta-rule mixer: as a state-space mixer's, and the counter that its token step finds at zero."""
+    __slots__ = ("ticket",)
+
+    def __init__(self, heads, vdim, dim, taps, channels, dtype):
+        super().__init__(heads, vdim, dim, taps, channels, dtype)
+        self.ticket = torch.zeros(1, dtype=torch.int32, device="cuda")
+
+    def free(self):
+        super().free()
+        self.ticket = None
+
+
 class DeviceGroupedKV(_PositionCounter):
     """Key and value rows of grouped-query attention in the model's element type, position p in row p of `cap`, with a
     device-side length counter."""

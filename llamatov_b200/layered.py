@@ -4,6 +4,7 @@ residual stream in fp32.  Mixers and feed-forwards are in `mixers`; a block puts
   SequentialBlock   x <- x + ls1 * mixer(norm1(x)), x <- x + ls2 * ff(norm2(x))
   ParallelBlock     h = norm1(x), x <- x + m * (mixer(h) + ff(h)).  The projections of h are one stacked matrix, and so are the
                     two output projections: a token's layer is one launch into the block, the mixer's core, one out of it
+                    (a feed-forward of experts stays apart)
 
 A design (`Layered` and its subclasses) says which block, mixers and feed-forwards it has, and how its config is read:
 
@@ -18,7 +19,7 @@ import torch
 from . import _lib, archs
 from . import dev_residency as dr
 from .dense_ops import (DTYPES, Linear, Norm, _pad_cols, _pad_rows, cast_input, epilogue, pad8, typed_input, with_tail)
-from .mixers import MIXERS, clamped_feed_forward, gelu_feed_forward
+from .mixers import MIXERS, clamped_experts, clamped_feed_forward, gelu_experts, gelu_feed_forward
 
 
 class DenseWeights(dict):
@@ -64,6 +65,7 @@ class SequentialBlock(Block):
         del mixer.w_in, mixer.w_out
         if ff is not None:
             self.norm2, self.ls2 = norm("norm2"), scale("ls2")
+        if ff is not None and not ff.routed:
             self.gu, self.down = Linear(ff.w_gu, pk.dtype), Linear(ff.w_down, pk.dtype)
             self.epi_glu = epilogue(_lib.DN_GLU, glu=ff.glu)
             self.epi_down = epilogue(_lib.DN_RESID, ls=self.ls2)
@@ -75,7 +77,11 @@ class SequentialBlock(Block):
         y, mid, tail = b.y.data_ptr(), b.mid.data_ptr(), b.tail.data_ptr()
         self.inp.row(self.norm1.prologue(x), y, with_tail(self.epi_in, tail, m.ntail) if m.ntail else self.epi_in)
         self.out.row(m.step_core(pk, y, tail, mid, cache), x, self.epi_out)
-        if self.ff is not None:
+        if self.ff is not None and self.ff.routed:
+            h = b.h.data_ptr()
+            self.norm2.rows(x, pk.Ep, h, pk.Ep, pk.f32, 1, pk.Ep)
+            self.ff.step(pk, h, x, self.ls2)
+        elif self.ff is not None:
             self.gu.row(self.norm2.prologue(x), mid, self.epi_glu, M=self.ff.F)
             self.down.row(typed_input(mid), x, self.epi_down)
 
@@ -87,7 +93,10 @@ class SequentialBlock(Block):
         X = st.buf("mid", R * m.nin, pk.dtype)
         m.rows_core(pk, st, y, tail, X, m.nin, caches)
         self.out.rows(X, m.nin, st.x, Ep, R, self.epi_out)
-        if self.ff is not None:
+        if self.ff is not None and self.ff.routed:
+            self.norm2.rows(st.x, Ep, h, Ep, pk.f32, R, Ep)
+            self.ff.rows(pk, st, h, st.x, self.ls2)
+        elif self.ff is not None:
             F = self.ff.F
             self.norm2.rows(st.x, Ep, h, Ep, pk.f32, R, Ep)
             f = st.buf("f", R * F, pk.dtype)
@@ -99,7 +108,8 @@ class ParallelBlock(Block):
     def __init__(self, pk, cfg, mixer, ff, norm, scale):
         self.norm1 = norm("norm1")
         self._input(pk, mixer)
-        F = self.F = 0 if ff is None else ff.F
+        self.experts = ff if ff is not None and ff.routed else None
+        F = self.F = 0 if ff is None or ff.routed else ff.F
         self.nm = mixer.width + mixer.ntail                 # matrix rows of the mixer; gate and up rows follow
         w_in, w_out = mixer.w_in, mixer.w_out
         del mixer.w_in, mixer.w_out
@@ -120,11 +130,15 @@ class ParallelBlock(Block):
         if F:
             e.kind, e.glu_from, e.y2 = _lib.DN_STORE_GLU, self.nm, f
             e.glu_act, e.glu_alpha, e.glu_limit = self.epi_glu.glu_act, self.epi_glu.glu_alpha, self.epi_glu.glu_limit
+        if self.experts is not None:             # of the row as it is ahead of the block
+            self.norm1.rows(x, pk.Ep, b.h.data_ptr(), pk.Ep, pk.f32, 1, pk.Ep)
         self.inp.row(self.norm1.prologue(x), y, e, M=self.nm + F)
         pro = m.step_core(pk, y, tail, mid, cache)
         if F and pro.kind == _lib.DN_IN_NORM:
             pro.n1, pro.x2 = m.nin, f                       # a typed input already has f behind it
         self.out.row(pro, x, self.epi_out)
+        if self.experts is not None:
+            self.experts.step(pk, b.h.data_ptr(), x, self.mult)
 
     def rows(self, pk, st, caches):
         R, Ep, m, F = st.R, st.ldx, self.mixer, self.F
@@ -137,6 +151,8 @@ class ParallelBlock(Block):
             self.inp.rows(h, Ep, X + m.nin * pk.esize, ld, R, self.epi_glu, M=F, first=self.nm)
         m.rows_core(pk, st, y, tail, X, ld, caches)
         self.out.rows(X, ld, st.x, Ep, R, self.epi_out)
+        if self.experts is not None:
+            self.experts.rows(pk, st, h, st.x, self.mult)
 
 
 # --------------------------------------------------------------------------- a model's packed weights
@@ -196,8 +212,9 @@ class Packed:
         b.x = [torch.zeros(Ep, **f32), torch.zeros(Ep, **f32)]
         b.x0 = torch.zeros(Ep, **f32)
         typed = dict(dtype=self.dtype, device="cuda")
-        b.y, b.mid, b.vfirst = [torch.zeros(max(n.get(k, 0), 8), **typed) for k in ("y", "mid", "vfirst")]
-        b.o, b.tail, b.ws = [torch.zeros(max(n.get(k, 0), 8), **f32) for k in ("o", "tail", "ws")]
+        b.y, b.mid, b.vfirst, b.h, b.hidden = [torch.zeros(max(n.get(k, 0), 8), **typed) for k in ("y", "mid", "vfirst", "h", "hidden")]
+        b.o, b.tail, b.ws, b.scores, b.weights = [torch.zeros(max(n.get(k, 0), 8), **f32) for k in ("o", "tail", "ws", "scores", "weights")]
+        b.ids = torch.zeros(max(n.get("ids", 0), 1), dtype=torch.int32, device="cuda")
         b.tickets = torch.zeros(max(n.get("tickets", 0), 1), dtype=torch.int32, device="cuda")
         b.tok = torch.zeros(1, dtype=torch.int32, device="cuda")
         b.cur = 0
@@ -245,7 +262,7 @@ class Layered(archs.Architecture):
     device_token = True
     max_rows = 2048
     mixers = MIXERS
-    feed_forwards = {"dense": gelu_feed_forward}
+    feed_forwards = {"dense": gelu_feed_forward, "experts": gelu_experts}
     block = SequentialBlock
     norm_offset = 0.0       # added to stored norm weights
     embed_norm = False      # the embedding row is normed ("embed.norm")
@@ -352,7 +369,7 @@ class Layered(archs.Architecture):
 
 
 class Pakalix(Layered):
-    feed_forwards = {"dense": clamped_feed_forward}
+    feed_forwards = {"dense": clamped_feed_forward, "experts": clamped_experts}
     block = ParallelBlock
     norm_offset = 1.0
     embed_norm = True

@@ -6,6 +6,7 @@ list the same mixers with other numbers:
                          (a decay per key channel from a low-rank projection, norm per head) and "lightning" (a constant
                          decay per head, activations on q, k, v, norm over all heads)
   Mamba2Mixer            state-space recurrence with step sizes per token and head behind a short convolution
+  GatedDeltaMixer        gated delta rule: a decaying fp32 state that is corrected instead of added to, behind a short convolution
   LatentAttentionMixer   attention over a sliding window with keys and values projected from a cached latent
   GroupedAttentionMixer  grouped-query attention over all positions: normed and rotated queries and keys, capped scores,
                          values mixed with an earlier layer's, a gate per head
@@ -26,7 +27,8 @@ import torch
 
 from . import _lib
 from . import dev_residency as dr
-from .dense_ops import (DTYPES, Linear, Norm, _head_cols, _head_rows, _pad_cols, _pad_rows, epilogue, pad8, typed_input)
+from .dense_ops import (DTYPES, DeltaRule, Experts, Linear, Norm, Places, Router, _head_cols, _head_rows, _pad_cols, _pad_rows, epilogue, pad8,
+                        typed_input)
 
 # bf16 portions of at least this many tokens take the chunked form of the recurrence, for head sizes up to the limit
 CHUNKED_FROM = 64
@@ -196,6 +198,71 @@ class Mamba2Mixer:
         self.norm.rows(o, self.nv, X, ldx, pk.f32, R, self.nv, gate=y, ldg=w)
 
 
+class GatedDeltaMixer:
+    """S <- e^(A dt_t) S, then S <- S + beta_t (v_t - S k_t) k_t^T, o_t = S q_t per head; v, k and q pass a causal convolution and silu, k
+    and q are brought to unit length (q times dim^-0.5) and shared by the heads of a group, dt is softplus(dt + bias), beta a
+    sigmoid.  The output is W_o of norm(o) * silu(z), the norm per head."""
+    NORM_EPS = 1e-6          # of the unit keys and queries
+
+    def __init__(self, pk, cfg, m, tensor):
+        E, eps = cfg["n_embd"], cfg["norm_eps"]
+        H, G, d, dv, taps = m["heads"], m["key_heads"], m["dim"], m["vdim"], m["conv"]
+        if H % G:
+            raise ValueError(f"{H} heads on {G} key heads")
+        nv, nk = H * dv, G * d
+        if tuple(tensor("conv").shape) != (nv + 2 * nk, taps):
+            raise ValueError(f"convolution {tuple(tensor('conv').shape)} for {nv + 2 * nk} channels and {taps} taps")
+        self.H, self.G, self.dp, self.dvp, self.taps = H, G, pad8(d), pad8(dv), taps
+        self.nv, self.nk = H * self.dvp, G * self.dp
+
+        def split(W):           # v | k | q, head by head
+            v, k, q = W.split([nv, nk, nk])
+            return torch.cat([_head_rows(v, [(dv, self.dvp)], H), _head_rows(k, [(d, self.dp)], G), _head_rows(q, [(d, self.dp)], G)])
+        z, vkq, dt, b = tensor("in").split([nv, nv + 2 * nk, H, H])
+        self.w_in = _pad_cols(torch.cat([_head_rows(z, [(dv, self.dvp)], H), split(vkq), dt, b]), pad8(E))
+        self.off_v, self.channels = self.nv, self.nv + 2 * self.nk
+        self.tail_from = self.width = self.nv + self.channels
+        self.ntail = 2 * H
+        self.segs = [(self.nv, "silu", 1.0), (self.width + H, None, 1.0), (self.width + 2 * H, "sigmoid", 1.0)]
+        f32 = lambda n: tensor(n).float().cuda().contiguous()
+        A = (-torch.exp(tensor("A_log").double())).float().cuda()
+        conv = split(tensor("conv").float()).T.contiguous().cuda()
+        self.keep = [conv, split(tensor("conv.b").float()).cuda(), f32("dt_bias"), A, torch.zeros(H, device="cuda")]
+        self.desc = _lib.DnSsd(H, G, self.dp, self.dvp, taps, *[t.data_ptr() for t in self.keep])      # of the rows' convolution
+        self.rule = DeltaRule(H, G, self.dp, self.dvp, pk.dtype, d ** -0.5, self.NORM_EPS, taps, conv, self.keep[1], self.keep[2], A)
+        self.norm = Norm(_pad_rows(tensor("norm").float(), self.dvp), dv, self.dvp, eps)
+        self.w_out = _pad_rows(_head_cols(tensor("o"), dv, H), pad8(E))
+        self.nin = self.nv
+        pk.want(o=self.nv)
+
+    def new_cache(self, cfg, max_rows):
+        return dr.DeviceDeltaState(self.H, self.dvp, self.dp, self.taps, self.channels, DTYPES[cfg["dtype"]])
+
+    def step_core(self, pk, y, tail, out, cache):
+        o = pk.step.o.data_ptr()
+        lp = cache._ensure_len_ptr(seed=not dr._capturing())
+        self.rule.step(y + self.off_v * pk.esize, tail, tail + self.H * 4, cache.ring.data_ptr(), cache.state.data_ptr(), o, lp,
+                       cache.ticket.data_ptr())
+        cache.length += 1
+        return self.norm.prologue(o, y)
+
+    def rows_core(self, pk, st, y, tail, X, ldx, caches):
+        e, T, R, w, H, C = pk.esize, st.T, st.R, self.width, self.H, self.channels
+        u = st.buf("conv", R * C, pk.dtype)
+        o = st.buf("o", R * self.nv, torch.float32)
+        hla, hdt = st.buf("hla", R * H, torch.float32), st.buf("hdt", R * H, torch.float32)
+        for b, c in enumerate(caches):
+            _lib.call("lt_dn_ssd_rows", y + (b * T * w + self.off_v) * e, w, tail + b * T * self.ntail * 4, self.ntail, c.ring.data_ptr(),
+                      u + b * T * C * e, C, hla + b * T * H * 4, hdt + b * T * H * 4, pk.f32, T, c.length, ctypes.byref(self.desc), dr._stream())
+        k = u + self.nv * e
+        self.rule.rows(k + self.nk * e, k, u, C, hla, tail + H * 4, H, o, self.nv, [c.state.data_ptr() for c in caches], [T] * len(caches),
+                       ldb=self.ntail)
+        for c in caches:
+            c.length += T
+            c._ensure_len_ptr()
+        self.norm.rows(o, self.nv, X, ldx, pk.f32, R, self.nv, gate=y, ldg=w)
+
+
 class LatentAttentionMixer:
     """Softmax attention over a sliding window.  A head's query and key have `dim` plain and `rot_dim` rotated components;
     plain keys and values are projections of a cached, normed latent, the rotated key part is shared by the heads."""
@@ -356,12 +423,13 @@ def _lightning(pk, cfg, m, tensor):
 
 
 MIXERS = {"gla": _gla, "lightning": _lightning, "latent_attention": LatentAttentionMixer, "mamba2": Mamba2Mixer,
-          "attention": GroupedAttentionMixer}
+          "attention": GroupedAttentionMixer, "gated_delta": GatedDeltaMixer}
 
 
 class GatedFeedForward:
     """W_down glu(W_gate h, W_up h); gate and up are one launch that stores the product.  `glu` is the gated activation as the
     epilogue takes it: (kind, alpha, limit)."""
+    routed = False           # its matrices are the same for every token, so that a block may stack them with a mixer's
 
     def __init__(self, pk, cfg, m, tensor, glu):
         E = pad8(cfg["n_embd"])
@@ -371,11 +439,87 @@ class GatedFeedForward:
         self.w_down = _pad_rows(_pad_cols(tensor("down"), F), E)
 
 
+class ExpertsFeedForward:
+    """Sum over a token's experts e of w_e W_down[e] glu(W_gate[e] h, W_up[e] h), the experts and weights chosen by a router, and the
+    same of one gated feed-forward for all tokens ("shared_ff").  Config: experts, top, ff; score ("softmax" or "sigmoid"), bias
+    (added for the choice alone), groups and top_groups, renorm, scale."""
+    routed = True
+
+    def __init__(self, pk, cfg, m, tensor, glu):
+        E, n = pad8(cfg["n_embd"]), m["experts"]
+        F = self.F = pad8(m["ff"])
+        self.n, self.top, self.Ep = n, m["top"], E
+        for name, shape in (("router", (n, cfg["n_embd"])), ("gate", (n, m["ff"], cfg["n_embd"])), ("up", (n, m["ff"], cfg["n_embd"])),
+                            ("down", (n, cfg["n_embd"], m["ff"]))):
+            if tuple(tensor(name).shape) != shape:
+                raise ValueError(f"{name} {tuple(tensor(name).shape)} for {n} experts of {m['ff']} and width {cfg['n_embd']}")
+        self.route = Router(n, self.top, m.get("score", "softmax"), tensor("router.bias") if m.get("bias") else None, m.get("groups", 1),
+                            m.get("top_groups", 1), m.get("renorm", True), m.get("scale", 1.0))
+
+        def padded(name, rows, cols):
+            W = tensor(name)
+            out = W.new_zeros(n, rows, cols)
+            out[:, :W.shape[1], :W.shape[2]] = W
+            return out.to(pk.dtype)
+        self.scores = Linear(_pad_cols(tensor("router"), E), pk.dtype)
+        self.epi_scores = epilogue(out_f32=True)
+        self.gu = Experts(torch.cat([padded("gate", F, E), padded("up", F, E)], dim=1), True, glu)
+        self.down = Experts(padded("down", E, F), False)
+        self.shared = None
+        if m.get("shared_ff"):
+            ff = GatedFeedForward(pk, cfg, {"ff": m["shared_ff"]}, lambda name: tensor("shared." + name), glu)
+            self.shared = (ff.F, Linear(ff.w_gu, pk.dtype), Linear(ff.w_down, pk.dtype), epilogue(_lib.DN_GLU, glu=glu))
+            pk.want(mid=ff.F)
+        self.places = None
+        pk.want(h=E, scores=n, weights=self.top, ids=self.top, hidden=self.top * F)
+
+    def step(self, pk, h, x, ls):
+        """x += ls * of the normed row h."""
+        b = pk.step
+        if self.places is None:
+            self.places = Places(b.ids[:self.top].reshape(1, self.top), self.n)
+        scores, w, hid = b.scores.data_ptr(), b.weights.data_ptr(), b.hidden.data_ptr()
+        self.scores.row(typed_input(h), scores, self.epi_scores)
+        self.route.rows(scores, self.n, b.ids.data_ptr(), w, 1)
+        self.gu.hidden(h, self.Ep, self.places, hid, self.F)
+        self.down.add_sum(hid, self.F, self.places, w, x, self.Ep, None if ls is None else ls.data_ptr())
+        if self.shared:
+            F, gu, down, epi = self.shared
+            gu.row(typed_input(h), b.mid.data_ptr(), epi, M=F)
+            down.row(typed_input(b.mid.data_ptr()), x, epilogue(_lib.DN_RESID, ls=ls))
+
+    def rows(self, pk, st, h, x, ls):
+        """The same of the rows of a pass."""
+        R, Ep, n, top = st.R, self.Ep, self.n, self.top
+        scores = st.buf("scores", R * n, torch.float32)
+        self.scores.rows(h, Ep, scores, n, R, self.epi_scores)
+        ids = torch.empty((R, top), dtype=torch.int32, device="cuda")
+        w = torch.empty((R, top), dtype=torch.float32, device="cuda")
+        self.route.rows(scores, n, ids.data_ptr(), w.data_ptr(), R)
+        places = self.gu.plan(ids, R)
+        hid = st.buf("hidden", R * top * self.F, pk.dtype)
+        self.gu.hidden(h, Ep, places, hid, self.F)
+        self.down.add_sum(hid, self.F, places, w.data_ptr(), x, Ep, None if ls is None else ls.data_ptr())
+        if self.shared:
+            F, gu, down, epi = self.shared
+            f = st.buf("f", R * F, pk.dtype)
+            gu.rows(h, Ep, f, F, R, epi, M=F)
+            down.rows(f, F, x, Ep, R, epilogue(_lib.DN_RESID, ls=ls))
+
+
 def gelu_feed_forward(pk, cfg, m, tensor):
     """glu(g, u) = gelu_tanh(g) * u"""
     return GatedFeedForward(pk, cfg, m, tensor, (_lib.DN_GLU_GELU, 0.0, 0.0))
 
 
+def gelu_experts(pk, cfg, m, tensor):
+    return ExpertsFeedForward(pk, cfg, m, tensor, (_lib.DN_GLU_GELU, 0.0, 0.0))
+
+
 def clamped_feed_forward(pk, cfg, m, tensor):
     """glu(g, u) = g' sigmoid(1.702 g') (u' + 1) with g' = min(g, limit) and u' = u clamped to [-limit, limit]"""
     return GatedFeedForward(pk, cfg, m, tensor, (_lib.DN_GLU_CLAMPED, 1.702, float(m["limit"])))
+
+
+def clamped_experts(pk, cfg, m, tensor):
+    return ExpertsFeedForward(pk, cfg, m, tensor, (_lib.DN_GLU_CLAMPED, 1.702, float(m["limit"])))

@@ -9,6 +9,8 @@ Notation: x residual stream [T, E]; h a normed input [T, E]; tensors are a dict 
 """
 import numpy as np
 
+from . import sparse
+
 F = np.float64
 
 
@@ -137,6 +139,8 @@ class Model:
             m = cfg["layers"][i]["mixer"]
             if cfg["layers"][i]["type"] == "latent_attention":
                 self.state.append({"c": [], "kr": []})
+            elif cfg["layers"][i]["type"] == "gated_delta":
+                self.state.append(sparse.new_state(m))
             else:
                 self.state.append(np.zeros((m["heads"], m["dim"], m["vdim"]), F))
         self.taps = []
@@ -149,11 +153,18 @@ class Model:
             y = gla(h, ly["mixer"], mix, eps, st)
         elif ly["type"] == "lightning":
             y = lightning(h, ly["mixer"], mix, eps, st)
+        elif ly["type"] == "gated_delta":
+            y = sparse.gated_delta(h, ly["mixer"], mix, eps, st)
         else:
             y = latent_attention(h, ly["mixer"], mix, eps, st, self.pos)
         x = x + y * self.w[p + "ls1"]
         if ly["mlp"] is not None:
-            x = x + feed_forward(rms(x, self.w[p + "norm2"], eps), lambda n: self.w[p + "mlp." + n]) * self.w[p + "ls2"]
+            h, mlp = rms(x, self.w[p + "norm2"], eps), lambda n: self.w[p + "mlp." + n]
+            if ly["mlp"].get("kind") == "experts":
+                y = sparse.experts(h, ly["mlp"], mlp, lambda g, u: gelu_tanh(g) * u)
+            else:
+                y = feed_forward(h, mlp)
+            x = x + y * self.w[p + "ls2"]
         return x
 
     def run(self, tokens):

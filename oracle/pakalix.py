@@ -9,6 +9,7 @@ Notation: x residual stream [T, E]; h a normed input [T, E]; tensors are a dict 
 """
 import numpy as np
 
+from . import sparse
 from .layered import F, linear, rms, rotate_half, sigmoid, silu
 
 
@@ -125,7 +126,9 @@ class Model:
         self.state = []
         for i, ly in enumerate(cfg["layers"]):
             m = ly["mixer"]
-            if ly["type"] == "mamba2":
+            if ly["type"] == "gated_delta":
+                self.state.append(sparse.new_state(m))
+            elif ly["type"] == "mamba2":
                 ch, taps = self.w[f"l{i}.mix.conv"].shape
                 self.state.append({"S": np.zeros((m["heads"], m["state"], m["vdim"]), F), "before": np.zeros((taps - 1, ch), F)})
             else:
@@ -139,11 +142,17 @@ class Model:
         for i, (ly, st) in enumerate(zip(cfg["layers"], self.state)):
             mix = lambda n: w[f"l{i}.mix." + n]
             h = one_plus_rms(x, w[f"l{i}.norm1"], eps)
-            if ly["type"] == "mamba2":
+            if ly["type"] == "gated_delta":
+                y = sparse.gated_delta(h, ly["mixer"], mix, eps, st)
+            elif ly["type"] == "mamba2":
                 y = mamba2(h, ly["mixer"], mix, eps, st)
             else:
                 y = grouped_attention(h, ly["mixer"], mix, eps, st, self.pos, first_v)
-            if ly["mlp"] is not None:
+            if ly["mlp"] is not None and ly["mlp"].get("kind") == "experts":
+                lim = ly["mlp"]["limit"]
+                y = y + sparse.experts(h, ly["mlp"], lambda n: w[f"l{i}.mlp." + n], lambda g, u: np.minimum(g, lim) * sigmoid(
+                    1.702 * np.minimum(g, lim)) * (np.clip(u, -lim, lim) + 1))
+            elif ly["mlp"] is not None:
                 y = y + clamped_feed_forward(h, lambda n: w[f"l{i}.mlp." + n], ly["mlp"]["limit"])
             x = x + cfg["residual_mult"] * y
             self.taps.append(x)

@@ -51,7 +51,7 @@ def route64(l, top, score, bias, groups, top_groups, renorm, scale):
     for t in range(T):
         x = np.where(np.isnan(l[t]), -np.inf, l[t])
         gone = x == -np.inf
-        with np.errstate(invalid="ignore"):
+        with np.errstate(invalid="ignore", over="ignore"):
             if score == "softmax":
                 s = np.zeros(n) if gone.all() else np.exp(x - x.max())
                 s = s / s.sum() if s.sum() > 0 else s
@@ -373,7 +373,7 @@ def test_delta_rows_between_other_rows(chunks, f32):
     lengths, H, G, d, dv = [5, 0, 70], 4, 2, 24, 40
 
     def call(op, q, k, v, ld, la, beta, o, seqs):
-        args = (q, k, v, ld, la.data_ptr(), beta.data_ptr(), H, o.data_ptr(), H * dv + 2)
+        args = (q, k, v, ld, la.data_ptr(), H, beta.data_ptr(), H, o.data_ptr(), H * dv + 2)
         if not chunks:
             _lib.call("lt_dn_delta_rows", *args, f32, op._ref, ctypes.byref(seqs), stream())
             return

@@ -76,7 +76,7 @@ def test_experts_refusals():
 
 def test_delta_refusals():
     rows = lambda text, d=delta(), q=seqs((0, 5, 256)), ld=96, ldh=4, ldo=96: _refused(
-        "lt_dn_delta_rows", text, one, one, one, ld, one, one, ldh, one, ldo, 0, d, q, None)
+        "lt_dn_delta_rows", text, one, one, one, ld, one, ldh, one, ldh, one, ldo, 0, d, q, None)
     rows("multiple of the key heads", delta(H=3))
     rows("multiples of 8", delta(dp=12))
     rows("above 512", delta(dp=520))
@@ -89,12 +89,12 @@ def test_delta_refusals():
     rows("rows of a sequence", q=seqs((2 ** 31 - 2, 5, 256)))
     rows("one state", q=seqs((0, 5, 256), (5, 5, 256)))
     rows("share rows", q=seqs((0, 5, 256), (4, 5, 512)))
-    rows("ldh=3", ldh=3)
+    rows("ldla=3", ldh=3)
     rows("ldo=95", ldo=95)
     rows("alignment", ld=100)
     rows("alignment", ldo=97)
     chunked = lambda text, d=delta(), q=seqs((0, 5, 256)), k=one, ld=96, ldo=96, ws=one: _refused(
-        "lt_dn_delta_chunked", text, one, k, one, ld, one, one, 4, one, ldo, d, q, ws, None)
+        "lt_dn_delta_chunked", text, one, k, one, ld, one, 4, one, 4, one, ldo, d, q, ws, None)
     chunked("above 256", delta(dp=264))
     chunked("above 256", delta(dvp=520))
     chunked("alignment", k=ctypes.c_void_p(258))
@@ -112,7 +112,7 @@ def test_delta_refusals():
 
 def test_no_rows_is_no_launch():
     n = _lib.launch_count()
-    assert _lib.dense().lt_dn_delta_rows(one, one, one, 96, one, one, 4, one, 96, 0, delta(), seqs((0, 0, 256), (7, 0, 512)), None) == 0
+    assert _lib.dense().lt_dn_delta_rows(one, one, one, 96, one, 4, one, 4, one, 96, 0, delta(), seqs((0, 0, 256), (7, 0, 512)), None) == 0
     assert _lib.launch_count() == n
 
 
@@ -133,3 +133,55 @@ def test_objects_refuse():
         P.Experts(torch.zeros(2, 5, 8), gated=True)
     with pytest.raises(ValueError, match="key heads"):
         P.DeltaRule(3, 2, 8, 8, torch.float32, 1.0, 1e-6)
+
+
+def test_models_with_bad_sizes_are_refused(monkeypatch):
+    """Packing refuses what does not fit together (no device is reached)."""
+    from llamatov_b200 import mixers
+    from tests import layered_util as U
+    from tests import sparse_util as X
+
+    class Pk:
+        dtype, Ep, f32 = torch.float32, 80, 1
+
+        def want(self, **kw):
+            pass
+    cfg = X.config(U)
+    t = X.random_tensors(U, cfg)
+    c = {"n_embd": cfg["width"], "norm_eps": 1e-5, "dtype": "float32"}
+    get = lambda p, **change: (lambda n: change[n] if n in change else t[p + n])
+    m = cfg["layers"][0]["mixer"]
+    with pytest.raises(ValueError, match="key heads"):
+        mixers.GatedDeltaMixer(Pk(), c, dict(m, key_heads=3), get("l0.mix."))
+    with pytest.raises(ValueError, match="convolution"):
+        mixers.GatedDeltaMixer(Pk(), c, dict(m, conv=3), get("l0.mix."))
+    ff = cfg["layers"][0]["mlp"]
+    with pytest.raises(ValueError, match="router"):
+        mixers.gelu_experts(Pk(), c, dict(ff, experts=7), get("l0.mlp."))
+    with pytest.raises(ValueError, match="down"):
+        mixers.gelu_experts(Pk(), c, ff, get("l0.mlp.", down=t["l0.mlp.down"][:, :-1]))
+    with pytest.raises(ValueError, match="top 9"):
+        mixers.gelu_experts(Pk(), c, dict(ff, top=9), get("l0.mlp."))
+    with pytest.raises(ValueError, match="groups"):
+        mixers.clamped_experts(Pk(), c, dict(ff, groups=3, limit=1.0), get("l0.mlp."))
+
+
+def test_oracle_of_the_delta_rule_is_the_chunked_equation():
+    """The token-by-token restatement against the matrix form of a chunk, so that the tests' yardstick stands on two legs."""
+    import numpy as np
+    from oracle import sparse as O
+    r = np.random.default_rng(0)
+    T, H, G, d, dv = 23, 4, 2, 6, 5
+    q, k, v = r.standard_normal((T, G, d)), r.standard_normal((T, G, d)), r.standard_normal((T, H, dv))
+    la, beta, S0 = -r.random((T, H)), r.random((T, H)), r.standard_normal((H, dv, d))
+    S = S0.copy()
+    o = O.delta_rule(q, k, v, la, beta, S, 0.3, 1e-6)
+    for h in range(H):
+        kh = k[:, h // 2] / np.sqrt((k[:, h // 2] ** 2).sum(1, keepdims=True) + 1e-6)
+        qh = 0.3 * q[:, h // 2] / np.sqrt((q[:, h // 2] ** 2).sum(1, keepdims=True) + 1e-6)
+        c = np.cumsum(la[:, h])
+        D = np.tril(np.exp(c[:, None] - c[None]))
+        A = np.tril(beta[:, h, None] * D * (kh @ kh.T), -1)
+        Uv = np.linalg.solve(np.eye(T) + A, beta[:, h, None] * (v[:, h] - np.exp(c)[:, None] * (kh @ S0[h].T)))
+        assert np.allclose(o[:, h], np.exp(c)[:, None] * (qh @ S0[h].T) + (np.tril(qh @ kh.T) * D) @ Uv)
+        assert np.allclose(S[h], np.exp(c[-1]) * S0[h] + (Uv * np.exp(c[-1] - c)[:, None]).T @ kh)
