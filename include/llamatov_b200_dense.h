@@ -283,13 +283,14 @@ long lt_dn_experts_plan_ints(int T, int top, int n);
 int lt_dn_experts_plan(const int* ids, int T, int top, int n, int* plan, void* stream);
 
 /* H[t*top + j] = glu(gate, up) of x_t and the expert's matrix: W [n][2F][ldw], F gate rows, then F up rows.  h_epi: LT_DN_GLU.
- * Rows of H whose place is left out stay as they are. */
+ * Rows of H whose place is left out stay as they are.  With a plan ws holds lt_dn_experts_glu_ws(T, top, K, f32) fp32 elements. */
+long lt_dn_experts_glu_ws(int T, int top, int K, int f32);
 int lt_dn_experts_glu(const void* W, int ldw, const void* X, int ldx, void* H, int ldh, int f32, int F, int K, const lt_dn_choice* h_c,
-                      const lt_dn_epilogue* h_epi, void* stream);
+                      const lt_dn_epilogue* h_epi, void* ws, void* stream);
 
 /* Y[t] (fp32) += ls * sum_j w[t*top + j] * (W of the expert) H[t*top + j]; W [n][M][ldw]; ls [M] or NULL (1).  With a plan ws holds
- * lt_dn_experts_sum_ws(T, top, M) fp32 elements. */
-long lt_dn_experts_sum_ws(int T, int top, int M);
+ * lt_dn_experts_sum_ws(T, top, M, K, f32) fp32 elements. */
+long lt_dn_experts_sum_ws(int T, int top, int M, int K, int f32);
 int lt_dn_experts_sum(const void* W, int ldw, const void* H, int ldh, float* Y, int ldy, int f32, int M, int K, const lt_dn_choice* h_c,
                       const float* w, const float* ls, float* ws, void* stream);
 

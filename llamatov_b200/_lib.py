@@ -177,7 +177,7 @@ DENSE_SIGNATURES = {
     "lt_dn_delta_step": [_vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, ctypes.POINTER(DnDelta), _vp],
     "lt_dn_route": [_vp, _i, _vp, _vp, _i, ctypes.POINTER(DnRouter), _vp],
     "lt_dn_experts_plan": [_vp, _i, _i, _i, _vp, _vp],
-    "lt_dn_experts_glu": [_vp, _i, _vp, _i, _vp, _i, _i, _i, _i, ctypes.POINTER(DnChoice), ctypes.POINTER(DnEpilogue), _vp],
+    "lt_dn_experts_glu": [_vp, _i, _vp, _i, _vp, _i, _i, _i, _i, ctypes.POINTER(DnChoice), ctypes.POINTER(DnEpilogue), _vp, _vp],
     "lt_dn_experts_sum": [_vp, _i, _vp, _i, _vp, _i, _i, _i, _i, ctypes.POINTER(DnChoice), _vp, _vp, _vp, _vp],
     "lt_dn_gqa_step": [_vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _vp, ctypes.POINTER(DnGqa), _i, _vp, _vp, _vp],
 }
@@ -186,7 +186,8 @@ _DENSE_QUERIES = {"lt_dn_gqa_step_ws": ([_i, _i, _i], ctypes.c_long),
                   "lt_dn_latent_step_ws": ([_i, _i, _i, _i], ctypes.c_long),
                   "lt_dn_delta_chunked_ws": ([ctypes.POINTER(DnDelta), ctypes.POINTER(DnSeqs)], ctypes.c_long),
                   "lt_dn_experts_plan_ints": ([_i, _i, _i], ctypes.c_long),
-                  "lt_dn_experts_sum_ws": ([_i, _i, _i], ctypes.c_long),
+                  "lt_dn_experts_glu_ws": ([_i, _i, _i, _i], ctypes.c_long),
+                  "lt_dn_experts_sum_ws": ([_i, _i, _i, _i, _i], ctypes.c_long),
                   "lt_dn_recurrence_chunked_ws": ([_i, _i, _i, _i], ctypes.c_long)}
 # what the common library exports (the Q8_0 library passes these through to its users as well)
 _COMMON_NAMES = ("lt_last_error", "lt_version", "lt_launch_count", "lt_set_chained_launch", "lt_device_status",

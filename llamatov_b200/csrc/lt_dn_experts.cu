@@ -139,7 +139,7 @@ using namespace lt;
 using namespace lt::dn;
 
 extern "C" int lt_dn_experts_glu(const void* W, int ldw, const void* X, int ldx, void* H, int ldh, int f32, int F, int K,
-                                 const lt_dn_choice* h_c, const lt_dn_epilogue* h_epi, void* stream) {
+                                 const lt_dn_choice* h_c, const lt_dn_epilogue* h_epi, void* ws, void* stream) {
     LT_REQUIRE(W && X && H, "lt_dn_experts_glu: null pointer");
     const char* bad = choice_error(h_c);
     if (bad == nullptr) bad = epi_error(h_epi);
@@ -149,9 +149,10 @@ extern "C" int lt_dn_experts_glu(const void* W, int ldw, const void* X, int ldx,
                "lt_dn_experts_glu: F=%d K=%d ldw=%d ldx=%d ldh=%d (multiples of 8)", F, K, ldw, ldx, ldh);
     LT_REQUIRE(aligned16(W) && aligned16(X), "lt_dn_experts_glu: W and X must be 16-byte aligned");
     if (h_c->plan != nullptr) {
+        LT_REQUIRE(f32 || (ws != nullptr && aligned16(ws)), "lt_dn_experts_glu: a plan needs the workspace, 16-byte aligned");
         GroupP G = {W, X, H, device_status_ptr(), F, K, ldw, ldx, ldh, h_c->top, 0, *h_c, *h_epi};
         LT_REQUIRE(G.status != nullptr, "lt_dn_experts_glu: status word unavailable");
-        return launch_group(G, true, f32, (cudaStream_t)stream);
+        return launch_group(G, true, f32, ws, (cudaStream_t)stream);
     }
     FewP P = {W, X, H, nullptr, nullptr, device_status_ptr(), ldw, ldx, ldh, F, K, *h_c, *h_epi};
     LT_REQUIRE(P.status != nullptr, "lt_dn_experts_glu: status word unavailable");
@@ -162,7 +163,12 @@ extern "C" int lt_dn_experts_glu(const void* W, int ldw, const void* X, int ldx,
     return check_launch("lt_dn_experts_glu");
 }
 
-extern "C" long lt_dn_experts_sum_ws(int T, int top, int M) { return (long)T * top * M; }
+// the sums of the places, on a boundary of 16 bytes, then (bf16) their rows in the order of the plan
+static long places_floats(int T, int top, int M) { return ((long)T * top * M + 3) / 4 * 4; }
+extern "C" long lt_dn_experts_glu_ws(int T, int top, int K, int f32) { return f32 ? 0 : (long)T * top * K / 2; }
+extern "C" long lt_dn_experts_sum_ws(int T, int top, int M, int K, int f32) {
+    return places_floats(T, top, M) + (f32 ? 0 : (long)T * top * K / 2);
+}
 
 extern "C" int lt_dn_experts_sum(const void* W, int ldw, const void* H, int ldh, float* Y, int ldy, int f32, int M, int K,
                                  const lt_dn_choice* h_c, const float* w, const float* ls, float* ws, void* stream) {
@@ -173,10 +179,10 @@ extern "C" int lt_dn_experts_sum(const void* W, int ldw, const void* H, int ldh,
                "lt_dn_experts_sum: M=%d K=%d ldw=%d ldh=%d ldy=%d (multiples of 8)", M, K, ldw, ldh, ldy);
     LT_REQUIRE(aligned16(W) && aligned16(H), "lt_dn_experts_sum: W and H must be 16-byte aligned");
     if (h_c->plan != nullptr) {
-        LT_REQUIRE(ws != nullptr, "lt_dn_experts_sum: a plan needs the workspace");
+        LT_REQUIRE(ws != nullptr && aligned16(ws), "lt_dn_experts_sum: a plan needs the workspace, 16-byte aligned");
         GroupP G = {W, H, ws, device_status_ptr(), M, K, ldw, ldh, M, 1, 0, *h_c, {}};
         LT_REQUIRE(G.status != nullptr, "lt_dn_experts_sum: status word unavailable");
-        const int rc = launch_group(G, false, f32, (cudaStream_t)stream);
+        const int rc = launch_group(G, false, f32, ws + places_floats(h_c->T, h_c->top, M), (cudaStream_t)stream);
         return rc != LT_OK ? rc : launch_combine(ws, w, ls, Y, ldy, M, *h_c, (cudaStream_t)stream);
     }
     LT_REQUIRE(h_c->T <= 65535, "lt_dn_experts_sum: %d tokens without an order of the places (at most 65535)", h_c->T);

@@ -16,8 +16,8 @@ struct GroupP {
     lt_dn_choice c;
     lt_dn_epilogue epi;
 };
-// Y[p] = products of place p, with the plan of P.c: gated outputs in the element type, or fp32 sums
-int launch_group(GroupP P, bool glu, bool f32, cudaStream_t s);
+// Y[p] = products of place p, with the plan of P.c: gated outputs in the element type, or fp32 sums.  rows: bf16, K elements a place
+int launch_group(GroupP P, bool glu, bool f32, void* rows, cudaStream_t s);
 
 // Y[t] += ls * sum_j w[t][j] ws[t * top + j]
 int launch_combine(const float* ws, const float* w, const float* ls, float* Y, int ldy, int M, const lt_dn_choice& c, cudaStream_t s);

@@ -4,11 +4,14 @@
 // bf16 (k_group_tc): tcgen05.mma kind::f16, fp32 accumulators in tensor memory.  A tile is 128 gate rows with their 128 up rows (or
 // 256 output rows) of one expert, two MMAs of M = 128, by N places of it.  An expert's places are shared out evenly over as few tiles
 // as hold them, and N is the share rounded up to 16: rows of no place cost at most 15 columns of a tile, whatever the shares are.
-//   warp 8 : weights, by tiled TMA
-//   warps 10-13 : the rows of X, by asynchronous copies of 16 bytes into the swizzled layout.  (Gathering TMA, four rows an
-//                 instruction, took 83 clocks each and 425 us where these copies take 121.)
-//   warp 9 : one thread issues the MMAs
-//   warps 0-7 : epilogue, a thread per weight row
+// The rows of X are first put in the order of the plan (k_gather), so that tiled TMA fetches them.  (Fetched from where they are by
+// gathering TMA, four rows an instruction: 83 clocks each, 425 us for gate|up 2 x 1024 x 2048 of 8 of 64 experts, 2000 tokens; by
+// asynchronous copies of 16 bytes: 203; in order 167, 12 of it for putting them there.)
+//   warp 16 : producer, TMA
+//   warp 17 : one thread issues the MMAs
+//   warps 0-15 : epilogue, a thread per weight row and a quarter of the places
+// What bounds it is the traffic between L2 and the SMs (64 KB for 1024 clocks of MMAs at N = 256) and the epilogue, which runs alone
+// where 2 N columns fill the tensor memory.
 // fp32 (k_group_f32): register-blocked tiles on the CUDA cores.
 #include "lt_dn_experts.cuh"
 #include "lt_tc.cuh"
@@ -19,6 +22,7 @@ namespace dn {
 using namespace tc;
 
 constexpr int GK = 64;           // k elements of a stage (128 bytes)
+constexpr int XBOX = 64;         // places of a TMA box
 constexpr int MAX_EXPERTS = 1024;
 
 template <int NT>
@@ -27,7 +31,7 @@ struct GroupCfg {
     static constexpr int NSTAGE = (206 * 1024) / STAGE > 8 ? 8 : (206 * 1024) / STAGE;
     static constexpr int BUFS = NT <= 128 ? 2 : 1;          // sets of accumulators
     static constexpr int TMEM = BUFS * 2 * NT;
-    static constexpr int EW = 8, XW = 4, THREADS = (EW + 2 + XW) * 32;
+    static constexpr int EW = 16, THREADS = (EW + 2) * 32;
     static constexpr int SMEM = 1024 + NSTAGE * STAGE + 512 + (MAX_EXPERTS + 1) * 4;
     static_assert(TMEM <= 512 && (TMEM & (TMEM - 1)) == 0, "tensor memory columns");
     static_assert(SMEM <= 227 * 1024, "shared memory");
@@ -37,7 +41,7 @@ struct GroupBars {
     unsigned long long full[8], empty[8], tfull[2], tempty[2];
     unsigned tmem_base;
     int abort_flag;
-    int warp_tiles[14];
+    int warp_tiles[18];
 };
 
 // D[tmem] (+)= A[smem] * B[smem], bf16 x bf16 -> fp32
@@ -49,9 +53,11 @@ __device__ __forceinline__ void group_mma(unsigned d, unsigned long long a, unsi
         "l"(a), "l"(b), "r"(idesc), "r"((int)acc)
         : "memory");
 }
-// arrives when this thread's copies so far have landed
-__device__ __forceinline__ void cp_async_arrive(unsigned bar) {
-    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+// gelu(z) u = z u / (1 + 2^(-z (a + b z^2))) with the constants of the tanh form times log2 e
+__device__ __forceinline__ float gelu_up(float z, float u) {
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * fmaf(z * z, -0.10294324f, -2.3022082f)));
+    return __fdividef(z * u, 1.0f + e);
 }
 
 // Tiles of places by expert: cum[e] tiles lie before expert e's.  Every role walks them with a cursor of its own.
@@ -72,7 +78,7 @@ struct Cursor {
 
 template <int NT, bool GLU>
 __global__ void __launch_bounds__(GroupCfg<NT>::THREADS, 1)
-k_group_tc(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ GroupP P) {
+k_group_tc(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const __grid_constant__ GroupP P) {
     using C = GroupCfg<NT>;
     constexpr int NS = C::NSTAGE;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -87,7 +93,7 @@ k_group_tc(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ Grou
 
     if (tid == 0) {
         for (int s = 0; s < NS; s++) {
-            mbar_init(&B->full[s], 1 + C::XW * 32);
+            mbar_init(&B->full[s], 1);
             mbar_init(&B->empty[s], 1);
         }
         for (int s = 0; s < 2; s++) {
@@ -151,42 +157,14 @@ k_group_tc(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ Grou
                     break;
                 }
                 if (lane == 0) {
-                    bar_expect_tx(full, C::W_STAGE);
+                    bar_expect_tx(full, C::W_STAGE + ((cur.n + XBOX - 1) & ~(XBOX - 1)) * 128);
                     tma_load_2d(st, &tmW, kb * GK, row, full);
                     tma_load_2d(st + 128 * 128, &tmW, kb * GK, row2, full);
+                    for (int x = 0; x < cur.n; x += XBOX) tma_load_2d(st + C::W_STAGE + x * 128, &tmX, kb * GK, cur.from + x, full);
                 }
                 __syncwarp();
             }
         }
-    } else if (warp >= C::EW + 2) {
-        // eight threads a row, 16 rows at a time; the row's 16-byte units stand where the 128-byte swizzle puts them
-        const int xt = tid - (C::EW + 2) * 32, r0 = xt >> 3, unit = xt & 7;
-        const unsigned dst0 = smem_u32(base) + C::W_STAGE + r0 * 128 + ((unit ^ (r0 & 7)) << 4);
-        unsigned it = 0;
-        bool go = true;
-        for (int tile = blockIdx.x; go && tile < tiles; tile += gridDim.x) {
-            cur.seek(P, cum, tile);
-            const bf16* src[NT / 16];
-#pragma unroll
-            for (int i = 0; i < NT / 16; i++)
-                src[i] = (const bf16*)P.X + (long)(places[cur.from + min(r0 + 16 * i, cur.count - 1)] / P.per) * P.ldx + unit * 8;
-            for (int kb = 0; kb < nk; kb++, it++) {
-                const int s = it % NS;
-                if (!acquire(smem_u32(&B->empty[s]), ((it / NS) & 1) ^ 1, abort_flag, P.status)) {
-                    go = false;
-                    break;
-                }
-                const int k = kb * GK, bytes = k + unit * 8 < P.K ? 16 : 0;
-                const unsigned dst = dst0 + s * C::STAGE;
-#pragma unroll
-                for (int i = 0; i < NT / 16; i++)
-                    if (16 * i < cur.n)
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + i * 2048), "l"(bytes ? src[i] + k : (const bf16*)P.X), "r"(bytes)
-                                     : "memory");
-                cp_async_arrive(smem_u32(&B->full[s]));
-            }
-        }
-        asm volatile("cp.async.wait_all;" ::: "memory");
     } else if (warp == C::EW + 1) {
         if (lane == 0) {
             const unsigned long long w0 = smem_desc<4>(smem_u32(base));
@@ -203,7 +181,6 @@ k_group_tc(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ Grou
                 for (int kb = 0; kb < nk; kb++, it++) {
                     const unsigned s = it % NS;
                     mbar_wait<0>(&B->full[s], (it / NS) & 1, abort_flag, P.status);
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // X was copied through the generic proxy
                     tc_fence_after();
                     const unsigned long long wd = w0 + (unsigned long long)(s * (C::STAGE >> 4));
                     const unsigned long long xd = x0 + (unsigned long long)(s * (C::STAGE >> 4));
@@ -225,15 +202,21 @@ k_group_tc(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ Grou
             cur.seek(P, cum, tile);
             const int row = cur.rt * (GLU ? 128 : 256) + q * 32 + lane;
             const unsigned slot = n % C::BUFS;
-            int mine[NT / 32];                // places of this warp's columns, fetched under the products
+            int mine[NT / 64];                // places of this warp's columns, fetched under the products
 #pragma unroll
-            for (int i = 0; i < NT / 32; i++) mine[i] = places[cur.from + min(32 * i + cg * 16 + (lane & 15), cur.count - 1)];
+            for (int i = 0; i < NT / 64; i++) mine[i] = places[cur.from + min(64 * i + cg * 16 + (lane & 15), cur.count - 1)];
             mbar_wait<32>(&B->tfull[slot], (n / C::BUFS) & 1, abort_flag, P.status);
             tc_fence_after();
             const unsigned ta = tmem + ((unsigned)(q * 32) << 16) + slot * 2 * NT;
+            auto release = [&]() {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&B->tempty[slot]);
+            };
+            unsigned out[GLU ? NT / 64 : 1][8];      // gated outputs, so that the accumulators are free before the stores
 #pragma unroll
-            for (int i = 0; i < NT / 32; i++) {
-                const int c0 = 32 * i + cg * 16, left = cur.count - c0;
+            for (int i = 0; i < NT / 64; i++) {
+                const int c0 = 64 * i + cg * 16, left = cur.count - c0;
                 if (left <= 0) break;
                 int v[2][16];
 #pragma unroll
@@ -245,12 +228,16 @@ k_group_tc(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ Grou
                     for (int c = 0; c < 16; c += 4) reg_fence4(&v[a][c]);
                 if (GLU) {
                     float f[16];
-                    glu_bf16(P.epi, v[0], v[1], f);
-                    bf16* y = (bf16*)P.Y + row;
+                    if (P.epi.glu_act == LT_DN_GLU_GELU) {
 #pragma unroll
-                    for (int c = 0; c < 16; c++) {
-                        const int p = __shfl_sync(0xffffffffu, mine[i], c);
-                        if (row < P.M && c < left) y[(long)p * P.ldy] = from_f<bf16>(f[c]);
+                        for (int c = 0; c < 16; c++) f[c] = gelu_up(__int_as_float(v[0][c]), __int_as_float(v[1][c]));
+                    } else {
+                        glu_bf16(P.epi, v[0], v[1], f);
+                    }
+#pragma unroll
+                    for (int c = 0; c < 8; c++) {
+                        const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * c], f[2 * c + 1]);
+                        out[GLU ? i : 0][c] = *(const unsigned*)&h;
                     }
                 } else {
                     float* y = (float*)P.Y + row;
@@ -264,9 +251,20 @@ k_group_tc(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ Grou
                     }
                 }
             }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&B->tempty[slot]);
+            release();
+            if (GLU) {
+#pragma unroll
+                for (int i = 0; i < NT / 64; i++) {
+                    const int left = cur.count - 64 * i - cg * 16;
+                    if (left <= 0) break;
+                    unsigned short* y = (unsigned short*)P.Y + row;
+#pragma unroll
+                    for (int c = 0; c < 16; c++) {
+                        const int p = __shfl_sync(0xffffffffu, mine[i], c);
+                        if (row < P.M && c < left) y[(long)p * P.ldy] = (unsigned short)(out[GLU ? i : 0][c >> 1] >> (16 * (c & 1)));
+                    }
+                }
+            }
             n++;
         }
     }
@@ -285,12 +283,12 @@ k_group_tc(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ Grou
     }
 }
 
-static int group_map(CUtensorMap* m, const void* ptr, long rows, int K, int ld) {
+static int group_map(CUtensorMap* m, const void* ptr, long rows, int K, int ld, int box_rows) {
     encode_fn_t fn = encode_fn();
     LT_REQUIRE(fn != nullptr, "experts' products: cuTensorMapEncodeTiled is not available from this driver");
     cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
     cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
-    cuuint32_t box[2] = {(cuuint32_t)GK, 128};
+    cuuint32_t box[2] = {(cuuint32_t)GK, (cuuint32_t)box_rows};
     cuuint32_t estr[2] = {1, 1};
     CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -301,24 +299,48 @@ static int group_map(CUtensorMap* m, const void* ptr, long rows, int K, int ld) 
     return LT_OK;
 }
 
+// rows of X in the order of the plan: a warp per place, 16 bytes a lane
+__global__ void __launch_bounds__(256) k_gather(const __grid_constant__ GroupP P, uint4* out) {
+    const int s = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, units = P.K / 8;
+    if (s >= P.c.plan[P.c.n]) return;
+    const int place = P.c.plan[P.c.n + 1 + s];
+    const uint4* in = (const uint4*)((const bf16*)P.X + (long)(place / P.per) * P.ldx);
+    uint4* o = out + (long)s * units;
+    for (int x = lane; x < units; x += 128) {
+        uint4 v[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+            if (x + 32 * u < units) v[u] = in[x + 32 * u];
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+            if (x + 32 * u < units) o[x + 32 * u] = v[u];
+    }
+}
+
 template <int NT, bool GLU>
-static int launch_group_tc(GroupP P, cudaStream_t s) {
+static int launch_group_tc(GroupP P, void* rows, cudaStream_t s) {
     using C = GroupCfg<NT>;
-    CUtensorMap tmW;
-    const int rc = group_map(&tmW, P.W, (long)P.c.n * P.M * (GLU ? 2 : 1), P.K, P.ldw);
+    const long places = (long)P.c.T * P.c.top;
+    CUtensorMap tmW, tmX;
+    int rc = group_map(&tmW, P.W, (long)P.c.n * P.M * (GLU ? 2 : 1), P.K, P.ldw, 128);
+    if (rc != LT_OK) return rc;
+    rc = group_map(&tmX, rows, places, P.K, P.K, XBOX);
     if (rc != LT_OK) return rc;
     static PerDeviceOnce once;
     if (once.first()) LT_CUDA(cudaFuncSetAttribute(k_group_tc<NT, GLU>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    k_gather<<<(unsigned)((places + 7) / 8), 256, 0, s>>>(P, (uint4*)rows);
+    rc = check_launch("experts' products (rows in order)");
+    if (rc != LT_OK) return rc;
     P.row_tiles = (P.M + (GLU ? 127 : 255)) / (GLU ? 128 : 256);
-    k_group_tc<NT, GLU><<<sm_count(), C::THREADS, C::SMEM, s>>>(tmW, P);
+    k_group_tc<NT, GLU><<<sm_count(), C::THREADS, C::SMEM, s>>>(tmW, tmX, P);
     return check_launch("experts' products");
 }
 template <bool GLU>
-static int pick_group_tc(const GroupP& P, cudaStream_t s) {
+static int pick_group_tc(const GroupP& P, void* rows, cudaStream_t s) {
     const long each = (long)P.c.T * P.c.top / P.c.n;        // places of an expert
-    if (each <= 24) return launch_group_tc<64, GLU>(P, s);
-    if (each <= 64) return launch_group_tc<128, GLU>(P, s);
-    return launch_group_tc<256, GLU>(P, s);
+    if (each <= 24) return launch_group_tc<64, GLU>(P, rows, s);
+    if (each <= 64) return launch_group_tc<128, GLU>(P, rows, s);
+    return launch_group_tc<256, GLU>(P, rows, s);
 }
 
 // ---------------------------------------------------------------------------- fp32
@@ -469,9 +491,9 @@ static int pick_group_f32(const GroupP& P, cudaStream_t s) {
     return launch_group_f32<GLU, 4>(P, s);
 }
 
-int launch_group(GroupP P, bool glu, bool f32, cudaStream_t s) {
+int launch_group(GroupP P, bool glu, bool f32, void* rows, cudaStream_t s) {
     if (f32) return glu ? pick_group_f32<true>(P, s) : pick_group_f32<false>(P, s);
-    return glu ? pick_group_tc<true>(P, s) : pick_group_tc<false>(P, s);
+    return glu ? pick_group_tc<true>(P, rows, s) : pick_group_tc<false>(P, rows, s);
 }
 
 // ---------------------------------------------------------------------------- sum over a token's places

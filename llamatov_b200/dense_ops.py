@@ -202,16 +202,19 @@ class Experts:
 
     def hidden(self, x, ldx, places, h, ldh):
         """h[t*top + j] = glu of the gate and up rows of place (t, j)'s expert, for the rows of x."""
+        ws = self._workspace(places, "lt_dn_experts_glu_ws", self.K)
         _lib.call("lt_dn_experts_glu", self.ptr, self.K, x, ldx, h, ldh, self.f32, self.M, self.K, places.ref, ctypes.byref(self.epi),
-                  _stream())
+                  None if ws is None else ws.data_ptr(), _stream())
 
     def add_sum(self, h, ldh, places, w, y, ldy, ls=None):
         """y[t] += ls * sum over j of w[t][j] W h[t*top + j]."""
-        ws = None
-        if places.buf is not None:
-            buf = torch.empty(_lib.dense().lt_dn_experts_sum_ws(places.T, places.top, self.M), dtype=torch.float32, device="cuda")
-            ws = buf.data_ptr()
-        _lib.call("lt_dn_experts_sum", self.ptr, self.K, h, ldh, y, ldy, self.f32, self.M, self.K, places.ref, w, ls, ws, _stream())
+        ws = self._workspace(places, "lt_dn_experts_sum_ws", self.M, self.K)
+        _lib.call("lt_dn_experts_sum", self.ptr, self.K, h, ldh, y, ldy, self.f32, self.M, self.K, places.ref, w, ls,
+                  None if ws is None else ws.data_ptr(), _stream())
+
+    def _workspace(self, places, query, *sizes):
+        n = 0 if places.buf is None else getattr(_lib.dense(), query)(places.T, places.top, *sizes, self.f32)
+        return torch.empty(n, dtype=torch.float32, device="cuda") if n else None
 
 
 # --------------------------------------------------------------------------- delta rule

@@ -51,13 +51,15 @@ def test_route_refusals(kw, ld, T, text):
 
 def test_experts_refusals():
     e = P.epilogue(_lib.DN_GLU, glu=(0, 0.0, 0.0))
-    glu = lambda text, ldw=16, ldx=16, ldh=24, F=24, K=16, c=choice(), epi=e, W=one: _refused(
-        "lt_dn_experts_glu", text, W, ldw, one, ldx, one, ldh, 0, F, K, c, ctypes.byref(epi), None)
+    glu = lambda text, ldw=16, ldx=16, ldh=24, F=24, K=16, c=choice(), epi=e, W=one, ws=None: _refused(
+        "lt_dn_experts_glu", text, W, ldw, one, ldx, one, ldh, 0, F, K, c, ctypes.byref(epi), ws, None)
     glu("null", W=None)
     glu("multiples of 8", K=12)
     glu("multiples of 8", ldw=8)
     glu("ldh=23", ldh=23)
     glu("aligned", W=ctypes.c_void_p(264))
+    glu("workspace", c=choice(plan=256))
+    glu("workspace", c=choice(plan=256), ws=ctypes.c_void_p(264))
     glu("null choice", c=choice(ids=None))
     glu("experts", c=choice(n=1025))
     glu("top", c=choice(top=33))
@@ -69,9 +71,12 @@ def test_experts_refusals():
     s("ldy=23", ldy=23)
     s("multiples of 8", ldh=12)
     s("without an order", c=choice(T=65536))
+    s("workspace", c=choice(plan=256))
     _refused("lt_dn_experts_plan", "n=1025", one, 3, 2, 1025, one, None)
     _refused("lt_dn_experts_plan", "null", None, 3, 2, 8, one, None)
-    assert _lib.dense().lt_dn_experts_plan_ints(5, 3, 8) == 24 and _lib.dense().lt_dn_experts_sum_ws(5, 3, 8) == 120
+    L = _lib.dense()
+    assert L.lt_dn_experts_plan_ints(5, 3, 8) == 24 and L.lt_dn_experts_glu_ws(5, 3, 16, 0) == 120 and L.lt_dn_experts_glu_ws(5, 3, 16, 1) == 0
+    assert L.lt_dn_experts_sum_ws(5, 3, 9, 16, 1) == 136 and L.lt_dn_experts_sum_ws(5, 3, 9, 16, 0) == 256
 
 
 def test_delta_refusals():
