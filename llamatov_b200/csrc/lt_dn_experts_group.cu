@@ -345,6 +345,34 @@ static int pick_group_tc(const GroupP& P, void* rows, cudaStream_t s) {
 
 // ---------------------------------------------------------------------------- fp32
 
+// By one warp: the expert whose tiles of BN places hold number g, 32 experts at a time.  found: expert, places (none past the last
+// tile); place: the tile's places, the last repeated.
+template <int BN>
+__device__ __forceinline__ void find_tile(const lt_dn_choice& c, int g, int lane, int* found, int* place) {
+    int before = 0, from = 0, count = 0;
+    for (int e0 = 0; e0 < c.n && before <= g; e0 += 32) {
+        const int e = e0 + lane, at = e < c.n ? c.plan[e] : 0, all = e < c.n ? c.plan[e + 1] - at : 0;
+        const int tiles = (all + BN - 1) / BN;
+        int up = tiles;
+#pragma unroll
+        for (int s = 1; s < 32; s <<= 1) {
+            const int o = __shfl_up_sync(0xffffffffu, up, s);
+            if (lane >= s) up += o;
+        }
+        const int first = before + up - tiles;
+        const unsigned here = __ballot_sync(0xffffffffu, g >= first && g < first + tiles);
+        if (here != 0) {
+            const int l = __ffs(here) - 1, skip = (g - __shfl_sync(0xffffffffu, first, l)) * BN;
+            from = __shfl_sync(0xffffffffu, at, l) + skip;
+            count = min(BN, __shfl_sync(0xffffffffu, all, l) - skip);
+            if (lane == 0) found[0] = e0 + l;
+        }
+        before += __shfl_sync(0xffffffffu, up, 31);
+    }
+    if (lane == 0) found[1] = count;
+    if (count > 0 && lane < BN) place[lane] = c.plan[c.n + 1 + from + min(lane, count - 1)];
+}
+
 // 64 weight rows (with GLU: and their 64 up rows) x 8 MQ places of one expert per CTA of 128 threads; a thread owns 4 rows x MQ
 // places, 16-byte reads of shared memory, three stages of 32 k filled by asynchronous copies.  k is added up 256 at a time, so that
 // chains of roundings stay short.  Instructions bound it, and places that a tile has no use for cost as many as the others.
@@ -355,37 +383,12 @@ __global__ void __launch_bounds__(GF_THREADS) k_group_f32(const __grid_constant_
     constexpr int GF_BN = 8 * MQ, NG = GLU ? 2 : 1, ROWS = NG * GF_BM + GF_BN;
     extern __shared__ __align__(16) float gf_smem[];
     __shared__ int place[GF_BN];
-    __shared__ int found[3];                 // expert, first place in the list, places
-    const int tid = threadIdx.x, lane = tid & 31, n = tid & 15, m = tid >> 4;
-    const int n0 = blockIdx.x * GF_BM, g = blockIdx.y;
-    if (tid < 32) {                          // the expert whose tiles hold number g: 32 experts at a time
-        int before = 0;
-        bool done = false;
-        for (int e0 = 0; e0 < P.c.n && !done; e0 += 32) {
-            const int e = e0 + lane, at = e < P.c.n ? P.c.plan[e] : 0, c = e < P.c.n ? P.c.plan[e + 1] - at : 0;
-            const int tiles = (c + GF_BN - 1) / GF_BN;
-            int up = tiles;
-#pragma unroll
-            for (int s = 1; s < 32; s <<= 1) {
-                const int o = __shfl_up_sync(0xffffffffu, up, s);
-                if (lane >= s) up += o;
-            }
-            const int first = before + up - tiles;
-            if (g >= first && g < first + tiles) {
-                found[0] = e;
-                found[1] = at + (g - first) * GF_BN;
-                found[2] = min(GF_BN, c - (g - first) * GF_BN);
-            }
-            before += __shfl_sync(0xffffffffu, up, 31);
-            done = before > g;
-        }
-        if (!done && lane == 0) found[2] = 0;
-        __syncwarp();
-        const int count = found[2];
-        if (count > 0 && lane < GF_BN) place[lane] = P.c.plan[P.c.n + 1 + found[1] + min(lane, count - 1)];
-    }
+    __shared__ int found[2];
+    const int tid = threadIdx.x, n = tid & 15, m = tid >> 4;
+    const int n0 = blockIdx.x * GF_BM;
+    if (tid < 32) find_tile<GF_BN>(P.c, blockIdx.y, tid, found, place);
     __syncthreads();
-    const int count = found[2];
+    const int count = found[1];
     if (count == 0) return;
     const float* W = (const float*)P.W + (long)found[0] * NG * P.M * P.ldw;
     const int nk = (P.K + GF_BK - 1) / GF_BK;
@@ -472,22 +475,140 @@ __global__ void __launch_bounds__(GF_THREADS) k_group_f32(const __grid_constant_
     }
 }
 
+// Few places an expert: up to 16 of them per CTA of four warps.  A warp owns four weight rows (two gate rows and their up rows),
+// streams them through registers once, 16 bytes a lane and a chunk of 256 k ahead, and multiplies them with the places' rows from
+// shared memory; the 64 sums go over the lanes at the end.  Bound by the matrices' bytes until reads of shared memory, one for 16
+// multiply-adds, take as long.  (16 experts of 616 x 896 gated, 148 places: 34 us; register-blocked tiles of 64 rows x 16 places 50,
+// x 32 places 63.)
+constexpr int FM_PLACES = 16, FM_K = 256;
+
+template <bool GLU>
+__global__ void __launch_bounds__(128, 3) k_group_f32_few(const __grid_constant__ GroupP P) {
+    __shared__ __align__(16) float4 sx[2][FM_PLACES][FM_K / 4];
+    __shared__ int place[FM_PLACES], found[2];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nq = P.K / 4, nk = (P.K + FM_K - 1) / FM_K;
+    if (tid < 32) find_tile<FM_PLACES>(P.c, blockIdx.y, tid, found, place);
+    __syncthreads();
+    const int count = found[1];
+    if (count == 0) return;
+    const int r0 = (blockIdx.x * 4 + warp) * (GLU ? 2 : 4);      // first pair or row
+    const float4* w[4];
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        const int row = GLU ? min(r0 + (r & 1), P.M - 1) + (r >> 1) * P.M : min(r0 + r, P.M - 1);
+        w[r] = (const float4*)((const float*)P.W + ((long)found[0] * (GLU ? 2 : 1) * P.M + row) * P.ldw);
+    }
+    auto copy = [&](int c) {
+        if (c < nk) {
+#pragma unroll
+            for (int e = tid; e < FM_PLACES * (FM_K / 4); e += 128) {
+                const int p = e / (FM_K / 4), x = e % (FM_K / 4), q = c * (FM_K / 4) + x;
+                const bool ok = p < count && q < nq;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(&sx[c & 1][p][x])),
+                             "l"(ok ? (const float4*)((const float*)P.X + (long)(place[p] / P.per) * P.ldx) + q : (const float4*)P.W), "r"(ok ? 16 : 0)
+                             : "memory");
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    int4 next[4][2];
+    auto fetch = [&](int c) {
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int q = c * (FM_K / 4) + lane + 32 * u;
+                next[r][u] = q < nq ? ld_stream_v4(w[r] + q) : make_int4(0, 0, 0, 0);
+            }
+    };
+    float acc[4 * FM_PLACES];
+#pragma unroll
+    for (int i = 0; i < 4 * FM_PLACES; i++) acc[i] = 0.0f;
+    copy(0);
+    fetch(0);
+    for (int c = 0; c < nk; c++) {
+        float4 v[4][2];
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+                v[r][u] = make_float4(__int_as_float(next[r][u].x), __int_as_float(next[r][u].y), __int_as_float(next[r][u].z), __int_as_float(next[r][u].w));
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();             // chunk c is there, and nobody reads the one before
+        copy(c + 1);
+        if (c + 1 < nk) fetch(c + 1);
+#pragma unroll
+        for (int g = 0; g < FM_PLACES; g += 4) {
+            if (g >= count) break;
+#pragma unroll
+            for (int p = g; p < g + 4; p++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const float4 x = sx[c & 1][p][lane + 32 * u];
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        acc[r * FM_PLACES + p] = fmaf(v[r][u].w, x.w, fmaf(v[r][u].z, x.z, fmaf(v[r][u].y, x.y, fmaf(v[r][u].x, x.x, acc[r * FM_PLACES + p]))));
+                }
+        }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    // at every step a lane hands on one half of its sums and keeps the other: it ends with numbers 2 lane and 2 lane + 1
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1)
+#pragma unroll
+        for (int i = 0; i < 2 * s; i++) {
+            const bool up = (lane & s) != 0;
+            const float give = up ? acc[i] : acc[i + 2 * s], have = up ? acc[i + 2 * s] : acc[i];
+            acc[i] = have + __shfl_xor_sync(0xffffffffu, give, s);
+        }
+    const int r = lane >> 3, p = (lane & 7) * 2;
+    float u[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) u[i] = __shfl_down_sync(0xffffffffu, acc[i], 16);      // the up rows' sums to the gate rows' lanes
+    const int row = r0 + r;
+    if (row >= P.M || (GLU && r >= 2)) return;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        if (p + i >= count) break;
+        const long y = (long)place[p + i] * P.ldy + row;
+        if (GLU) glu_store<float>(P.epi, P.Y, y, acc[i], u[i]);
+        else ((float*)P.Y)[y] = acc[i];
+    }
+}
+
+static int f32_tiles(const GroupP& P, int BN, long* tiles) {         // at most: one begun by every expert
+    const long places = (long)P.c.T * P.c.top;
+    *tiles = places < P.c.n ? places : P.c.n + (places - P.c.n) / BN;
+    LT_REQUIRE(*tiles <= 65535, "experts' products: %ld places in fp32", places);
+    return LT_OK;
+}
 template <bool GLU, int MQ>
 static int launch_group_f32(const GroupP& P, cudaStream_t s) {
     constexpr int BN = 8 * MQ, SMEM = GF_STAGES * ((GLU ? 2 : 1) * GF_BM + BN) * GF_ST * 4;
     static PerDeviceOnce once;
     if (once.first()) LT_CUDA(cudaFuncSetAttribute(k_group_f32<GLU, MQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
-    const long places = (long)P.c.T * P.c.top;
-    const long tiles = places < P.c.n ? places : P.c.n + (places - P.c.n) / BN;        // at most: one begun by every expert
-    LT_REQUIRE(tiles <= 65535, "experts' products: %ld places in fp32", places);
+    long tiles;
+    const int rc = f32_tiles(P, BN, &tiles);
+    if (rc != LT_OK) return rc;
     k_group_f32<GLU, MQ><<<dim3((P.M + GF_BM - 1) / GF_BM, (unsigned)tiles), GF_THREADS, SMEM, s>>>(P);
     return check_launch("experts' products");
 }
 template <bool GLU>
+static int launch_group_f32_few(const GroupP& P, cudaStream_t s) {
+    long tiles;
+    const int rc = f32_tiles(P, FM_PLACES, &tiles);
+    if (rc != LT_OK) return rc;
+    const int rows = GLU ? 8 : 16;
+    k_group_f32_few<GLU><<<dim3((P.M + rows - 1) / rows, (unsigned)tiles), 128, 0, s>>>(P);
+    return check_launch("experts' products");
+}
+// By places of an expert.  Gated, 64 experts of 512 x 2048, us in registers / tiles of 32 places: 8 180 / 294, 16 275 / 321, 24 375 / 322.
+// Sums, 2048 x 512, in registers / tiles of 16 / of 32: 4 91 / 92 / 125, 8 122 / 114 / 137, 16 180 / 147 / 156, 24 242 / 187 / 180.
+template <bool GLU>
 static int pick_group_f32(const GroupP& P, cudaStream_t s) {
-    const long each = (long)P.c.T * P.c.top / P.c.n;        // places of an expert
-    if (each <= 6) return launch_group_f32<GLU, 1>(P, s);
-    if (each <= 14) return launch_group_f32<GLU, 2>(P, s);
+    const long each = (long)P.c.T * P.c.top / P.c.n;
+    if (each <= (GLU ? 18 : 5)) return launch_group_f32_few<GLU>(P, s);
+    if (!GLU && each <= 20) return launch_group_f32<false, 2>(P, s);
     return launch_group_f32<GLU, 4>(P, s);
 }
 
