@@ -6,16 +6,24 @@
 //   S <- e^(b_end) S + U^T diag(r e^(b_end - b)) K
 //   O = rq q_scale (diag(e^b) Q S^T + tril(Q K^T .* r_j e^(b_i - b_j)) U)
 //
-//   k_delta_prep    every chunk and head at once: T by forward substitution in blocks, in fp32
+// With W = T diag(e^b r) K and U0 = T V, which need no state, U = U0 - W S^T.
+//
+//   k_delta_prep    every chunk and head at once: T by forward substitution in blocks, in fp32; W, U0
 //   k_delta_states  walks the chunks: a CTA owns 16 value columns of one head of one sequence, its warps the key channels; the state
 //                   stays in their accumulators, transposed (rows are value columns), so that it is the A operand of the next
 //                   product as it stands; stores the state a chunk starts from, and U
 //   k_delta_out     every chunk and head at once
 //
-// What is bf16 in memory (q, k) enters exactly.  Everything else is fp32: it enters as the sum of three bf16 (24 significant
+// What is bf16 in memory (q, k, v) enters exactly.  Everything else is fp32: it enters as the sum of three bf16 (24 significant
 // bits), three products against bf16 and six against another such sum, so that chunks are as exact as token order.  The
 // products of the leading parts have accumulators of their own: the tensor cores cut sums off instead of rounding them, which costs
 // up to 2^-24 of the accumulator at every step.
+//
+// The walk over the chunks is the longest of the three, and bound by the instructions and waits of a chunk's dependent chain.  So W, U0
+// and the keys lie in memory as the lanes hold them (16 bytes a lane, side by side) and go straight into registers, asked for when
+// the chunk before has used them; a chunk passes two barriers.  (16 heads of 128, 2048 rows: 32, 70 and 37 us; four
+// sequences of them 437 together.  With T in place of W, one product and barrier more, and operands through shared memory: 17, 76 and 38;
+// 484.)
 #include "lt_dn_delta.cuh"
 #include "lt_dn_mma.cuh"
 
@@ -25,14 +33,18 @@ namespace dn {
 constexpr int DC = 64;                          // tokens of a chunk
 constexpr float DLOG2E = 1.4426950408889634f;
 constexpr int TS = DC + 8;                      // row stride of 64-column bf16 tiles: an odd number of 16-byte units
-constexpr int DVEC = 2 * DC + 4;                // e^b r, r e^(b_end - b), e^(b_end)
+constexpr int DVEC = DC + 4;                    // r e^(b_end - b), e^(b_end)
 
 struct DeltaChunkP {
     const bf16 *q, *k, *v;
     const float *la, *beta;
     float* o;
-    bf16* T3;                // [chunk][H][3][64][64]
-    float *vec, *S0, *U;     // [chunk][H]: [DVEC], [dvp][dp], [dvp][64]
+    // [chunk][H], in lanes' order: W [dp/16][64/16][3] of uint4 x 32; starting states [dvp/16][dp/16][3] of uint4 x 32; U0, then U
+    // [dvp/16][64/8] of float4 x 32; vec [DVEC].  [chunk][G]: keys [dp/16][64/16] of uint4 x 32
+    uint4 *W, *S0, *Kf;
+    float4* U;
+    float* vec;
+    int nkt, nvt;            // tiles of 16 key channels, of 16 value columns
     int ld, ldla, ldb, ldo;
     int first[LT_DN_SEQS + 1];    // chunks before a sequence's
     lt_dn_delta D;
@@ -113,18 +125,30 @@ __device__ __forceinline__ void row_norms(const bf16* s, int stride, int units, 
 constexpr int MS = DC + 4;       // row stride of fp32 tiles
 constexpr int PREP_THREADS = 256;
 
+// four numbers of a row as three rows of bf16
+__device__ __forceinline__ void store_parts(bf16* p, float4 x) {
+    uint2 p0, p1, p2;
+    split3(x.x, x.y, p0.x, p1.x, p2.x);
+    split3(x.z, x.w, p0.y, p1.y, p2.y);
+    *(uint2*)p = p0;
+    *(uint2*)(p + DC * TS) = p1;
+    *(uint2*)(p + 2 * DC * TS) = p2;
+}
+
 // I + A is inverted in place: diagonal blocks of 16 by forward substitution, a column per lane, then the blocks below them,
 // X21 = -X22 (A21 X11), first of 16, then of 32.
-__global__ void __launch_bounds__(PREP_THREADS) k_delta_prep(const __grid_constant__ DeltaChunkP P) {
+__global__ void __launch_bounds__(PREP_THREADS, 4) k_delta_prep(const __grid_constant__ DeltaChunkP P) {
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ __align__(16) double sb[DC];
-    __shared__ __align__(16) float sr[DC], sbeta[DC];
-    const int dpr = (P.D.dp + 31) & ~31, KS = dpr + 8;
+    __shared__ __align__(16) float sr[DC], sbeta[DC], sgrow[DC];
+    const int dpr = (P.D.dp + 31) & ~31, KS = dpr + 8, dvr = P.nvt * 16, VS = dvr + 8, per = P.D.H / P.D.G;
     float* sA = (float*)smem;                 // [64][MS]
-    bf16* sk = (bf16*)(sA + DC * MS);
-    float* sT = (float*)sk;                   // [32][36], once the keys are used
+    float* sT = sA + DC * MS;                 // [32][36]
+    bf16* sP = (bf16*)smem;                   // [3][64][TS]: parts of T, once its numbers are in registers
+    bf16* sk = sP + 3 * DC * TS;              // keys, then values, then keys again
+    bf16* sv = sk;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tg = lane & 3;
-    const int h = blockIdx.y, hq = h / (P.D.H / P.D.G);
+    const int h = blockIdx.y, hq = h / per;
     const Chunk c = chunk_of(P, blockIdx.x);
     const long at = (long)blockIdx.x * P.D.H + h;
     load_rows(sk, KS, dpr / 8, P.k, c, P.ld, hq * P.D.dp, P.D.dp);
@@ -134,6 +158,14 @@ __global__ void __launch_bounds__(PREP_THREADS) k_delta_prep(const __grid_consta
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
     row_norms(sk, KS, dpr / 8, P.D.eps, 1.0f, sr);
+    if (h == hq * per) {                      // the keys as the update of the state takes them
+        uint4* out = P.Kf + ((long)blockIdx.x * P.D.G + hq) * P.nkt * 4 * 32 + lane;
+        for (int e = warp; e < P.nkt * 4; e += PREP_THREADS / 32) {
+            unsigned r[4];
+            ldsm4t(r, sk + ((e & 3) * 16 + (lane & 15)) * KS + (e >> 2) * 16 + (lane >> 4) * 8);
+            out[e * 32] = make_uint4(r[0], r[1], r[2], r[3]);
+        }
+    }
     const int m = warp & 3;      // k_i . k_j: rows 16 m + g (+ 8), columns 16 n + 2 tg (+ 1, + 8, + 9) of every other n up to m
     float a[2][2][4];
 #pragma unroll
@@ -154,6 +186,8 @@ __global__ void __launch_bounds__(PREP_THREADS) k_delta_prep(const __grid_consta
         }
     }
     __syncthreads();
+    load_rows(sv, VS, dvr / 8, P.v, c, P.ld, h * P.D.dvp, P.D.dvp);
+    asm volatile("cp.async.commit_group;" ::: "memory");
 #pragma unroll
     for (int n = 0; n < 2; n++) {
         const int col = 2 * n + (warp >> 2);
@@ -166,9 +200,9 @@ __global__ void __launch_bounds__(PREP_THREADS) k_delta_prep(const __grid_consta
     }
     if (tid < DC) {
         float* vec = P.vec + at * DVEC;
-        vec[tid] = exp2f((float)sb[tid]) * sr[tid];
-        vec[DC + tid] = exp2f((float)(sb[DC - 1] - sb[tid])) * sr[tid];
-        if (tid == 0) vec[2 * DC] = exp2f((float)sb[DC - 1]);
+        sgrow[tid] = exp2f((float)sb[tid]) * sr[tid];
+        vec[tid] = exp2f((float)(sb[DC - 1] - sb[tid])) * sr[tid];
+        if (tid == 0) vec[DC] = exp2f((float)sb[DC - 1]);
     }
     __syncthreads();
     if (warp < 4 && lane < 16) {
@@ -231,131 +265,192 @@ __global__ void __launch_bounds__(PREP_THREADS) k_delta_prep(const __grid_consta
         *(float4*)(sA + i * MS + 32 + j) = make_float4(0, 0, 0, 0);
     }
     __syncthreads();
-    bf16* out = P.T3 + at * 3 * DC * DC;
+    {   // parts of T = (I + A)^-1 diag(beta), over its numbers
+        float4 T[4];
 #pragma unroll
-    for (int e = tid; e < DC * DC / 4; e += PREP_THREADS) {
-        const int i = e >> 4, j = (e & 15) * 4;
-        const float4 x = *(const float4*)(sA + i * MS + j), be = *(const float4*)(sbeta + j);
-        uint2 t0, t1, t2;
-        split3(x.x * be.x, x.y * be.y, t0.x, t1.x, t2.x);
-        split3(x.z * be.z, x.w * be.w, t0.y, t1.y, t2.y);
-        *(uint2*)(out + i * DC + j) = t0;
-        *(uint2*)(out + DC * DC + i * DC + j) = t1;
-        *(uint2*)(out + 2 * DC * DC + i * DC + j) = t2;
+        for (int u = 0; u < 4; u++) {
+            const int e = tid + u * PREP_THREADS, j = (e & 15) * 4;
+            const float4 x = *(const float4*)(sA + (e >> 4) * MS + j), be = *(const float4*)(sbeta + j);
+            T[u] = make_float4(x.x * be.x, x.y * be.y, x.z * be.z, x.w * be.w);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int e = tid + u * PREP_THREADS;
+            store_parts(sP + (e >> 4) * TS + (e & 15) * 4, T[u]);
+        }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+    for (int vt = warp; vt < P.nvt; vt += PREP_THREADS / 32) {       // U0, transposed
+        float4* out = P.U + (at * P.nvt + vt) * 8 * 32 + lane;
+        unsigned x[4][4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) ldsm4t(x[j], sv + (j * 16 + (lane >> 4) * 8 + (lane & 7)) * VS + vt * 16 + ((lane >> 3) & 1) * 8);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            float d[3][4];
+#pragma unroll
+            for (int p = 0; p < 3; p++) {
+                d[p][0] = d[p][1] = d[p][2] = d[p][3] = 0.0f;
+#pragma unroll
+                for (int k2 = 0; k2 < 2; k2++) {
+                    if (4 * k2 > i) break;
+                    unsigned r[4];
+                    ldsm4(r, sP + (p * DC + i * 8 + (lane & 7)) * TS + k2 * 32 + (lane >> 3) * 8);
+                    mma16816(d[p], x[2 * k2], r[0], r[1]);
+                    if (4 * k2 + 2 <= i) mma16816(d[p], x[2 * k2 + 1], r[2], r[3]);
+                }
+            }
+            out[i * 32] = make_float4(d[0][0] + (d[1][0] + d[2][0]), d[0][1] + (d[1][1] + d[2][1]), d[0][2] + (d[1][2] + d[2][2]),
+                                      d[0][3] + (d[1][3] + d[2][3]));
+        }
+    }
+    __syncthreads();
+    load_rows(sk, KS, dpr / 8, P.k, c, P.ld, hq * P.D.dp, P.D.dp);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+#pragma unroll
+    for (int u = 0; u < 4; u++) {             // of T diag(e^b r): the parts add up to T again
+        const int e = tid + u * PREP_THREADS, j = (e & 15) * 4;
+        bf16* p = sP + (e >> 4) * TS + j;
+        float x[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 2; i >= 0; i--) {
+            const uint2 w = *(const uint2*)(p + i * DC * TS);
+            x[0] += lo_f(w.x); x[1] += hi_f(w.x); x[2] += lo_f(w.y); x[3] += hi_f(w.y);
+        }
+        const float4 f = *(const float4*)(sgrow + j);
+        store_parts(p, make_float4(x[0] * f.x, x[1] * f.y, x[2] * f.z, x[3] * f.w));
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+    // W: tokens 16 m .., every other tile of channels, two tiles at a time
+    for (int kt = warp >> 2; kt < P.nkt; kt += 4) {
+        float d[2][2][4];
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) d[u][0][e] = d[u][1][e] = 0.0f;
+#pragma unroll
+        for (int p = 2; p >= 0; p--)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if (j > m) break;
+                unsigned x[4];
+                ldsm4(x, sP + (p * DC + m * 16 + (lane & 15)) * TS + j * 16 + (lane >> 4) * 8);
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    if (kt + 2 * u >= P.nkt) break;
+                    unsigned r[4];
+                    ldsm4t(r, sk + (j * 16 + (lane & 15)) * KS + (kt + 2 * u) * 16 + (lane >> 4) * 8);
+                    mma16816(d[u][0], x, r[0], r[1]);
+                    mma16816(d[u][1], x, r[2], r[3]);
+                }
+            }
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            if (kt + 2 * u >= P.nkt) break;
+            uint4 q0, q1, q2;
+            split3(d[u][0][0], d[u][0][1], q0.x, q1.x, q2.x);
+            split3(d[u][1][0], d[u][1][1], q0.y, q1.y, q2.y);
+            split3(d[u][0][2], d[u][0][3], q0.z, q1.z, q2.z);
+            split3(d[u][1][2], d[u][1][3], q0.w, q1.w, q2.w);
+            uint4* o = P.W + ((at * P.nkt + kt + 2 * u) * 4 + m) * 3 * 32 + lane;
+            o[0] = q0;
+            o[32] = q1;
+            o[64] = q2;
+        }
     }
 }
-static size_t prep_smem(int dp) {
-    const size_t keys = (size_t)DC * (((dp + 31) & ~31) + 8) * 2, T = 32 * 36 * 4;
-    return (size_t)DC * MS * 4 + (keys > T ? keys : T);
+static size_t prep_smem(int dp, int nvt) {
+    const int dpr = (dp + 31) & ~31, dvr = nvt * 16;
+    return (size_t)3 * DC * TS * 2 + (size_t)DC * ((dpr > dvr ? dpr : dvr) + 8) * 2;
 }
+static_assert(DC * MS * 4 + 32 * 36 * 4 <= 3 * DC * TS * 2, "A and its products lie where the parts of T do later");
 
 // ---------------------------------------------------------------------------- states
 
-// NW warps, each with 16 KT key channels
-template <int NW, int KT, int STAGES_>
-struct DeltaStates {
-    static constexpr int STAGES = STAGES_, DPR = NW * 16 * KT, KS = DPR + 8, VS = 24, YS = DC + 8;
-    static constexpr int K_B = DC * KS * 2, T_B = 3 * DC * TS * 2, V_B = DC * VS * 2, VEC_B = DVEC * 4;
-    static constexpr int STAGE = K_B + T_B + V_B + VEC_B;
-    static constexpr int Y_B = NW * 16 * YS * 4, X_B = 3 * 16 * TS * 2;
-    static constexpr int SMEM = STAGES * STAGE + Y_B + 2 * X_B;
-    static_assert(STAGE % 16 == 0 && SMEM <= 227 * 1024, "shared memory");
-};
-
-template <int NW, int KT, int ST>
-__global__ void __launch_bounds__(NW * 32) k_delta_states(const __grid_constant__ DeltaChunkP P) {
-    using L = DeltaStates<NW, KT, ST>;
-    constexpr int KS = L::KS, THREADS = NW * 32;
-    extern __shared__ __align__(16) unsigned char smem[];
-    float* sY = (float*)(smem + L::STAGES * L::STAGE);       // [warp][16][YS]
-    bf16* sXp = (bf16*)((unsigned char*)sY + L::Y_B);        // [3][16][TS]
-    bf16* sZp = (bf16*)((unsigned char*)sXp + L::X_B);
+// NW warps, each with KT tiles of 16 key channels
+template <int NW, int KT>
+__global__ void __launch_bounds__(NW * 32, NW == 8 && KT == 1 ? 2 : 1) k_delta_states(const __grid_constant__ DeltaChunkP P) {
+    constexpr int YS = DC + 8, NT = 8 / NW;              // blocks of 8 tokens that a warp makes U of
+    // Keys are asked for a chunk ahead, or half a chunk where the registers of two CTAs an SM leave no room: with one CTA 16 heads of
+    // 128 take as long, 32 heads or four sequences of 16 a fifth longer.
+    constexpr bool AHEAD = NW != 8 || KT != 1;
+    __shared__ __align__(16) float sY[NW * 16 * YS];     // shares of (W S^T)^T
+    __shared__ __align__(16) bf16 sZ[3 * 16 * TS];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tg = lane & 3;
-    const int v0 = blockIdx.x * 16, h = blockIdx.y, b = blockIdx.z, hq = h / (P.D.H / P.D.G);
+    const int vt = blockIdx.x, h = blockIdx.y, b = blockIdx.z, hq = h / (P.D.H / P.D.G);
     const int nchunk = P.first[b + 1] - P.first[b], dp = P.D.dp, dvp = P.D.dvp;
     if (nchunk == 0) return;
-    const int active = (dp + 16 * KT - 1) / (16 * KT);       // warps with key channels
-    const int cw = warp * 16 * KT;
-    const int va = v0 + g, vb = va + 8;
-
-    // this thread's 16-byte units of a stage: one column of the keys, one of T, one of the values; pointers go on by chunks
-    constexpr int KU = L::DPR / 8, KR = THREADS / KU;        // units of a row of keys, rows of them at a time
-    const int kt_ = tid / KU, kx = (tid % KU) * 8, tt = tid >> 3, tx = (tid & 7) * 8, vt = tid >> 1, vx = (tid & 1) * 8;
-    const bool k_ok = kx < dp, v_ok = tid < 2 * DC && v0 + vx < dvp;
-    const bf16* kp = P.k + ((long)P.Q.start[b] + kt_) * P.ld + (long)hq * dp + kx;
-    const bf16* vp = P.v + ((long)P.Q.start[b] + vt) * P.ld + (long)h * dvp + v0 + vx;
+    const int active = (P.nkt + KT - 1) / KT;            // warps with key channels
+    const int kt0 = warp * KT, va = vt * 16 + g, vb = va + 8;
     const long at0 = (long)P.first[b] * P.D.H + h;
-    const bf16* tp = P.T3 + at0 * 3 * DC * DC + tid * 8;
-    const float* cp = P.vec + at0 * DVEC + tid * 4;
-    int left = P.Q.rows[b], next = 0;         // rows not yet asked for, chunk that is asked for next
-    auto load = [&]() {
-        if (next < nchunk) {
-            unsigned char* st = smem + (next % L::STAGES) * L::STAGE;
-            bf16* sk = (bf16*)st + kt_ * KS + kx;
-            bf16* sT = (bf16*)(st + L::K_B) + tt * TS + tx;
-#pragma unroll
-            for (int i = 0; i < DC / KR; i++) {
-                const bool ok = k_ok && kt_ + i * KR < left;
-                cp16(sk + i * KR * KS, ok ? kp + (long)i * KR * P.ld : P.k, ok);
-            }
-#pragma unroll
-            for (int i = 0; i < 3 * DC * 8 / THREADS; i++) cp16(sT + i * (THREADS / 8) * TS, tp + i * THREADS * 8, true);
-            if (tid < 2 * DC) {
-                const bool ok = v_ok && vt < left;
-                cp16((bf16*)(st + L::K_B + L::T_B) + vt * L::VS + vx, ok ? vp : P.v, ok);
-            }
-            if (tid < DVEC / 4) cp16((float*)(st + L::K_B + L::T_B + L::V_B) + tid * 4, cp, true);
-            kp += (long)DC * P.ld;
-            vp += (long)DC * P.ld;
-            tp += (long)P.D.H * 3 * DC * DC;
-            cp += (long)P.D.H * DVEC;
-            left -= DC;
-            next++;
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    };
 
-    float s[2 * KT][4];              // S[va or vb][cw + 8 i + 2 tg + (0, 1)]
-    const long sa = (long)va * dp + cw + 2 * tg, sd = (long)vb * dp + cw + 2 * tg;
-    const bool a_ok = va < dvp, b_ok = vb < dvp;
+    float s[2 * KT][4];              // S[va or vb][16 kt0 + 8 i + 2 tg + (0, 1)]
+    const long sa = (long)va * dp + kt0 * 16 + 2 * tg, sd = sa + 8L * dp;
     float* S = P.Q.S[b] + (long)h * dvp * dp;
 #pragma unroll
     for (int i = 0; i < 2 * KT; i++) {
         float2 a = make_float2(0, 0), d = a;
-        if (cw + 8 * i < dp && a_ok) a = *(const float2*)(S + sa + 8 * i);
-        if (cw + 8 * i < dp && b_ok) d = *(const float2*)(S + sd + 8 * i);
+        if (kt0 * 16 + 8 * i < dp && va < dvp) a = *(const float2*)(S + sa + 8 * i);
+        if (kt0 * 16 + 8 * i < dp && vb < dvp) d = *(const float2*)(S + sd + 8 * i);
         s[i][0] = a.x; s[i][1] = a.y; s[i][2] = d.x; s[i][3] = d.y;
     }
-    auto keep = [&](float* to) {
+    // what a chunk needs beside the state, asked for as soon as the registers are free
+    const uint4* Wp = P.W + (at0 * P.nkt + kt0) * 12 * 32 + lane;
+    const uint4* Kp = P.Kf + (((long)P.first[b] * P.D.G + hq) * P.nkt + kt0) * 4 * 32 + lane;
+    float4* Up = P.U + ((at0 * P.nvt + vt) * 8 + warp) * 32 + lane;
+    const float* vp = P.vec + at0 * DVEC + warp * 8 + 2 * tg;
+    uint4* S0 = P.S0 + ((at0 * P.nvt + vt) * P.nkt + kt0) * 3 * 32 + lane;
+    uint4 w[KT][4][3], kf[KT][4];
+    float4 u0[NT];
+    float2 z[NT];
+    float end = 0.0f;
+    bool mine[KT];
 #pragma unroll
-        for (int i = 0; i < 2 * KT; i++) {
-            if (cw + 8 * i < dp && a_ok) *(float2*)(to + sa + 8 * i) = make_float2(s[i][0], s[i][1]);
-            if (cw + 8 * i < dp && b_ok) *(float2*)(to + sd + 8 * i) = make_float2(s[i][2], s[i][3]);
-        }
-    };
-    // operands that do not wait for the state are read ahead of the barrier that the state's own share waits at
-    auto keys = [&](unsigned (&r)[KT][4][4], const bf16* sk) {
+    for (int kt = 0; kt < KT; kt++) mine[kt] = kt0 + kt < P.nkt;
+    auto ask_w = [&]() {
 #pragma unroll
         for (int kt = 0; kt < KT; kt++)
 #pragma unroll
-            for (int n = 0; n < 4; n++)
-                ldsm4(r[kt][n], sk + (n * 16 + (lane & 7) + ((lane >> 4) << 3)) * KS + cw + kt * 16 + ((lane >> 3) & 1) * 8);
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int p = 0; p < 3; p++)
+                    if (mine[kt]) w[kt][t][p] = Wp[((kt * 4 + t) * 3 + p) * 32];
+        Wp += (long)P.D.H * P.nkt * 12 * 32;
+    };
+    auto ask_k = [&]() {
+#pragma unroll
+        for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+                if (mine[kt]) kf[kt][t] = Kp[(kt * 4 + t) * 32];
+        Kp += (long)P.D.G * P.nkt * 4 * 32;
+    };
+    auto ask_u = [&]() {
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            u0[n] = Up[n * NW * 32];
+            z[n] = *(const float2*)(vp + n * NW * 8);
+        }
+        end = vp[DC - warp * 8 - 2 * tg];
+        vp += (long)P.D.H * DVEC;
     };
 #pragma unroll
-    for (int i = 0; i < L::STAGES - 1; i++) load();
-    asm volatile("cp.async.wait_group %0;" ::"n"(L::STAGES - 2) : "memory");
-    __syncthreads();
-    unsigned kf[KT][4][4];
-    keys(kf, (const bf16*)smem);
-    float* S0 = P.S0 + at0 * dvp * dp;
-    float* U = P.U + at0 * dvp * DC;
+    for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            kf[kt][t] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int p = 0; p < 3; p++) w[kt][t][p] = make_uint4(0, 0, 0, 0);
+        }
+    ask_w();
+    ask_u();
+    if (AHEAD) ask_k();
     for (int chunk = 0; chunk < nchunk; chunk++) {
-        const unsigned char* st = smem + (chunk % L::STAGES) * L::STAGE;
-        const bf16* sk = (const bf16*)st;
-        const bf16* sT = (const bf16*)(st + L::K_B);
-        const bf16* sv = (const bf16*)(st + L::K_B + L::T_B);
-        const float* sc = (const float*)(st + L::K_B + L::T_B + L::V_B);
-        if (warp < active) {         // this warp's share of (K S^T)^T
+        const bool more = chunk + 1 < nchunk;
+        if (warp < active) {         // this warp's share of (W S^T)^T
             float y[8][4];
 #pragma unroll
             for (int n = 0; n < 8; n++) y[n][0] = y[n][1] = y[n][2] = y[n][3] = 0.0f;
@@ -366,97 +461,57 @@ __global__ void __launch_bounds__(NW * 32) k_delta_states(const __grid_constant_
                 split3(s[2 * kt][2], s[2 * kt][3], a[0][1], a[1][1], a[2][1]);
                 split3(s[2 * kt + 1][0], s[2 * kt + 1][1], a[0][2], a[1][2], a[2][2]);
                 split3(s[2 * kt + 1][2], s[2 * kt + 1][3], a[0][3], a[1][3], a[2][3]);
+                if (mine[kt]) {
 #pragma unroll
-                for (int p = 2; p >= 0; p--)
+                    for (int p = 0; p < 3; p++) S0[(kt * 3 + p) * 32] = make_uint4(a[p][0], a[p][1], a[p][2], a[p][3]);
+                }
 #pragma unroll
-                    for (int n = 0; n < 4; n++) {
-                        mma16816(y[2 * n], a[p], kf[kt][n][0], kf[kt][n][1]);
-                        mma16816(y[2 * n + 1], a[p], kf[kt][n][2], kf[kt][n][3]);
-                    }
+                for (int sum = 2; sum >= 0; sum--)       // parts i and j with i + j = sum, the smallest first
+#pragma unroll
+                    for (int p = 0; p <= sum; p++)
+#pragma unroll
+                        for (int t = 0; t < 4; t++) {
+                            mma16816(y[2 * t], a[p], w[kt][t][sum - p].x, w[kt][t][sum - p].y);
+                            mma16816(y[2 * t + 1], a[p], w[kt][t][sum - p].z, w[kt][t][sum - p].w);
+                        }
             }
-            float* o = sY + (warp * 16 + g) * L::YS + 2 * tg;
+            if (more) ask_w();
+            if (!AHEAD) ask_k();
+            float* o = sY + (warp * 16 + g) * YS + 2 * tg;
 #pragma unroll
             for (int n = 0; n < 8; n++) {
                 *(float2*)(o + 8 * n) = make_float2(y[n][0], y[n][1]);
-                *(float2*)(o + 8 * L::YS + 8 * n) = make_float2(y[n][2], y[n][3]);
+                *(float2*)(o + 8 * YS + 8 * n) = make_float2(y[n][2], y[n][3]);
             }
         }
-        keep(S0);
-        S0 += (long)P.D.H * dvp * dp;
-        __syncthreads();             // shares are there; nobody works on the chunk before
-        load();
+        S0 += (long)P.D.H * P.nvt * P.nkt * 3 * 32;
+        const float decay = end;
+        __syncthreads();             // shares are there; nobody reads Z of the chunk before
 #pragma unroll
-        for (int e = tid; e < 256; e += THREADS) {       // X = V - e^b r (K S^T), transposed
-            const int v = e >> 4, t = (e & 15) * 4;
-            float4 y = *(const float4*)(sY + v * L::YS + t);
+        for (int n = 0; n < NT; n++) {
+            const int t = (n * NW + warp) * 8 + 2 * tg;
+            float2 ya = *(const float2*)(sY + g * YS + t), yb = *(const float2*)(sY + (8 + g) * YS + t);
 #pragma unroll
-            for (int w = 1; w < NW; w++)
-                if (w < active) {
-                    const float4 z = *(const float4*)(sY + (w * 16 + v) * L::YS + t);
-                    y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
+            for (int k = 1; k < NW; k++)
+                if (k < active) {
+                    const float2 xa = *(const float2*)(sY + (k * 16 + g) * YS + t), xb = *(const float2*)(sY + (k * 16 + 8 + g) * YS + t);
+                    ya.x += xa.x; ya.y += xa.y; yb.x += xb.x; yb.y += xb.y;
                 }
-            const float4 f = *(const float4*)(sc + t);
-            uint2 a, d, l;
-            split3(fmaf(-f.x, y.x, to_f(sv[t * L::VS + v])), fmaf(-f.y, y.y, to_f(sv[(t + 1) * L::VS + v])), a.x, d.x, l.x);
-            split3(fmaf(-f.z, y.z, to_f(sv[(t + 2) * L::VS + v])), fmaf(-f.w, y.w, to_f(sv[(t + 3) * L::VS + v])), a.y, d.y, l.y);
-            *(uint2*)(sXp + v * TS + t) = a;
-            *(uint2*)(sXp + (16 + v) * TS + t) = d;
-            *(uint2*)(sXp + (32 + v) * TS + t) = l;
-        }
-        unsigned kb[4][KT][4];       // the keys again, as rows of tokens
-#pragma unroll
-        for (int kk = 0; kk < 4; kk++)
-#pragma unroll
-            for (int i = 0; i < KT; i++) ldsm4t(kb[kk][i], sk + (kk * 16 + (lane & 15)) * KS + cw + i * 16 + (lane >> 4) * 8);
-#pragma unroll
-        for (int u = 0; u < 8 / NW; u++) {       // U^T = X^T T^T: tokens 8 i ..; warps that share a scheduler have as much together
-            const int i = NW == 8 ? (warp < 4 ? warp : 11 - warp) : (u == 0 ? warp : 7 - warp);
-            unsigned tb[3][2][4];
-#pragma unroll
-            for (int p = 0; p < 3; p++)
-#pragma unroll
-                for (int k2 = 0; k2 < 2; k2++)
-                    if (4 * k2 <= i) ldsm4(tb[p][k2], sT + (p * DC + i * 8 + (lane & 7)) * TS + k2 * 32 + (lane >> 3) * 8);
-            if (u == 0) __syncthreads();         // X is there
-            float d[6][4];
-#pragma unroll
-            for (int p = 0; p < 6; p++) d[p][0] = d[p][1] = d[p][2] = d[p][3] = 0.0f;
-#pragma unroll
-            for (int kt = 0; kt < 4; kt++) {
-                if (2 * kt > i) break;
-                unsigned xa[3][4];
-#pragma unroll
-                for (int p = 0; p < 3; p++) ldsm4(xa[p], sXp + (p * 16 + (lane & 15)) * TS + kt * 16 + (lane >> 4) * 8);
-                const int lo = 2 * (kt & 1);
-                mma16816(d[0], xa[0], tb[0][kt >> 1][lo], tb[0][kt >> 1][lo + 1]);
-                mma16816(d[1], xa[0], tb[1][kt >> 1][lo], tb[1][kt >> 1][lo + 1]);
-                mma16816(d[2], xa[1], tb[0][kt >> 1][lo], tb[0][kt >> 1][lo + 1]);
-                mma16816(d[3], xa[0], tb[2][kt >> 1][lo], tb[2][kt >> 1][lo + 1]);
-                mma16816(d[4], xa[1], tb[1][kt >> 1][lo], tb[1][kt >> 1][lo + 1]);
-                mma16816(d[5], xa[2], tb[0][kt >> 1][lo], tb[0][kt >> 1][lo + 1]);
-            }
-            const int t = i * 8 + 2 * tg;
-            const float2 z = *(const float2*)(sc + DC + t);
-            float x[4];
-#pragma unroll
-            for (int e = 0; e < 4; e++) x[e] = d[0][e] + ((d[1][e] + d[2][e]) + (d[3][e] + (d[4][e] + d[5][e])));
+            const float4 u = make_float4(u0[n].x - ya.x, u0[n].y - ya.y, u0[n].z - yb.x, u0[n].w - yb.y);
+            Up[n * NW * 32] = u;
             unsigned a, m, l;
-            split3(x[0] * z.x, x[1] * z.y, a, m, l);
-            *(unsigned*)(sZp + g * TS + t) = a;
-            *(unsigned*)(sZp + (16 + g) * TS + t) = m;
-            *(unsigned*)(sZp + (32 + g) * TS + t) = l;
-            split3(x[2] * z.x, x[3] * z.y, a, m, l);
-            *(unsigned*)(sZp + (8 + g) * TS + t) = a;
-            *(unsigned*)(sZp + (24 + g) * TS + t) = m;
-            *(unsigned*)(sZp + (40 + g) * TS + t) = l;
-            if (a_ok) *(float2*)(U + (long)va * DC + t) = make_float2(x[0], x[1]);
-            if (b_ok) *(float2*)(U + (long)vb * DC + t) = make_float2(x[2], x[3]);
+            split3(u.x * z[n].x, u.y * z[n].y, a, m, l);
+            *(unsigned*)(sZ + g * TS + t) = a;
+            *(unsigned*)(sZ + (16 + g) * TS + t) = m;
+            *(unsigned*)(sZ + (32 + g) * TS + t) = l;
+            split3(u.z * z[n].x, u.w * z[n].y, a, m, l);
+            *(unsigned*)(sZ + (8 + g) * TS + t) = a;
+            *(unsigned*)(sZ + (24 + g) * TS + t) = m;
+            *(unsigned*)(sZ + (40 + g) * TS + t) = l;
         }
-        U += (long)P.D.H * dvp * DC;
-        const float end = sc[2 * DC];
-        asm volatile("cp.async.wait_group %0;" ::"n"(L::STAGES - 2) : "memory");
-        __syncthreads();             // Z is there, and the next chunk
-        if (chunk + 1 < nchunk) keys(kf, (const bf16*)(smem + ((chunk + 1) % L::STAGES) * L::STAGE));
+        Up += (long)P.D.H * P.nvt * 8 * 32;
+        if (more) ask_u();
+        __syncthreads();             // Z is there, and the shares are used
         if (warp < active) {
             float d[3][2 * KT][4];
 #pragma unroll
@@ -467,47 +522,48 @@ __global__ void __launch_bounds__(NW * 32) k_delta_states(const __grid_constant_
             for (int kk = 0; kk < DC / 16; kk++) {
                 unsigned za[3][4];
 #pragma unroll
-                for (int p = 0; p < 3; p++) ldsm4(za[p], sZp + (p * 16 + (lane & 15)) * TS + kk * 16 + (lane >> 4) * 8);
+                for (int p = 0; p < 3; p++) ldsm4(za[p], sZ + (p * 16 + (lane & 15)) * TS + kk * 16 + (lane >> 4) * 8);
 #pragma unroll
-                for (int i = 0; i < KT; i++)
+                for (int kt = 0; kt < KT; kt++)
 #pragma unroll
                     for (int p = 0; p < 3; p++) {
-                        mma16816(d[p][2 * i], za[p], kb[kk][i][0], kb[kk][i][1]);
-                        mma16816(d[p][2 * i + 1], za[p], kb[kk][i][2], kb[kk][i][3]);
+                        mma16816(d[p][2 * kt], za[p], kf[kt][kk].x, kf[kt][kk].y);
+                        mma16816(d[p][2 * kt + 1], za[p], kf[kt][kk].z, kf[kt][kk].w);
                     }
             }
+            if (AHEAD && more) ask_k();
 #pragma unroll
             for (int i = 0; i < 2 * KT; i++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) s[i][e] = fmaf(end, s[i][e], d[0][i][e] + (d[1][i][e] + d[2][i][e]));
+                for (int e = 0; e < 4; e++) s[i][e] = fmaf(decay, s[i][e], d[0][i][e] + (d[1][i][e] + d[2][i][e]));
         }
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    keep(S);
+#pragma unroll
+    for (int i = 0; i < 2 * KT; i++) {
+        if (kt0 * 16 + 8 * i < dp && va < dvp) *(float2*)(S + sa + 8 * i) = make_float2(s[i][0], s[i][1]);
+        if (kt0 * 16 + 8 * i < dp && vb < dvp) *(float2*)(S + sd + 8 * i) = make_float2(s[i][2], s[i][3]);
+    }
 }
 
-template <int NW, int KT, int ST>
+template <int NW, int KT>
 static int launch_states(const DeltaChunkP& P, cudaStream_t s) {
-    using L = DeltaStates<NW, KT, ST>;
-    static PerDeviceOnce once;
-    if (once.first()) LT_CUDA(cudaFuncSetAttribute(k_delta_states<NW, KT, ST>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM));
-    k_delta_states<NW, KT, ST><<<dim3((P.D.dvp + 15) / 16, P.D.H, P.Q.n), NW * 32, L::SMEM, s>>>(P);
+    k_delta_states<NW, KT><<<dim3(P.nvt, P.D.H, P.Q.n), NW * 32, 0, s>>>(P);
     return check_launch("lt_dn_delta_chunked (states)");
 }
 
 // ---------------------------------------------------------------------------- outputs
 
-// NK: blocks of 16 key channels at most; a warp owns 8 value columns at a time
+// NK: blocks of 16 key channels at most; a warp owns 16 value columns at a time
 template <int NK, int NW>
 struct DeltaOut {
     static constexpr int QS = NK * 16 + 8;
     static constexpr int SMEM = 2 * DC * QS * 2 + 3 * DC * TS * 2;
-    static constexpr int CTAS = NW == 4 ? 4 : NK <= 8 ? 2 : 1;      // of an SM
+    static constexpr int CTAS = NK > 8 ? 1 : NW == 4 ? 4 : 2;       // of an SM
 };
 
 template <int NK, int NW>
 __global__ void __launch_bounds__(NW * 32, DeltaOut<NK, NW>::CTAS) k_delta_out(const __grid_constant__ DeltaChunkP P) {
-    constexpr int QS = DeltaOut<NK, NW>::QS, KB = NK < 8 ? NK : 8;      // blocks of channels whose state is fetched together
+    constexpr int QS = DeltaOut<NK, NW>::QS;
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ __align__(16) double sb[DC];
     __shared__ float sr[DC], srq[DC];
@@ -515,33 +571,12 @@ __global__ void __launch_bounds__(NW * 32, DeltaOut<NK, NW>::CTAS) k_delta_out(c
     bf16* sk = sq + DC * QS;
     bf16* sP = sk + DC * QS;                     // [3][64][TS]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tg = lane & 3;
-    const int h = blockIdx.y, hq = h / (P.D.H / P.D.G), dp = P.D.dp, dvp = P.D.dvp, nk = (dp + 15) >> 4;
+    const int h = blockIdx.y, hq = h / (P.D.H / P.D.G), dp = P.D.dp, dvp = P.D.dvp, nk = P.nkt;
     const Chunk c = chunk_of(P, blockIdx.x);
     const long at = (long)blockIdx.x * P.D.H + h;
     load_rows(sq, QS, NK * 2, P.q, c, P.ld, hq * dp, dp);
     load_rows(sk, QS, NK * 2, P.k, c, P.ld, hq * dp, dp);
     asm volatile("cp.async.commit_group;" ::: "memory");
-    const float* S0 = P.S0 + at * dvp * dp + 2 * tg;
-    const float* U = P.U + at * dvp * DC + 2 * tg;
-    float2 fS[KB][2], fU[4][2];
-    auto fetch_state = [&](int v, int kb) {
-#pragma unroll
-        for (int k = 0; k < KB; k++) {
-            const int x = (kb + k) * 16;
-            const float* p = S0 + (long)(v + g) * dp + x;
-            fS[k][0] = v < dvp && x < dp ? __ldcs((const float2*)p) : make_float2(0, 0);
-            fS[k][1] = v < dvp && x + 8 < dp ? __ldcs((const float2*)(p + 8)) : make_float2(0, 0);
-        }
-    };
-    auto fetch_u = [&](int v) {
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const float* p = U + (long)(v + g) * DC + k * 16;
-            fU[k][0] = v < dvp ? __ldcs((const float2*)p) : make_float2(0, 0);
-            fU[k][1] = v < dvp ? __ldcs((const float2*)(p + 8)) : make_float2(0, 0);
-        }
-    };
-    fetch_state(warp * 8, 0);
     if (warp == 0) log_sums(P, c, h, lane, sb);
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
@@ -591,56 +626,72 @@ __global__ void __launch_bounds__(NW * 32, DeltaOut<NK, NW>::CTAS) k_delta_out(c
         }
     }
     __syncthreads();
-    for (int v0 = warp * 8; v0 < dvp; v0 += NW * 8) {
-        if (v0 != warp * 8) fetch_state(v0, 0);
-        float acc[4][4], low[4][4];
+    for (int vt = warp; vt < P.nvt; vt += NW) {
+        const uint4* S0 = P.S0 + (at * P.nvt + vt) * nk * 3 * 32 + lane;
+        const float4* U = P.U + (at * P.nvt + vt) * 8 * 32 + lane;
+        float acc[4][2][4], low[4][2][4];
 #pragma unroll
         for (int m = 0; m < 4; m++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) acc[m][e] = low[m][e] = 0.0f;
+            for (int n = 0; n < 2; n++)
 #pragma unroll
-        for (int kb = 0; kb < NK; kb += KB) {
-            if (kb >= nk) break;
-            if (kb > 0) fetch_state(v0, kb);
+                for (int e = 0; e < 4; e++) acc[m][n][e] = low[m][n][e] = 0.0f;
+        uint4 next[3];
 #pragma unroll
-            for (int k = 0; k < KB; k++) {
-                if (kb + k >= nk) break;
-                unsigned b0[3], b1[3];
-                split3(fS[k][0].x, fS[k][0].y, b0[0], b0[1], b0[2]);
-                split3(fS[k][1].x, fS[k][1].y, b1[0], b1[1], b1[2]);
-                if (k == 0 && kb == 0) fetch_u(v0);
+        for (int p = 0; p < 3; p++) next[p] = __ldcs(S0 + p * 32);
 #pragma unroll
-                for (int m = 0; m < 4; m++) {
-                    unsigned x[4];
-                    ldsm4(x, sq + (m * 16 + (lane & 15)) * QS + (kb + k) * 16 + (lane >> 4) * 8);
-                    mma16816(acc[m], x, b0[0], b1[0]);
-                    mma16816(low[m], x, b0[2], b1[2]);
-                    mma16816(low[m], x, b0[1], b1[1]);
+        for (int kk = 0; kk < NK; kk++) {
+            if (kk >= nk) break;
+            uint4 f[3];
+#pragma unroll
+            for (int p = 0; p < 3; p++) {
+                f[p] = next[p];
+                if (kk + 1 < nk) next[p] = __ldcs(S0 + ((kk + 1) * 3 + p) * 32);
+            }
+#pragma unroll
+            for (int m = 0; m < 4; m++) {
+                unsigned x[4];
+                ldsm4(x, sq + (m * 16 + (lane & 15)) * QS + kk * 16 + (lane >> 4) * 8);
+                mma16816(acc[m][0], x, f[0].x, f[0].z);
+                mma16816(acc[m][1], x, f[0].y, f[0].w);
+#pragma unroll
+                for (int p = 2; p > 0; p--) {
+                    mma16816(low[m][0], x, f[p].x, f[p].z);
+                    mma16816(low[m][1], x, f[p].y, f[p].w);
                 }
             }
         }
 #pragma unroll
         for (int m = 0; m < 4; m++) {
             const float fa = exp2f((float)sb[m * 16 + g]), fb = exp2f((float)sb[m * 16 + g + 8]);
-            acc[m][0] *= fa; acc[m][1] *= fa; acc[m][2] *= fb; acc[m][3] *= fb;
-            low[m][0] *= fa; low[m][1] *= fa; low[m][2] *= fb; low[m][3] *= fb;
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                acc[m][n][0] *= fa; acc[m][n][1] *= fa; acc[m][n][2] *= fb; acc[m][n][3] *= fb;
+                low[m][n][0] *= fa; low[m][n][1] *= fa; low[m][n][2] *= fb; low[m][n][3] *= fb;
+            }
         }
 #pragma unroll
         for (int kt = 0; kt < 4; kt++) {
-            unsigned b0[3], b1[3];
-            split3(fU[kt][0].x, fU[kt][0].y, b0[0], b0[1], b0[2]);
-            split3(fU[kt][1].x, fU[kt][1].y, b1[0], b1[1], b1[2]);
+            const float4 ua = __ldcs(U + 2 * kt * 32), ub = __ldcs(U + (2 * kt + 1) * 32);
+            unsigned b0[2][3], b1[2][3];
+            split3(ua.x, ua.y, b0[0][0], b0[0][1], b0[0][2]);
+            split3(ub.x, ub.y, b1[0][0], b1[0][1], b1[0][2]);
+            split3(ua.z, ua.w, b0[1][0], b0[1][1], b0[1][2]);
+            split3(ub.z, ub.w, b1[1][0], b1[1][1], b1[1][2]);
 #pragma unroll
             for (int m = kt; m < 4; m++) {
                 unsigned x[3][4];
 #pragma unroll
                 for (int p = 0; p < 3; p++) ldsm4(x[p], sP + (p * DC + m * 16 + (lane & 15)) * TS + kt * 16 + (lane >> 4) * 8);
-                mma16816(acc[m], x[0], b0[0], b1[0]);
-                mma16816(low[m], x[0], b0[2], b1[2]);
-                mma16816(low[m], x[2], b0[0], b1[0]);
-                mma16816(low[m], x[1], b0[1], b1[1]);
-                mma16816(low[m], x[0], b0[1], b1[1]);
-                mma16816(low[m], x[1], b0[0], b1[0]);
+#pragma unroll
+                for (int n = 0; n < 2; n++) {
+                    mma16816(low[m][n], x[0], b0[n][2], b1[n][2]);
+                    mma16816(acc[m][n], x[0], b0[n][0], b1[n][0]);
+                    mma16816(low[m][n], x[2], b0[n][0], b1[n][0]);
+                    mma16816(low[m][n], x[1], b0[n][1], b1[n][1]);
+                    mma16816(low[m][n], x[0], b0[n][1], b1[n][1]);
+                    mma16816(low[m][n], x[1], b0[n][0], b1[n][0]);
+                }
             }
         }
 #pragma unroll
@@ -650,8 +701,11 @@ __global__ void __launch_bounds__(NW * 32, DeltaOut<NK, NW>::CTAS) k_delta_out(c
                 const int t = m * 16 + g + 8 * e;
                 if (t >= c.rows) continue;
                 const float f = srq[t];
-                *(float2*)(P.o + (c.row0 + t) * P.ldo + (long)h * dvp + v0 + 2 * tg) =
-                    make_float2(f * (acc[m][2 * e] + low[m][2 * e]), f * (acc[m][2 * e + 1] + low[m][2 * e + 1]));
+                float* o = P.o + (c.row0 + t) * P.ldo + (long)h * dvp + vt * 16 + 2 * tg;
+#pragma unroll
+                for (int n = 0; n < 2; n++)
+                    if (vt * 16 + 8 * n < dvp)
+                        *(float2*)(o + 8 * n) = make_float2(f * (acc[m][n][2 * e] + low[m][n][2 * e]), f * (acc[m][n][2 * e + 1] + low[m][n][2 * e + 1]));
             }
     }
 }
@@ -669,8 +723,11 @@ static long delta_chunks(const lt_dn_seqs* Q) {
     for (int i = 0; i < Q->n && i < LT_DN_SEQS; i++) n += (Q->rows[i] + DC - 1) / DC;
     return n;
 }
-// fp32 elements of one chunk and head
-static long delta_chunk_floats(const lt_dn_delta* D) { return 3L * DC * DC / 2 + DVEC + (long)D->dvp * D->dp + (long)D->dvp * DC; }
+// fp32 elements of one chunk, all heads
+static long delta_chunk_floats(const lt_dn_delta* D) {
+    const long nkt = (D->dp + 15) / 16, nvt = (D->dvp + 15) / 16;
+    return D->H * (nkt * 12 * 128 + nvt * nkt * 3 * 128 + nvt * 8 * 128 + DVEC) + D->G * nkt * 4 * 128;
+}
 
 }  // namespace dn
 }  // namespace lt
@@ -679,7 +736,7 @@ using namespace lt;
 using namespace lt::dn;
 
 extern "C" long lt_dn_delta_chunked_ws(const lt_dn_delta* h_d, const lt_dn_seqs* h_q) {
-    return delta_chunks(h_q) * h_d->H * delta_chunk_floats(h_d);
+    return delta_chunks(h_q) * delta_chunk_floats(h_d);
 }
 
 extern "C" int lt_dn_delta_chunked(const void* q, const void* k, const void* v, int ld, const float* la, int ldla, const float* beta, int ldb, float* o,
@@ -701,18 +758,21 @@ extern "C" int lt_dn_delta_chunked(const void* q, const void* k, const void* v, 
     for (int i = P.Q.n; i < LT_DN_SEQS; i++) P.first[i + 1] = P.first[P.Q.n];
     const int chunks = P.first[P.Q.n];
     const long n = (long)chunks * P.D.H;
-    P.T3 = (bf16*)ws;
-    P.vec = ws + n * (3 * DC * DC / 2);
-    P.S0 = P.vec + n * DVEC;
-    P.U = P.S0 + n * P.D.dvp * P.D.dp;
+    P.nkt = (P.D.dp + 15) / 16;
+    P.nvt = (P.D.dvp + 15) / 16;
+    P.W = (uint4*)ws;
+    P.S0 = P.W + n * P.nkt * 12 * 32;
+    P.U = (float4*)(P.S0 + n * P.nvt * P.nkt * 3 * 32);
+    P.Kf = (uint4*)(P.U + n * P.nvt * 8 * 32);
+    P.vec = (float*)(P.Kf + (long)chunks * P.D.G * P.nkt * 4 * 32);
     cudaStream_t s = (cudaStream_t)stream;
     const int dp = P.D.dp;
     static PerDeviceOnce once;
-    if (once.first()) LT_CUDA(cudaFuncSetAttribute(k_delta_prep, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)prep_smem(256)));
-    k_delta_prep<<<dim3(chunks, P.D.H), PREP_THREADS, prep_smem(dp), s>>>(P);
+    if (once.first()) LT_CUDA(cudaFuncSetAttribute(k_delta_prep, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)prep_smem(256, 32)));
+    k_delta_prep<<<dim3(chunks, P.D.H), PREP_THREADS, prep_smem(dp, P.nvt), s>>>(P);
     int rc = check_launch("lt_dn_delta_chunked (prepare)");
     if (rc != LT_OK) return rc;
-    rc = dp <= 64 ? launch_states<4, 1, 2>(P, s) : dp <= 128 ? launch_states<8, 1, 3>(P, s) : launch_states<8, 2, 2>(P, s);
+    rc = dp <= 64 ? launch_states<4, 1>(P, s) : dp <= 128 ? launch_states<8, 1>(P, s) : launch_states<8, 2>(P, s);
     if (rc != LT_OK) return rc;
     const bool few = P.D.dvp <= 64;
     if (dp <= 64) return few ? launch_delta_out<4, 4>(P, chunks, s) : launch_delta_out<4, 8>(P, chunks, s);

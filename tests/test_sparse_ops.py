@@ -107,7 +107,7 @@ def test_delta_refusals():
     chunked("alignment", ldo=97)
     chunked("null pointer", ws=None)
     chunked("one state", q=seqs((0, 5, 256), (5, 5, 256)))
-    assert _lib.dense().lt_dn_delta_chunked_ws(delta(), seqs((0, 65, 256), (65, 0, 512))) == 2 * 4 * (3 * 64 * 64 // 2 + 132 + 24 * 16 + 24 * 64)
+    assert _lib.dense().lt_dn_delta_chunked_ws(delta(), seqs((0, 65, 256), (65, 0, 512))) == 2 * (4 * (1536 + 2 * 384 + 2 * 1024 + 68) + 2 * 512)
     step = lambda text, d=delta(), S=one: _refused("lt_dn_delta_step", text, one, one, one, one, S, one, 0, one, one, d, None)
     step("taps=0", delta(taps=0))
     step("null constants", delta(conv=None))
