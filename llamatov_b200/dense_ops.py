@@ -134,7 +134,15 @@ def _here(t, what):
     return t
 
 
-GROUP_FROM = 64         # places from which on the products go expert by expert
+def group_from(n):
+    """Places from which on the products of n experts go expert by expert, and not place by place.  An expert's matrix is read once
+    then, which pays when experts are hit more than once, but the order of the places and the rows in that order cost launches.  (bf16,
+    gate|up, us place by place / by expert: 64 experts of 1024 x 2048, 32 places 42 / 54, 48 57 / 58, 64 74 / 66; 8 of 2048 x 2048, 8 places
+    26 / 34, 12 32 / 35, 16 39 / 34; 128 of 512 x 1024, 64 places 25 / 34.)"""
+    return GROUP_FROM if GROUP_FROM is not None else max(14, 3 * n // 4)
+
+
+GROUP_FROM = None       # a number: whatever the experts
 
 
 class Router:
@@ -194,7 +202,7 @@ class Experts:
         _here(ids, "ids")
         _here(self.W, "the experts' matrix")
         top = ids.shape[1]
-        if T * top < GROUP_FROM:
+        if T * top < group_from(self.n):
             return Places(ids, self.n)
         buf = torch.empty(_lib.dense().lt_dn_experts_plan_ints(T, top, self.n), dtype=torch.int32, device="cuda")
         _lib.call("lt_dn_experts_plan", ids.data_ptr(), T, top, self.n, buf.data_ptr(), _stream())
@@ -219,7 +227,15 @@ class Experts:
 
 # --------------------------------------------------------------------------- delta rule
 
-DELTA_CHUNKED_FROM = 64         # tokens of the longest sequence from which on bf16 rows are walked in chunks
+def delta_chunked_from(ctas):
+    """Tokens of the longest sequence from which on bf16 rows are walked in chunks, and not in token order, which takes no
+    preparation but more per token, the more CTAs (of 16 value columns) share an SM.  (us in token order / in chunks: 16 heads of 128,
+    128 CTAs: 256 tokens 37 / 39, 512 68 / 46; 32 heads: 128 tokens 32 / 38, 256 56 / 44; four sequences of 16 heads: 64 tokens 34 / 38,
+    128 57 / 45.)"""
+    return DELTA_CHUNKED_FROM if DELTA_CHUNKED_FROM is not None else 256 if ctas <= 148 else 176 if ctas <= 296 else 96
+
+
+DELTA_CHUNKED_FROM = None       # a number: whatever the sizes
 
 
 class DeltaRule:
@@ -250,7 +266,8 @@ class DeltaRule:
                 seqs.start[j], seqs.rows[j], seqs.S[j] = at, r, states[i + j]
                 at += r
             args = (q, k, v, ld, la, ldh, beta, ldb, o, ldo)
-            if self.f32 or max(part) < DELTA_CHUNKED_FROM or self.dim > 256 or self.vdim > 512:
+            ctas = (self.vdim + 15) // 16 * self.H * len(part)
+            if self.f32 or max(part) < delta_chunked_from(ctas) or self.dim > 256 or self.vdim > 512:
                 _lib.call("lt_dn_delta_rows", *args, self.f32, self._ref, ctypes.byref(seqs), _stream())
                 continue
             ws = torch.empty(_lib.dense().lt_dn_delta_chunked_ws(self._ref, ctypes.byref(seqs)), dtype=torch.float32, device="cuda")
