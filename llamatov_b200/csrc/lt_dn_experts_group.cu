@@ -6,12 +6,13 @@
 // as hold them, and N is the share rounded up to 16: rows of no place cost at most 15 columns of a tile, whatever the shares are.
 // The rows of X are first put in the order of the plan (k_gather), so that tiled TMA fetches them.  (Fetched from where they are by
 // gathering TMA, four rows an instruction: 83 clocks each, 425 us for gate|up 2 x 1024 x 2048 of 8 of 64 experts, 2000 tokens; by
-// asynchronous copies of 16 bytes: 203; in order 167, 12 of it for putting them there.)
+// asynchronous copies of 16 bytes: 203; in order 165, 12 of it for putting them there.)
 //   warp 16 : producer, TMA
 //   warp 17 : one thread issues the MMAs
 //   warps 0-15 : epilogue, a thread per weight row and a quarter of the places
-// What bounds it is the traffic between L2 and the SMs (64 KB for 1024 clocks of MMAs at N = 256) and the epilogue, which runs alone
-// where 2 N columns fill the tensor memory.
+// What bounds it is the traffic between L2 and the SMs (64 KB for 1024 clocks of MMAs at N = 256; 108 us of the 153 without MMAs and
+// epilogue) and the epilogue, which runs alone where 2 N columns fill the tensor memory.  (Two SMs on a tile, cta_group::2 with M = 256,
+// move 48 KB for the same MMAs, but a stage's way through the barriers of both took 1.4 us with four stages: 216.)
 // fp32 (k_group_f32): register-blocked tiles on the CUDA cores.
 #include "lt_dn_experts.cuh"
 #include "lt_tc.cuh"
@@ -291,7 +292,8 @@ static int group_map(CUtensorMap* m, const void* ptr, long rows, int K, int ld, 
     cuuint32_t box[2] = {(cuuint32_t)GK, (cuuint32_t)box_rows};
     cuuint32_t estr[2] = {1, 1};
     CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                    // 256 bytes into L2 at a time: a row's next 128 are the next stage's (gate|up of 2000 tokens 159 -> 153 us)
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
         set_error("experts' products: cuTensorMapEncodeTiled failed (%d) for rows=%ld K=%d ld=%d", (int)r, rows, K, ld);
         return LT_ERR_CUDA;

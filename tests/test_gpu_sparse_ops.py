@@ -153,7 +153,7 @@ def _ids(T, top, n, seed, how="spread"):
 SIZES = [  # T, top, n, K, F or M
     (1, 1, 1, 8, 1), (1, 2, 4, 24, 9), (1, 8, 64, 264, 136), (2, 3, 5, 40, 130), (17, 2, 3, 72, 33), (37, 4, 16, 896, 616), (64, 4, 8, 64, 128),
     (65, 1, 2, 128, 256), (200, 8, 16, 136, 264), (33, 32, 40, 16, 24), (300, 2, 70, 520, 136),
-    (600, 1, 2, 200, 40), (515, 2, 2, 64, 300)]
+    (600, 1, 2, 200, 40), (515, 2, 2, 64, 300), (300, 2, 3, 136, 264), (290, 2, 3, 72, 520), (700, 1, 1, 64, 1030)]
 
 
 def _check_glu(T, top, n, K, F, f32, how="spread", act="gelu", seed=1, ids=None):
