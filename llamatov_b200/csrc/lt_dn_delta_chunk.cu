@@ -19,6 +19,9 @@
 // products of the leading parts have accumulators of their own: the tensor cores cut sums off instead of rounding them, which costs
 // up to 2^-24 of the accumulator at every step.
 //
+// A row that is not finite (infinities, NaN) makes the outputs of its whole chunk not finite, earlier tokens' among them: products
+// over a chunk have zeros where token order has nothing.  Other sequences and earlier chunks are as they would be.
+//
 // The walk over the chunks is the longest of the three, and bound by the instructions and waits of a chunk's dependent chain.  So W, U0
 // and the keys lie in memory as the lanes hold them (16 bytes a lane, side by side) and go straight into registers, asked for when
 // the chunk before has used them; a chunk passes two barriers.  (16 heads of 128, 2048 rows: 32, 70 and 37 us; four

@@ -157,8 +157,8 @@ static int launch_route(const RouteP& P, int each, int own, cudaStream_t s) {
 
 // ---------------------------------------------------------------------------- order of the places by expert
 
-// A warp owns a stretch of the places and looks at 32 of them at a time, eight loads ahead: 16384 places of 64 experts take
-// 3 us.  (A stretch per thread made every load of a warp touch 32 lines: 19 us.)
+// A warp owns a stretch of the places and looks at 32 of them at a time, eight loads ahead: 16000 places of 64 experts take
+// 5 us.  (A stretch per thread made every load of a warp touch 32 lines: 19 us.)
 constexpr int PLAN_THREADS = 512, PLAN_AHEAD = 8;
 
 __global__ void __launch_bounds__(PLAN_THREADS) k_plan(const int* __restrict__ ids, int P, int n, int* __restrict__ plan, int* status) {

@@ -122,9 +122,13 @@ def cast_input(x, n1, x2=None):
 
 # --------------------------------------------------------------------------- sparse feed-forwards
 
-def _stream():
-    """The current stream's handle, as dev_residency._stream, without the Stream object that it makes (3 us of a call's 8)."""
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+def _stream(home=None):
+    """The current stream's handle, as dev_residency._stream, without the Stream object that it makes (3 us of a call's 8).  home:
+    the device that the caller's own memory is on; a launch on another one is refused."""
+    device = torch.cuda.current_device()
+    if home is not None and home != device:
+        raise ValueError(f"made on cuda:{home}, the current device is cuda:{device}")
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 def _here(t, what):
@@ -158,20 +162,21 @@ class Router:
             raise ValueError(f"bias {tuple(bias.shape)} for {n} experts")
         self.n, self.top = n, top
         self.bias = None if bias is None else bias.float().cuda().contiguous()
+        self.home = None if bias is None else self.bias.device.index
         self.desc = _lib.DnRouter(n, top, _lib.DN_SCORE[score], groups, top_groups, int(renorm), float(scale),
                                   None if bias is None else self.bias.data_ptr())
         self._ref = ctypes.byref(self.desc)
 
     def rows(self, logits, ld, ids, w, T):
         """ids int32 [T][top] and w fp32 [T][top] of T rows of logits."""
-        _lib.call("lt_dn_route", logits, ld, ids, w, T, self._ref, _stream())
+        _lib.call("lt_dn_route", logits, ld, ids, w, T, self._ref, _stream(self.home))
 
 
 class Places:
     """Chosen experts of T tokens (ids int32 [T, top]) and, with `plan`, the order of the places by expert."""
 
     def __init__(self, ids, n, plan=None):
-        self.ids, self.buf = ids, plan
+        self.ids, self.n, self.buf = ids, n, plan
         self.T, self.top = ids.shape
         self.desc = _lib.DnChoice(ids.data_ptr(), None if plan is None else plan.data_ptr(), self.T, self.top, n)
         self.ref = ctypes.byref(self.desc)
@@ -190,6 +195,7 @@ class Experts:
         if K % 8:
             W = torch.cat([W, W.new_zeros(n, M, pad8(K) - K)], dim=2)
         self.W = W.cuda().contiguous()
+        self.home = self.W.device.index
         self.n, self.M, self.K = n, M // 2 if gated else M, pad8(K)
         self.gated, self.f32 = gated, int(W.dtype == torch.float32)
         self.ptr = self.W.data_ptr()
@@ -199,28 +205,30 @@ class Experts:
         """The places of T tokens, ids int32 [T, top]."""
         if ids.dtype != torch.int32 or ids.dim() != 2 or ids.shape[0] != T or not ids.is_contiguous():
             raise ValueError(f"ids must be contiguous int32 [{T}, top], got {ids.dtype} {tuple(ids.shape)}")
+        stream = _stream(self.home)
         _here(ids, "ids")
-        _here(self.W, "the experts' matrix")
         top = ids.shape[1]
         if T * top < group_from(self.n):
             return Places(ids, self.n)
         buf = torch.empty(_lib.dense().lt_dn_experts_plan_ints(T, top, self.n), dtype=torch.int32, device="cuda")
-        _lib.call("lt_dn_experts_plan", ids.data_ptr(), T, top, self.n, buf.data_ptr(), _stream())
+        _lib.call("lt_dn_experts_plan", ids.data_ptr(), T, top, self.n, buf.data_ptr(), stream)
         return Places(ids, self.n, buf)
 
     def hidden(self, x, ldx, places, h, ldh):
         """h[t*top + j] = glu of the gate and up rows of place (t, j)'s expert, for the rows of x."""
         ws = self._workspace(places, "lt_dn_experts_glu_ws", self.K)
         _lib.call("lt_dn_experts_glu", self.ptr, self.K, x, ldx, h, ldh, self.f32, self.M, self.K, places.ref, ctypes.byref(self.epi),
-                  None if ws is None else ws.data_ptr(), _stream())
+                  None if ws is None else ws.data_ptr(), _stream(self.home))
 
     def add_sum(self, h, ldh, places, w, y, ldy, ls=None):
         """y[t] += ls * sum over j of w[t][j] W h[t*top + j]."""
         ws = self._workspace(places, "lt_dn_experts_sum_ws", self.M, self.K)
         _lib.call("lt_dn_experts_sum", self.ptr, self.K, h, ldh, y, ldy, self.f32, self.M, self.K, places.ref, w, ls,
-                  None if ws is None else ws.data_ptr(), _stream())
+                  None if ws is None else ws.data_ptr(), _stream(self.home))
 
     def _workspace(self, places, query, *sizes):
+        if places.n != self.n:
+            raise ValueError(f"places of {places.n} experts, the matrices are of {self.n}")
         n = 0 if places.buf is None else getattr(_lib.dense(), query)(places.T, places.top, *sizes, self.f32)
         return torch.empty(n, dtype=torch.float32, device="cuda") if n else None
 
@@ -248,6 +256,7 @@ class DeltaRule:
         self.H, self.G, self.dim, self.vdim = H, G, dim, vdim
         self.f32 = int(dtype == torch.float32)
         self.keep = [None if t is None else t.float().contiguous() for t in (conv, conv_b, dt_bias, A)]
+        self.home = next((t.device.index for t in self.keep if t is not None), None)
         self.desc = _lib.DnDelta(H, G, dim, vdim, float(q_scale), float(eps), taps, *[None if t is None else _here(t, "a constant").data_ptr()
                                                                                    for t in self.keep])
         self._ref = ctypes.byref(self.desc)
@@ -258,7 +267,9 @@ class DeltaRule:
         ldb = ldh if ldb is None else ldb
         if len(states) != len(rows):
             raise ValueError(f"{len(states)} states for {len(rows)} sequences")
-        at = 0
+        if len(set(states)) != len(states):
+            raise ValueError("two sequences with one state")
+        at, stream = 0, _stream(self.home)
         for i in range(0, len(rows), _lib.DN_SEQS):
             part = rows[i:i + _lib.DN_SEQS]
             seqs = _lib.DnSeqs(n=len(part))
@@ -268,10 +279,10 @@ class DeltaRule:
             args = (q, k, v, ld, la, ldh, beta, ldb, o, ldo)
             ctas = (self.vdim + 15) // 16 * self.H * len(part)
             if self.f32 or max(part) < delta_chunked_from(ctas) or self.dim > 256 or self.vdim > 512:
-                _lib.call("lt_dn_delta_rows", *args, self.f32, self._ref, ctypes.byref(seqs), _stream())
+                _lib.call("lt_dn_delta_rows", *args, self.f32, self._ref, ctypes.byref(seqs), stream)
                 continue
             ws = torch.empty(_lib.dense().lt_dn_delta_chunked_ws(self._ref, ctypes.byref(seqs)), dtype=torch.float32, device="cuda")
-            _lib.call("lt_dn_delta_chunked", *args, self._ref, ctypes.byref(seqs), ws.data_ptr(), _stream())
+            _lib.call("lt_dn_delta_chunked", *args, self._ref, ctypes.byref(seqs), ws.data_ptr(), stream)
 
     def step(self, row, dt, beta, ring, S, o, len_, ticket):
-        _lib.call("lt_dn_delta_step", row, dt, beta, ring, S, o, self.f32, len_, ticket, self._ref, _stream())
+        _lib.call("lt_dn_delta_step", row, dt, beta, ring, S, o, self.f32, len_, ticket, self._ref, _stream(self.home))

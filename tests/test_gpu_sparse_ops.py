@@ -435,3 +435,199 @@ def test_delta_steps(f32, H, G, d, dv, taps):
                      _np(beta), np.zeros((H, dv, d)), d ** -0.5, 1e-6)
     eo, eS = _off(_np(o), wo.reshape(T, -1)), _off(_np(S), wS)
     assert eo <= _delta_tol(T) and eS <= _delta_tol(T)
+
+
+# --------------------------------------------------------------------------- as they are used together
+
+@pytest.mark.parametrize("f32", [0, 1])
+def test_places_left_out_are_not_read(form, f32):
+    """NaN in rows, weights and outputs of places that are left out, and in the columns behind a row's last."""
+    T, top, n, K, M = 70, 3, 5, 40, 24
+    nan = float("nan")
+    ids = _ids(T, top, n, 1)
+    ids[::4] = -1
+    ids[1::4, 1] = -1
+    off = (ids < 0).cuda()
+    X, H = _randn((T, K + 8), 2, DT[f32]), _randn((T * top, K + 8), 3, DT[f32])
+    w = torch.rand(T, top, generator=torch.Generator().manual_seed(4)).cuda()
+    Wg, Wd = _randn((n, 2 * M, K), 5, DT[f32], K ** -0.5), _randn((n, M, K), 6, DT[f32], K ** -0.5)
+    gu, down = P.Experts(Wg, gated=True), P.Experts(Wd, gated=False)
+
+    def run():
+        places = gu.plan(ids.cuda(), T)
+        h, y = torch.zeros(T * top, M, dtype=DT[f32], device="cuda"), torch.zeros(T, M, device="cuda")
+        gu.hidden(X.data_ptr(), K + 8, places, h.data_ptr(), M)
+        down.add_sum(H.data_ptr(), K + 8, places, w.data_ptr(), y.data_ptr(), M)
+        return h, y
+    want = run()
+    X[:, K:], H[:, K:] = nan, nan
+    X[off.all(1)] = nan
+    H[off.reshape(-1)] = nan
+    w[off] = nan
+    for a, b in zip(run(), want):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("chunks,f32", [(0, 0), (0, 1), (1, 0)])
+def test_delta_reads_no_rows_of_others(chunks, f32):
+    lengths, H, G, d, dv = [5, 1, 70], 4, 2, 24, 40
+
+    def call(op, q, k, v, ld, la, beta, o, seqs):
+        args = (q, k, v, ld, la.data_ptr(), H, beta.data_ptr(), H, o.data_ptr(), H * dv + 2)
+        if not chunks:
+            _lib.call("lt_dn_delta_rows", *args, f32, op._ref, ctypes.byref(seqs), stream())
+            return
+        ws = torch.full((_lib.dense().lt_dn_delta_chunked_ws(op._ref, ctypes.byref(seqs)),), float("nan"), device="cuda")
+        _lib.call("lt_dn_delta_chunked", *args, op._ref, ctypes.byref(seqs), ws.data_ptr(), stream())
+    rows, la, beta, S = _delta_case(lengths, H, G, d, dv, f32, seed=4, gap=2)
+    rows[:, -8:] = float("nan")
+    for at in (0, 7, 10):
+        for t in (rows, la, beta):
+            t[at:at + 2] = float("nan")
+    eo, eS = _delta_run(rows, la, beta, S, lengths, H, G, d, dv, f32, gap=2, call=call)
+    assert eo <= _delta_tol(70) and eS <= _delta_tol(70)
+
+
+class _Layer:
+    """A router, experts and a delta rule on buffers of their own: one pass over them, as a layer makes it."""
+
+    def __init__(self, T, f32, seed):
+        n, top, E, F, H, d = 8, 2, 64, 40, 2, 32
+        self.T, self.n, self.top, self.E, self.F, self.H, self.d = T, n, top, E, F, H, d
+        dt = DT[f32]
+        self.router = P.Router(n, top, score="sigmoid", bias=_randn((n,), seed, scale=0.1))
+        self.gu = P.Experts(_randn((n, 2 * F, E), seed + 1, dt, E ** -0.5), gated=True)
+        self.down = P.Experts(_randn((n, E, F), seed + 2, dt, F ** -0.5), gated=False)
+        self.rule = P.DeltaRule(H, H, d, d, dt, d ** -0.5, 1e-6)
+        self.logits, self.x = _randn((T, n), seed + 3), _randn((T, E), seed + 4, dt)
+        self.row = _randn((T, 3 * H * d), seed + 5, dt)
+        self.la, self.beta = -torch.rand(T, H, device="cuda"), torch.rand(T, H, device="cuda")
+        self.S0, self.S = _randn((H, d, d), seed + 6), torch.empty(H, d, d, device="cuda")
+        self.y, self.o = torch.empty(T, E, device="cuda"), torch.empty(T, H * d, device="cuda")
+        self.h = torch.empty(T * top, F, dtype=dt, device="cuda")
+        self.ids = torch.empty(T, top, dtype=torch.int32, device="cuda")
+        self.w = torch.empty(T, top, device="cuda")
+
+    def run(self):
+        T, e, n = self.T, self.row.element_size(), self.H * self.d
+        self.y.zero_()
+        self.S.copy_(self.S0)
+        self.router.rows(self.logits.data_ptr(), self.n, self.ids.data_ptr(), self.w.data_ptr(), T)
+        places = self.gu.plan(self.ids, T)
+        self.gu.hidden(self.x.data_ptr(), self.E, places, self.h.data_ptr(), self.F)
+        self.down.add_sum(self.h.data_ptr(), self.F, places, self.w.data_ptr(), self.y.data_ptr(), self.E)
+        r = self.row.data_ptr()
+        self.rule.rows(r + 2 * n * e, r + n * e, r, 3 * n, self.la.data_ptr(), self.beta.data_ptr(), self.H, self.o.data_ptr(), n,
+                       [self.S.data_ptr()], [T])
+
+    def out(self):
+        return [t.clone() for t in (self.ids, self.w, self.h, self.y, self.o, self.S)]
+
+
+@pytest.mark.parametrize("f32", [0, 1])
+@pytest.mark.parametrize("T", [1, 300])
+def test_captured_passes_side_by_side(f32, T):
+    """Two captured graphs replayed at once on two streams, with inputs changed after the capture, and eager passes on a stream of
+    their own between them: every one gives what a pass alone gives, bit by bit."""
+    a, b, c = _Layer(T, f32, 10), _Layer(T, f32, 20), _Layer(T, f32, 30)
+    graphs = []
+    for l in (a, b):
+        l.run()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            l.run()
+        graphs.append(g)
+    for l, seed in ((a, 50), (b, 60)):
+        l.logits.copy_(_randn((T, l.n), seed))
+        l.x.copy_(_randn((T, l.E), seed + 1, DT[f32]))
+        l.row.copy_(_randn((T, l.row.shape[1]), seed + 2, DT[f32]))
+    want = []
+    for l in (a, b, c):
+        l.run()
+        want.append(l.out())
+        for t in (l.ids, l.w, l.h, l.y, l.o, l.S):
+            t.zero_()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for _ in range(5):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        with torch.cuda.stream(streams[2]):
+            c.run()
+    torch.cuda.synchronize()
+    for l, ws in zip((a, b, c), want):
+        for got, w in zip(l.out(), ws):
+            assert torch.equal(got, w)
+
+
+@pytest.mark.parametrize("f32", [0, 1])
+def test_many_places(f32):
+    """160000 places."""
+    T, top, n, K, M = 20000, 8, 64, 40, 24
+    ids = _ids(T, top, n, 1).cuda()
+    X, W = _randn((T, K), 2, DT[f32]), _randn((n, 2 * M, K), 3, DT[f32], K ** -0.5)
+    gu = P.Experts(W, gated=True)
+    places = gu.plan(ids, T)
+    h = torch.full((T * top, M), 7.0, dtype=DT[f32], device="cuda")
+    gu.hidden(X.data_ptr(), K, places, h.data_ptr(), M)
+    D, w = _randn((n, K, M), 4, DT[f32], M ** -0.5), torch.rand(T, top, device="cuda")
+    y = torch.zeros(T, K, device="cuda")
+    P.Experts(D, gated=False).add_sum(h.data_ptr(), M, places, w.data_ptr(), y.data_ptr(), K)
+    want, size = torch.zeros(T, K, dtype=torch.float64, device="cuda"), torch.zeros(T, K, dtype=torch.float64, device="cuda")
+    for j in range(top):
+        e = ids[:, j].long()
+        for t0 in range(0, T, 4000):
+            s = slice(t0, t0 + 4000)
+            v = torch.einsum("tmk,tk->tm", W[e[s]].double(), X[s].double())
+            g, u = v[:, :M], v[:, M:]
+            gu64 = 0.5 * g * (1 + torch.tanh((2 / np.pi) ** 0.5 * (g + 0.044715 * g ** 3))) * u
+            hj = h.reshape(T, top, M)[s, j].double()
+            tol = (8 * K ** 0.5 + 16) * E32 * (1 + g.abs()) * (1 + u.abs()) * 3 + (0 if f32 else 2.0 ** -8) * gu64.abs()     # as above
+            assert ((hj - gu64).abs() <= tol).all()
+            want[s] += w[s, j, None] * torch.einsum("tmk,tk->tm", D[e[s]].double(), hj)
+            size[s] += w[s, j, None] * torch.einsum("tmk,tk->tm", D[e[s]].double().abs(), hj.abs())
+    assert ((y - want).abs() <= (8 * M ** 0.5 + top + 2) * E32 * size).all()
+
+
+def test_matrices_past_32_bits(form):
+    """The last experts of matrices of 2.2e9 elements."""
+    n, M, K, T = 131, 1024, 8192, 40
+    W = torch.zeros(n, 2 * M, K, dtype=torch.bfloat16, device="cuda")
+    W[-2:] = _randn((2, 2 * M, K), 1, torch.bfloat16, K ** -0.5)
+    ids = (n - 2 + torch.arange(2 * T) % 2).reshape(T, 2).int().cuda()
+    X, h = _randn((T, K), 2, torch.bfloat16), torch.empty(2 * T, M, dtype=torch.bfloat16, device="cuda")
+    gu = P.Experts(W, gated=True, glu=GLU["clamped"][0])
+    places = gu.plan(ids, T)
+    gu.hidden(X.data_ptr(), K, places, h.data_ptr(), M)
+    down = P.Experts(W, gated=False)
+    y, w = torch.zeros(2 * T, 2 * M, device="cuda"), torch.ones(2 * T, 1, device="cuda")
+    X2 = X.repeat_interleave(2, 0)
+    places = down.plan(ids.reshape(-1, 1), 2 * T)
+    down.add_sum(X2.data_ptr(), K, places, w.data_ptr(), y.data_ptr(), 2 * M)
+    x = _np(X).repeat(2, 0).reshape(T, 2, K)
+    for j in range(2):
+        v = x[:, j] @ _np(W[n - 2 + j]).T
+        size = np.abs(x[:, j]) @ np.abs(_np(W[n - 2 + j])).T
+        assert (np.abs(_np(y).reshape(T, 2, -1)[:, j] - v) <= (8 * K ** 0.5 + 3) * E32 * size).all()
+        want = GLU["clamped"][1](v[:, :M], v[:, M:])
+        tol = (8 * K ** 0.5 + 16) * E32 * (1 + np.abs(v[:, :M])) * (1 + np.abs(v[:, M:])) * 3 + 2.0 ** -8 * np.abs(want)
+        assert (np.abs(_np(h).reshape(T, 2, -1)[:, j] - want) <= tol).all()
+
+
+def test_delta_rows_far_apart(walk):
+    """Rows 2^20 elements and more apart: offsets past 2^31."""
+    f32, T, H, d = walk, 2100, 1, 8
+    ld = 2 ** 20 + 32
+    rows = torch.empty(T, ld, dtype=DT[f32], device="cuda")
+    rows[:, :3 * d] = _randn((T, 3 * d), 1, DT[f32])
+    o = torch.empty(T, ld, device="cuda")
+    la, beta, S0 = -torch.rand(T, H, device="cuda") * 0.3, torch.rand(T, H, device="cuda"), _randn((H, d, d), 2)
+    S = S0.clone()
+    p, e = rows.data_ptr(), rows.element_size()
+    P.DeltaRule(H, H, d, d, DT[f32], 0.25, 1e-6).rows(p + 2 * d * e, p + d * e, p, ld, la.data_ptr(), beta.data_ptr(), H, o.data_ptr(), ld,
+                                                    [S.data_ptr()], [T])
+    x = _np(rows[:, :3 * d])[:, None]
+    wo, wS = delta64(x[..., 2 * d:], x[..., d:2 * d], x[..., :d], _np(la), _np(beta), _np(S0), 0.25, 1e-6)
+    assert _off(_np(o[:, :d]), wo[:, 0]) <= _delta_tol(T) and _off(_np(S), wS) <= _delta_tol(T)

@@ -140,6 +140,38 @@ def test_objects_refuse():
         P.DeltaRule(3, 2, 8, 8, torch.float32, 1.0, 1e-6)
 
 
+def test_calls_that_do_not_fit_together_are_refused(monkeypatch):
+    """Places of other experts, one state for two sequences, an object of another device (no device is reached)."""
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda d: 0, raising=False)
+    monkeypatch.setattr(torch.Tensor, "cuda", lambda t: t)
+    W = P.Experts(torch.zeros(4, 8, 8), gated=False)
+    places = P.Places(torch.zeros(3, 2, dtype=torch.int32), 5)
+    with pytest.raises(ValueError, match="places of 5 experts"):
+        W.add_sum(1, 8, places, 1, 1, 8)
+    with pytest.raises(ValueError, match="places of 5 experts"):
+        P.Experts(torch.zeros(4, 8, 8), gated=True).hidden(1, 8, places, 1, 8)
+    rule = P.DeltaRule(2, 2, 8, 8, torch.float32, 1.0, 1e-6)
+    with pytest.raises(ValueError, match="one state"):
+        rule.rows(1, 1, 1, 16, 1, 1, 2, 1, 16, [64, 128, 64], [1, 2, 3])
+    with pytest.raises(ValueError, match="2 states"):
+        rule.rows(1, 1, 1, 16, 1, 1, 2, 1, 16, [64, 128], [1, 2, 3])
+    router = P.Router(4, 2, bias=torch.zeros(4))
+    ids = torch.zeros(3, 2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="ids is on cpu"):
+        W.plan(ids, 3)
+    with pytest.raises(ValueError, match="contiguous int32"):
+        W.plan(ids.long(), 3)
+    with pytest.raises(ValueError, match="contiguous int32"):
+        W.plan(ids, 2)
+    for o in (W, rule, router):
+        o.home = 1
+    for call in (lambda: W.plan(ids, 3), lambda: W.add_sum(1, 8, P.Places(ids, 4), 1, 1, 8), lambda: router.rows(1, 4, 1, 1, 3),
+                 lambda: rule.rows(1, 1, 1, 16, 1, 1, 2, 1, 16, [64], [1]), lambda: rule.step(1, 1, 1, 1, 1, 1, 1, 1)):
+        with pytest.raises(ValueError, match="current device is cuda:0"):
+            call()
+
+
 def test_models_with_bad_sizes_are_refused(monkeypatch):
     """Packing refuses what does not fit together (no device is reached)."""
     from llamatov_b200 import mixers
