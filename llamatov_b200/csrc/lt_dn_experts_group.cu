@@ -8,7 +8,7 @@
 // gathering TMA, four rows an instruction: 83 clocks each, 425 us for gate|up 2 x 1024 x 2048 of 8 of 64 experts, 2000 tokens; by
 // asynchronous copies of 16 bytes: 203; in order 165, 12 of it for putting them there.)
 //   warp 16 : producer, TMA
-//   warp 17 : one thread issues the MMAs
+//   warp 17 : MMAs (a warp's loop with one thread picked at the instructions: 2 % less than that thread's own loop)
 //   warps 0-15 : epilogue, a thread per weight row and a quarter of the places
 // What bounds it is the traffic between L2 and the SMs (64 KB for 1024 clocks of MMAs at N = 256; 108 us of the 153 without MMAs and
 // epilogue) and the epilogue, which runs alone where 2 N columns fill the tensor memory.  (Two SMs on a tile, cta_group::2 with M = 256,
@@ -146,6 +146,7 @@ k_group_tc(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
     if (warp == C::EW) {
         unsigned it = 0;
         bool go = true;
+        const bool one = elect_one();
         for (int tile = blockIdx.x; go && tile < tiles; tile += gridDim.x) {
             cur.seek(P, cum, tile);
             const int row = GLU ? cur.e * 2 * P.M + cur.rt * 128 : cur.e * P.M + cur.rt * 256;
@@ -157,7 +158,7 @@ k_group_tc(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
                     go = false;
                     break;
                 }
-                if (lane == 0) {
+                if (one) {
                     bar_expect_tx(full, C::W_STAGE + ((cur.n + XBOX - 1) & ~(XBOX - 1)) * 128);
                     tma_load_2d(st, &tmW, kb * GK, row, full);
                     tma_load_2d(st + 128 * 128, &tmW, kb * GK, row2, full);
@@ -167,21 +168,22 @@ k_group_tc(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
             }
         }
     } else if (warp == C::EW + 1) {
-        if (lane == 0) {
+        {
+            const bool one = elect_one();
             const unsigned long long w0 = smem_desc<4>(smem_u32(base));
             const unsigned long long x0 = smem_desc<4>(smem_u32(base) + C::W_STAGE);
             unsigned it = 0, n = 0;
             for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
                 cur.seek(P, cum, tile);
-                    // D fp32, A and B bf16, both K-major, M = 128
+                // D fp32, A and B bf16, both K-major, M = 128
                 const unsigned idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(cur.n >> 3) << 17) | ((unsigned)(128 >> 4) << 24);
                 const unsigned slot = n % C::BUFS;
-                mbar_wait<32>(&B->tempty[slot], ((n / C::BUFS) & 1) ^ 1, abort_flag, P.status);
+                bar_wait(false, smem_u32(&B->tempty[slot]), ((n / C::BUFS) & 1) ^ 1, abort_flag, P.status);
                 tc_fence_after();
                 const unsigned d = tmem + slot * 2 * NT;
                 for (int kb = 0; kb < nk; kb++, it++) {
                     const unsigned s = it % NS;
-                    mbar_wait<0>(&B->full[s], (it / NS) & 1, abort_flag, P.status);
+                    bar_wait(false, smem_u32(&B->full[s]), (it / NS) & 1, abort_flag, P.status);
                     tc_fence_after();
                     const unsigned long long wd = w0 + (unsigned long long)(s * (C::STAGE >> 4));
                     const unsigned long long xd = x0 + (unsigned long long)(s * (C::STAGE >> 4));
@@ -189,10 +191,10 @@ k_group_tc(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
                     for (int j = 0; j < GK / 16; j++)
 #pragma unroll
                         for (int a = 0; a < 2; a++)
-                            group_mma(d + a * NT, wd + a * (128 * 128 >> 4) + 2 * j, xd + 2 * j, idesc, kb > 0 || j > 0);
-                    mma_commit(&B->empty[s]);
+                            if (one) group_mma(d + a * NT, wd + a * (128 * 128 >> 4) + 2 * j, xd + 2 * j, idesc, kb > 0 || j > 0);
+                    if (one) mma_commit(&B->empty[s]);
                 }
-                mma_commit(&B->tfull[slot]);
+                if (one) mma_commit(&B->tfull[slot]);
                 n++;
             }
         }
@@ -206,7 +208,7 @@ k_group_tc(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
             int mine[NT / 64];                // places of this warp's columns, fetched under the products
 #pragma unroll
             for (int i = 0; i < NT / 64; i++) mine[i] = places[cur.from + min(64 * i + cg * 16 + (lane & 15), cur.count - 1)];
-            mbar_wait<32>(&B->tfull[slot], (n / C::BUFS) & 1, abort_flag, P.status);
+            bar_wait(false, smem_u32(&B->tfull[slot]), (n / C::BUFS) & 1, abort_flag, P.status);
             tc_fence_after();
             const unsigned ta = tmem + ((unsigned)(q * 32) << 16) + slot * 2 * NT;
             auto release = [&]() {
