@@ -6,11 +6,11 @@
 // as hold them, and N is the share rounded up to 16: rows of no place cost at most 15 columns of a tile, whatever the shares are.
 // The rows of X are first put in the order of the plan (k_gather), so that tiled TMA fetches them.  (Fetched from where they are by
 // gathering TMA, four rows an instruction: 83 clocks each, 425 us for gate|up 2 x 1024 x 2048 of 8 of 64 experts, 2000 tokens; by
-// asynchronous copies of 16 bytes: 203; in order 165, 12 of it for putting them there.)
+// asynchronous copies of 16 bytes: 203; in order 162, 13 of it for putting them there.)
 //   warp 16 : producer, TMA
 //   warp 17 : MMAs (a warp's loop with one thread picked at the instructions: 2 % less than that thread's own loop)
 //   warps 0-15 : epilogue, a thread per weight row and a quarter of the places
-// What bounds it is the traffic between L2 and the SMs (64 KB for 1024 clocks of MMAs at N = 256; 108 us of the 153 without MMAs and
+// What bounds it is the traffic between L2 and the SMs (64 KB for 1024 clocks of MMAs at N = 256; 108 us of 153 without MMAs and
 // epilogue) and the epilogue, which runs alone where 2 N columns fill the tensor memory.  (Two SMs on a tile, cta_group::2 with M = 256,
 // move 48 KB for the same MMAs, but a stage's way through the barriers of both took 1.4 us with four stages: 216.)
 // fp32 (k_group_f32): register-blocked tiles on the CUDA cores.
@@ -33,7 +33,7 @@ struct GroupCfg {
     static constexpr int BUFS = NT <= 128 ? 2 : 1;          // sets of accumulators
     static constexpr int TMEM = BUFS * 2 * NT;
     static constexpr int EW = 16, THREADS = (EW + 2) * 32;
-    static constexpr int SMEM = 1024 + NSTAGE * STAGE + 512 + (MAX_EXPERTS + 1) * 4;
+    static constexpr int SMEM = 1024 + NSTAGE * STAGE + 512 + (MAX_EXPERTS + 1) * 4 + MAX_EXPERTS * 4;
     static_assert(TMEM <= 512 && (TMEM & (TMEM - 1)) == 0, "tensor memory columns");
     static_assert(SMEM <= 227 * 1024, "shared memory");
 };
@@ -42,7 +42,7 @@ struct GroupBars {
     unsigned long long full[8], empty[8], tfull[2], tempty[2];
     unsigned tmem_base;
     int abort_flag;
-    int warp_tiles[18];
+    int sums[18];
 };
 
 // D[tmem] (+)= A[smem] * B[smem], bf16 x bf16 -> fp32
@@ -61,21 +61,81 @@ __device__ __forceinline__ float gelu_up(float z, float u) {
     return __fdividef(z * u, 1.0f + e);
 }
 
-// Tiles of places by expert: cum[e] tiles lie before expert e's.  Every role walks them with a cursor of its own.
-template <int NT>
+// Experts in order of their tiles' columns, the widest first: cum[i] tiles lie before the i-th's, which is expert order[i].  CTAs take
+// tiles in turn, there and back, so that the wide and the last narrow ones are shared out evenly, as well as by handing them out one by
+// one.  (Gate|up of 2000 tokens 143 us, with experts as they are numbered 149.)  Every role walks them with a cursor of its own.
 struct Cursor {
-    int e;
+    int i, e;
     int from, count, n, rt;      // places of the tile in the plan's list, columns, row tile
-    __device__ __forceinline__ void seek(const GroupP& P, const int* cum, int tile) {
+    __device__ __forceinline__ void seek(const GroupP& P, const int* cum, const int* order, int tile) {
         const int g = tile / P.row_tiles;
         rt = tile - g * P.row_tiles;
-        while (cum[e + 1] <= g) e++;
-        const int at = P.c.plan[e], c = P.c.plan[e + 1] - at, tiles = cum[e + 1] - cum[e];
+        while (cum[i + 1] <= g) i++;
+        e = order[i];
+        const int at = P.c.plan[e], c = P.c.plan[e + 1] - at, tiles = cum[i + 1] - cum[i];
         n = ((c + tiles - 1) / tiles + 15) & ~15;
-        from = at + (g - cum[e]) * n;
+        from = at + (g - cum[i]) * n;
         count = min(n, at + c - from);       // at least 1: the tiles before hold (tiles - 1) n <= (tiles - 1) NT < c places
     }
 };
+__device__ __forceinline__ int tile_of(int round) {
+    return round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+}
+// makes cum and order; all threads, 16 warps and more
+template <int NT>
+__device__ __forceinline__ void sort_tiles(const lt_dn_choice& c, int* cum, int* order, int* sums) {
+    static_assert(NT / 16 <= 16, "a warp per number of columns");
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    int* columns = cum;                    // in units of 16, until the order is known
+    for (int e = tid; e < c.n; e += blockDim.x) {
+        const int all = c.plan[e + 1] - c.plan[e], tiles = (all + NT - 1) / NT;
+        columns[e] = tiles > 0 ? ((all + tiles - 1) / tiles + 15) / 16 : 0;
+    }
+    __syncthreads();
+    const int mine = NT / 16 - warp;       // this warp's number of columns
+    int at = 0;
+    if (mine > 0)
+        for (int e0 = 0; e0 < c.n; e0 += 32) at += __popc(__ballot_sync(0xffffffffu, e0 + lane < c.n && columns[e0 + lane] == mine));
+    if (lane == 0) sums[warp] = at;
+    __syncthreads();
+    at = 0;
+    for (int w = 0; w < warp; w++) at += sums[w];
+    int used = 0;
+    for (int w = 0; w < (int)(blockDim.x >> 5); w++) used += sums[w];
+    if (mine > 0)
+        for (int e0 = 0; e0 < c.n; e0 += 32) {
+            const bool ok = e0 + lane < c.n && columns[e0 + lane] == mine;
+            const unsigned here = __ballot_sync(0xffffffffu, ok);
+            if (ok) order[at + __popc(here & ((1u << lane) - 1))] = e0 + lane;
+            at += __popc(here);
+        }
+    __syncthreads();
+    int t[4], sum = 0;                     // sums of tiles: four experts a thread
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        t[k] = 0;
+        if (tid * 4 + k < used) {
+            const int e = order[tid * 4 + k];
+            t[k] = (c.plan[e + 1] - c.plan[e] + NT - 1) / NT;
+        }
+        sum += t[k];
+    }
+    int before = sum;
+#pragma unroll
+    for (int s = 1; s < 32; s <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, before, s);
+        if (lane >= s) before += o;
+    }
+    if (lane == 31) sums[warp] = before;
+    __syncthreads();
+    before -= sum;
+    for (int w = 0; w < warp; w++) before += sums[w];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        if (tid * 4 + k <= c.n) cum[tid * 4 + k] = before;
+        before += t[k];
+    }
+}
 
 template <int NT, bool GLU>
 __global__ void __launch_bounds__(GroupCfg<NT>::THREADS, 1)
@@ -86,6 +146,7 @@ k_group_tc(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
     unsigned char* base = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     GroupBars* B = (GroupBars*)(base + NS * C::STAGE);
     int* cum = (int*)(base + NS * C::STAGE + 512);
+    int* order = cum + MAX_EXPERTS + 1;
     static_assert(sizeof(GroupBars) <= 512, "barriers");
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int nk = (P.K + GK - 1) / GK;
@@ -111,44 +172,21 @@ k_group_tc(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    {   // sums of the experts' tiles: four experts a thread
-        int t[4], sum = 0;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int e = tid * 4 + i;
-            t[i] = e < P.c.n ? (P.c.plan[e + 1] - P.c.plan[e] + NT - 1) / NT : 0;
-            sum += t[i];
-        }
-        int before = sum;
-#pragma unroll
-        for (int s = 1; s < 32; s <<= 1) {
-            const int o = __shfl_up_sync(0xffffffffu, before, s);
-            if (lane >= s) before += o;
-        }
-        if (lane == 31) B->warp_tiles[warp] = before;
-        __syncthreads();
-        before -= sum;
-        for (int w = 0; w < warp; w++) before += B->warp_tiles[w];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if (tid * 4 + i <= P.c.n) cum[tid * 4 + i] = before;
-            before += t[i];
-        }
-    }
+    sort_tiles<NT>(P.c, cum, order, B->sums);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const unsigned tmem = B->tmem_base;
     const int tiles = cum[P.c.n] * P.row_tiles;
-    Cursor<NT> cur;
-    cur.e = 0;
+    Cursor cur;
+    cur.i = 0;
 
     if (warp == C::EW) {
         unsigned it = 0;
         bool go = true;
         const bool one = elect_one();
-        for (int tile = blockIdx.x; go && tile < tiles; tile += gridDim.x) {
-            cur.seek(P, cum, tile);
+        for (int round = 0, tile; go && (tile = tile_of(round)) < tiles; round++) {
+            cur.seek(P, cum, order, tile);
             const int row = GLU ? cur.e * 2 * P.M + cur.rt * 128 : cur.e * P.M + cur.rt * 256;
             const int row2 = GLU ? row + P.M : row + 128;
             for (int kb = 0; kb < nk; kb++, it++) {
@@ -173,8 +211,8 @@ k_group_tc(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
             const unsigned long long w0 = smem_desc<4>(smem_u32(base));
             const unsigned long long x0 = smem_desc<4>(smem_u32(base) + C::W_STAGE);
             unsigned it = 0, n = 0;
-            for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-                cur.seek(P, cum, tile);
+            for (int round = 0, tile; (tile = tile_of(round)) < tiles; round++) {
+                cur.seek(P, cum, order, tile);
                 // D fp32, A and B bf16, both K-major, M = 128
                 const unsigned idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(cur.n >> 3) << 17) | ((unsigned)(128 >> 4) << 24);
                 const unsigned slot = n % C::BUFS;
@@ -201,8 +239,8 @@ k_group_tc(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
     } else {
         const int q = warp & 3, cg = warp >> 2;
         unsigned n = 0;
-        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-            cur.seek(P, cum, tile);
+        for (int round = 0, tile; (tile = tile_of(round)) < tiles; round++) {
+            cur.seek(P, cum, order, tile);
             const int row = cur.rt * (GLU ? 128 : 256) + q * 32 + lane;
             const unsigned slot = n % C::BUFS;
             int mine[NT / 64];                // places of this warp's columns, fetched under the products
