@@ -5,7 +5,7 @@
 // With a plan: lt_dn_experts_group.cu.  Without one (few places) each place reads its expert's rows itself, and the time is that of
 // the matrices' bytes.
 //   k_few_glu   a warp per gate row and its up row
-//   k_few_sum   a CTA per rows of Y; its warps share the experts of the token, and their sums are added in order of j
+//   k_few_sum   a CTA per rows of Y; its warps share the experts of the token, and their sums are added in order
 #include "lt_dn_experts.cuh"
 
 namespace lt {
@@ -23,7 +23,7 @@ struct FewP {
 };
 
 // An SM has four CTAs of 64 registers a thread, each lane with two rows x 4 loads of 16 bytes under way.  (8 of 64 experts for one
-// token in bf16: gate|up 2 x 1024 x 2048 14.2 us, 4.7 TB/s, down 2048 x 1024 10.5; with two CTAs that also hold their part of x
+// token in bf16: gate|up 2 x 1024 x 2048 14.2 us, 4.7 TB/s, down 2048 x 1024 10.0; with two CTAs that also hold their part of x
 // ahead 15.1 and 13.3; twice the loads a lane 16.0 and 14.0; rows through rings of bulk copies in shared memory, 192 KB under way,
 // 20.1 and 15.9.)
 constexpr int FEW_THREADS = 256, FEW_U = 4, FEW_CTAS = 4;
@@ -188,10 +188,13 @@ extern "C" int lt_dn_experts_sum(const void* W, int ldw, const void* H, int ldh,
     LT_REQUIRE(h_c->T <= 65535, "lt_dn_experts_sum: %d tokens without an order of the places (at most 65535)", h_c->T);
     FewP P = {W, H, Y, w, ls, device_status_ptr(), ldw, ldh, ldy, M, K, *h_c, {}};
     LT_REQUIRE(P.status != nullptr, "lt_dn_experts_sum: status word unavailable");
+    // As many warps on a token's experts as leave no CTA more than its first pairs of rows.  (One token, 8 of 64 experts, 2048 x 1024, by 8 /
+    // 4 / 2 / 1 warps: 10.8 / 10.0 / 11.1 / 15.2 us, the rule takes 4; 4096 x 512: 14.1 / 11.5 / 10.0 / 12.5, 2; 1024 x 512: 6.6 / 6.9 / 7.9 /
+    // 11.1, 8; four tokens: 13.7 / 11.4 / 9.9 / 11.8, 2.)
+    const int npair = (M + 1) / 2, most = (FEW_CTAS * sm_count() + h_c->T - 1) / h_c->T;
     int wj = 1;
-    while (wj < h_c->top && wj < FEW_THREADS / 32) wj *= 2;
-    const int pairs = FEW_THREADS / 32 / wj, need = ((M + 1) / 2 + pairs - 1) / pairs;
-    const int most = (FEW_CTAS * sm_count() + h_c->T - 1) / h_c->T;
+    while (wj < h_c->top && wj < FEW_THREADS / 32 && (long)npair * 2 * wj <= (long)most * (FEW_THREADS / 32)) wj *= 2;
+    const int pairs = FEW_THREADS / 32 / wj, need = (npair + pairs - 1) / pairs;
     const dim3 grid(need < most ? need : most, h_c->T);
     if (f32) k_few_sum<float><<<grid, FEW_THREADS, 0, (cudaStream_t)stream>>>(P, wj);
     else k_few_sum<bf16><<<grid, FEW_THREADS, 0, (cudaStream_t)stream>>>(P, wj);
