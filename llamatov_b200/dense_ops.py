@@ -244,6 +244,7 @@ def delta_chunked_from(ctas):
 
 
 DELTA_CHUNKED_FROM = None       # a number: whatever the sizes
+DELTA_PORTION = 4096            # rows of a sequence that are walked in chunks at a time (a multiple of 64): 32 heads of 128 have 6 MB of workspace a chunk
 
 
 class DeltaRule:
@@ -253,6 +254,8 @@ class DeltaRule:
     def __init__(self, H, G, dim, vdim, dtype, q_scale, eps, taps=0, conv=None, conv_b=None, dt_bias=None, A=None):
         if H % G or dim % 8 or vdim % 8:
             raise ValueError(f"{H} heads on {G} key heads, sizes {dim} and {vdim} (multiples of 8)")
+        if dtype not in DTYPES.values():
+            raise ValueError(f"rows of {dtype}")
         self.H, self.G, self.dim, self.vdim = H, G, dim, vdim
         self.f32 = int(dtype == torch.float32)
         self.keep = [None if t is None else t.float().contiguous() for t in (conv, conv_b, dt_bias, A)]
@@ -269,6 +272,8 @@ class DeltaRule:
             raise ValueError(f"{len(states)} states for {len(rows)} sequences")
         if len(set(states)) != len(states):
             raise ValueError("two sequences with one state")
+        if any(r < 0 for r in rows):
+            raise ValueError(f"rows of sequences {rows}")
         at, stream = 0, _stream(self.home)
         for i in range(0, len(rows), _lib.DN_SEQS):
             part = rows[i:i + _lib.DN_SEQS]
@@ -281,8 +286,12 @@ class DeltaRule:
             if self.f32 or max(part) < delta_chunked_from(ctas) or self.dim > 256 or self.vdim > 512:
                 _lib.call("lt_dn_delta_rows", *args, self.f32, self._ref, ctypes.byref(seqs), stream)
                 continue
-            ws = torch.empty(_lib.dense().lt_dn_delta_chunked_ws(self._ref, ctypes.byref(seqs)), dtype=torch.float32, device="cuda")
-            _lib.call("lt_dn_delta_chunked", *args, self._ref, ctypes.byref(seqs), ws.data_ptr(), stream)
+            starts = seqs.start[:len(part)]
+            for done in range(0, max(part), DELTA_PORTION):
+                for j, r in enumerate(part):
+                    seqs.start[j], seqs.rows[j] = starts[j] + min(done, r), max(0, min(r - done, DELTA_PORTION))
+                ws = torch.empty(_lib.dense().lt_dn_delta_chunked_ws(self._ref, ctypes.byref(seqs)), dtype=torch.float32, device="cuda")
+                _lib.call("lt_dn_delta_chunked", *args, self._ref, ctypes.byref(seqs), ws.data_ptr(), stream)
 
     def step(self, row, dt, beta, ring, S, o, len_, ticket):
         _lib.call("lt_dn_delta_step", row, dt, beta, ring, S, o, self.f32, len_, ticket, self._ref, _stream(self.home))

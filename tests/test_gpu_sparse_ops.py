@@ -616,6 +616,21 @@ def test_matrices_past_32_bits(form):
         assert (np.abs(_np(h).reshape(T, 2, -1)[:, j] - want) <= tol).all()
 
 
+def test_delta_long_sequences_in_portions(monkeypatch):
+    """Sequences longer than a portion of the chunked walk give the bits of one portion."""
+    lengths, H, G, d, dv = [300, 0, 65, 128, 1], 4, 2, 24, 40
+    monkeypatch.setattr(P, "DELTA_CHUNKED_FROM", 1)
+    out = []
+    for portion in (4096, 128):
+        monkeypatch.setattr(P, "DELTA_PORTION", portion)
+        rows, la, beta, S = _delta_case(lengths, H, G, d, dv, 0, seed=6)
+        eo, eS = _delta_run(rows, la, beta, S, lengths, H, G, d, dv, 0)
+        assert eo <= _delta_tol(300) and eS <= _delta_tol(300)
+        out.append(S)
+    for a, b in zip(*out):
+        assert torch.equal(a, b)
+
+
 def test_delta_rows_far_apart(walk):
     """Rows 2^20 elements and more apart: offsets past 2^31."""
     f32, T, H, d = walk, 2100, 1, 8

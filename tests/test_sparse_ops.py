@@ -154,6 +154,10 @@ def test_calls_that_do_not_fit_together_are_refused(monkeypatch):
     rule = P.DeltaRule(2, 2, 8, 8, torch.float32, 1.0, 1e-6)
     with pytest.raises(ValueError, match="one state"):
         rule.rows(1, 1, 1, 16, 1, 1, 2, 1, 16, [64, 128, 64], [1, 2, 3])
+    with pytest.raises(ValueError, match="rows of sequences"):
+        rule.rows(1, 1, 1, 16, 1, 1, 2, 1, 16, [64, 128], [1000, -1])
+    with pytest.raises(ValueError, match="float16"):
+        P.DeltaRule(2, 2, 8, 8, torch.float16, 1.0, 1e-6)
     with pytest.raises(ValueError, match="2 states"):
         rule.rows(1, 1, 1, 16, 1, 1, 2, 1, 16, [64, 128], [1, 2, 3])
     router = P.Router(4, 2, bias=torch.zeros(4))
