@@ -723,7 +723,7 @@ static int launch_delta_out(const DeltaChunkP& P, int chunks, cudaStream_t s) {
 
 static long delta_chunks(const lt_dn_seqs* Q) {
     long n = 0;
-    for (int i = 0; i < Q->n && i < LT_DN_SEQS; i++) n += (Q->rows[i] + DC - 1) / DC;
+    for (int i = 0; i < Q->n && i < LT_DN_SEQS; i++) n += ((long)Q->rows[i] + DC - 1) / DC;
     return n;
 }
 // fp32 elements of one chunk, all heads
@@ -739,6 +739,8 @@ using namespace lt;
 using namespace lt::dn;
 
 extern "C" long lt_dn_delta_chunked_ws(const lt_dn_delta* h_d, const lt_dn_seqs* h_q) {
+    int rows = 0;      // of a call that would be refused: nothing
+    if (delta_error(h_d) != nullptr || delta_seqs_error(h_q, &rows) != nullptr) return 0;
     return delta_chunks(h_q) * delta_chunk_floats(h_d);
 }
 
@@ -757,7 +759,7 @@ extern "C" int lt_dn_delta_chunked(const void* q, const void* k, const void* v, 
     DeltaChunkP P = {};
     P.q = (const bf16*)q; P.k = (const bf16*)k; P.v = (const bf16*)v; P.la = la; P.beta = beta; P.o = o;
     P.ld = ld; P.ldla = ldla; P.ldb = ldb; P.ldo = ldo; P.D = *h_d; P.Q = *h_q;
-    for (int i = 0; i < P.Q.n; i++) P.first[i + 1] = P.first[i] + (P.Q.rows[i] + DC - 1) / DC;
+    for (int i = 0; i < P.Q.n; i++) P.first[i + 1] = P.first[i] + (int)(((long)P.Q.rows[i] + DC - 1) / DC);
     for (int i = P.Q.n; i < LT_DN_SEQS; i++) P.first[i + 1] = P.first[P.Q.n];
     const int chunks = P.first[P.Q.n];
     const long n = (long)chunks * P.D.H;

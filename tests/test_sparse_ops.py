@@ -121,6 +121,13 @@ def test_no_rows_is_no_launch():
     assert _lib.launch_count() == n
 
 
+def test_workspace_of_a_refused_call_is_none():
+    size = _lib.dense().lt_dn_delta_chunked_ws
+    assert size(delta(), seqs((0, 100, 256))) == 2 * size(delta(), seqs((0, 1, 256))) > 0
+    assert size(None, seqs((0, 1, 256))) == 0 and size(delta(), None) == 0
+    assert size(delta(), seqs((0, -70, 256))) == 0 and size(delta(G=3), seqs((0, 1, 256))) == 0
+
+
 def test_objects_refuse():
     with pytest.raises(ValueError, match="score"):
         P.Router(8, 2, score="tanh")
