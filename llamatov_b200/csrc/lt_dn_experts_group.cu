@@ -10,9 +10,9 @@
 //   warp 16 : producer, TMA
 //   warp 17 : MMAs (a warp's loop with one thread picked at the instructions: 2 % less than that thread's own loop)
 //   warps 0-15 : epilogue, a thread per weight row and a quarter of the places
-// What bounds it is the traffic between L2 and the SMs (64 KB for 1024 clocks of MMAs at N = 256; 108 us of 153 without MMAs and
-// epilogue) and the epilogue, which runs alone where 2 N columns fill the tensor memory.  (Two SMs on a tile, cta_group::2 with M = 256,
-// move 48 KB for the same MMAs, but a stage's way through the barriers of both took 1.4 us with four stages: 216.)
+// What bounds it is the matrices' bytes with what shares the way: of 143 us (gate|up, 537 MB in 607 MB of reads) the copies of W alone take
+// 109, 5.6 TB/s; the sums' fp32 outputs are 23 us of 92.  (Two SMs on a tile, cta_group::2 with M = 256, halve X's bytes: 137 and 92 us for as
+// much code again.  An L2 prefetch four stages ahead: 4 % more; one accumulator of the sums kept in registers over its release: nothing.)
 // fp32 (k_group_f32): register-blocked tiles on the CUDA cores.
 #include "lt_dn_experts.cuh"
 #include "lt_tc.cuh"
