@@ -141,8 +141,9 @@ def _here(t, what):
 def group_from(n):
     """Places from which on the products of n experts go expert by expert, and not place by place.  An expert's matrix is read once
     then, which pays when experts are hit more than once, but the order of the places and the rows in that order cost launches.  (bf16,
-    gate|up, us place by place / by expert: 64 experts of 1024 x 2048, 32 places 42 / 54, 48 57 / 58, 64 74 / 66; 8 of 2048 x 2048, 8 places
-    26 / 34, 12 32 / 35, 16 39 / 34; 128 of 512 x 1024, 64 places 25 / 34.)"""
+    us place by place / by expert, gate|up and then down: 64 experts of 1024 x 2048, 32 places 43 / 50 and 25 / 36, 48 57 / 53 and
+    36 / 38, 64 75 / 59 and 39 / 41; 8 of 2048 x 2048, 8 places 26 / 32 and 15 / 26, 12 34 / 32 and 19 / 28, 16 40 / 33 and 21 / 28, 24
+    52 / 33 and 30 / 29; 128 of 512 x 1024, 64 places 25 / 33 and 16 / 23.)"""
     return GROUP_FROM if GROUP_FROM is not None else max(14, 3 * n // 4)
 
 
