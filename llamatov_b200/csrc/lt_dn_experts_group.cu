@@ -646,10 +646,14 @@ static int launch_group_f32_few(const GroupP& P, cudaStream_t s) {
 }
 // By places of an expert.  Gated, 64 experts of 512 x 2048, us in registers / tiles of 32 places: 8 180 / 294, 16 275 / 321, 24 375 / 322.
 // Sums, 2048 x 512, in registers / tiles of 16 / of 32: 4 91 / 92 / 125, 8 122 / 114 / 137, 16 180 / 147 / 156, 24 242 / 187 / 180.
+// Gated tiles that leave SMs idle are in registers too, in many more CTAs.  (About so many tiles, us in registers /
+// tiles: 82 of 2048 x 512 64 / 93, 92 of 4096 x 1024 127 / 174, 109 of 1616 x 264 66 / 76, 107 of 512 x 256 30 / 29, 208 of 896 x 616
+// 90 / 69.)
 template <bool GLU>
 static int pick_group_f32(const GroupP& P, cudaStream_t s) {
     const long each = (long)P.c.T * P.c.top / P.c.n;
-    if (each <= (GLU ? 18 : 5)) return launch_group_f32_few<GLU>(P, s);
+    const long tiles = (P.M + GF_BM - 1) / GF_BM * ((long)P.c.T * P.c.top / 32 + P.c.n / 2);
+    if (each <= (GLU ? 18 : 5) || (GLU && tiles <= 3 * sm_count() / 4)) return launch_group_f32_few<GLU>(P, s);
     if (!GLU && each <= 20) return launch_group_f32<false, 2>(P, s);
     return launch_group_f32<GLU, 4>(P, s);
 }
