@@ -184,8 +184,9 @@ class Places:
 
 
 class Experts:
-    """A matrix per expert, [n, rows, columns].  gated: rows are gate rows and as many up rows, and `hidden` stores their gated
-    product; else `add_sum` adds the weighted sum of the chosen experts' outputs to fp32 rows.  glu: as in `epilogue`."""
+    """A matrix per expert, [n, rows, columns], the columns a multiple of 8.  gated: rows are gate rows and as many up rows, and
+    `hidden` stores their gated product; else `add_sum` adds the weighted sum of the chosen experts' outputs to fp32 rows.  glu: as
+    in `epilogue`."""
 
     def __init__(self, W, gated, glu=(_lib.DN_GLU_GELU, 0.0, 0.0)):
         if W.dim() != 3 or W.dtype not in DTYPES.values():
@@ -193,11 +194,11 @@ class Experts:
         n, M, K = W.shape
         if gated and M % 2:
             raise ValueError(f"{M} gate and up rows")
-        if K % 8:
-            W = torch.cat([W, W.new_zeros(n, M, pad8(K) - K)], dim=2)
+        if K % 8:                # columns added here would be read of the caller's rows too, where nothing has written them
+            raise ValueError(f"{K} columns: they must be a multiple of 8 (zeros in the matrices and in the rows)")
         self.W = W.cuda().contiguous()
         self.home = self.W.device.index
-        self.n, self.M, self.K = n, M // 2 if gated else M, pad8(K)
+        self.n, self.M, self.K = n, M // 2 if gated else M, K
         self.gated, self.f32 = gated, int(W.dtype == torch.float32)
         self.ptr = self.W.data_ptr()
         self.epi = epilogue(_lib.DN_GLU, glu=glu) if gated else None

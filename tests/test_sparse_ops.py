@@ -147,6 +147,16 @@ def test_objects_refuse():
         P.DeltaRule(3, 2, 8, 8, torch.float32, 1.0, 1e-6)
 
 
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("K", [1, 9, 12, 63])
+def test_columns_that_are_no_multiple_of_8_are_refused(monkeypatch, K, gated):
+    """The products read whole units of 8 columns of a caller's rows, and a NaN there times a column of zeros is a NaN."""
+    monkeypatch.setattr(torch.Tensor, "cuda", lambda t: t)
+    with pytest.raises(ValueError, match=f"{K} columns"):
+        P.Experts(torch.zeros(2, 6, K), gated=gated)
+    assert P.Experts(torch.zeros(2, 6, 64), gated=gated).K == 64
+
+
 def test_calls_that_do_not_fit_together_are_refused(monkeypatch):
     """Places of other experts, one state for two sequences, an object of another device (no device is reached)."""
     monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
