@@ -218,12 +218,16 @@ class Experts:
 
     def hidden(self, x, ldx, places, h, ldh):
         """h[t*top + j] = glu of the gate and up rows of place (t, j)'s expert, for the rows of x."""
+        if not self.gated:
+            raise ValueError("the matrices have no gate and up rows: their products are add_sum's")
         ws = self._workspace(places, "lt_dn_experts_glu_ws", self.K)
         _lib.call("lt_dn_experts_glu", self.ptr, self.K, x, ldx, h, ldh, self.f32, self.M, self.K, places.ref, ctypes.byref(self.epi),
                   None if ws is None else ws.data_ptr(), _stream(self.home))
 
     def add_sum(self, h, ldh, places, w, y, ldy, ls=None):
         """y[t] += ls * sum over j of w[t][j] W h[t*top + j]."""
+        if self.gated:
+            raise ValueError("the matrices are gate and up rows: their product is hidden's")
         ws = self._workspace(places, "lt_dn_experts_sum_ws", self.M, self.K)
         _lib.call("lt_dn_experts_sum", self.ptr, self.K, h, ldh, y, ldy, self.f32, self.M, self.K, places.ref, w, ls,
                   None if ws is None else ws.data_ptr(), _stream(self.home))

@@ -157,6 +157,18 @@ def test_columns_that_are_no_multiple_of_8_are_refused(monkeypatch, K, gated):
     assert P.Experts(torch.zeros(2, 6, 64), gated=gated).K == 64
 
 
+def test_products_of_the_other_kind_of_matrices_are_refused(monkeypatch):
+    """Gate and up rows are twice as many as the sums would count, so that every expert but the first would be another."""
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.Tensor, "cuda", lambda t: t)
+    monkeypatch.setattr(_lib, "call", lambda name, *a: pytest.fail(f"{name} was called"))
+    places = P.Places(torch.zeros(3, 2, dtype=torch.int32), 4)
+    with pytest.raises(ValueError, match="gate and up rows"):
+        P.Experts(torch.zeros(4, 8, 8), gated=True).add_sum(256, 8, places, 256, 256, 8)
+    with pytest.raises(ValueError, match="gate and up rows"):
+        P.Experts(torch.zeros(4, 8, 8), gated=False).hidden(256, 8, places, 256, 8)
+
+
 def test_calls_that_do_not_fit_together_are_refused(monkeypatch):
     """Places of other experts, one state for two sequences, an object of another device (no device is reached)."""
     monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
