@@ -264,6 +264,10 @@ class DeltaRule:
             raise ValueError(f"rows of {dtype}")
         self.H, self.G, self.dim, self.vdim = H, G, dim, vdim
         self.f32 = int(dtype == torch.float32)
+        C = H * vdim + 2 * G * dim
+        for name, t, shape in (("conv", conv, (taps, C)), ("conv_b", conv_b, (C,)), ("dt_bias", dt_bias, (H,)), ("A", A, (H,))):
+            if t is not None and tuple(t.shape) != shape:        # a token's step reads all of it
+                raise ValueError(f"{name} {tuple(t.shape)} for {taps} taps, {C} channels and {H} heads")
         self.keep = [None if t is None else t.float().contiguous() for t in (conv, conv_b, dt_bias, A)]
         self.home = next((t.device.index for t in self.keep if t is not None), None)
         self.desc = _lib.DnDelta(H, G, dim, vdim, float(q_scale), float(eps), taps, *[None if t is None else _here(t, "a constant").data_ptr()

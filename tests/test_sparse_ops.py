@@ -169,6 +169,18 @@ def test_products_of_the_other_kind_of_matrices_are_refused(monkeypatch):
         P.Experts(torch.zeros(4, 8, 8), gated=False).hidden(256, 8, places, 256, 8)
 
 
+@pytest.mark.parametrize("name,shape", [("conv", (4, 95)), ("conv", (3, 96)), ("conv", (96, 4)), ("conv_b", (95,)), ("dt_bias", (1,)), ("A", (2, 1))])
+def test_constants_of_other_sizes_are_refused(monkeypatch, name, shape):
+    """A token's step would read behind them."""
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(P, "_here", lambda t, what: t)
+    sizes = {"conv": (4, 96), "conv_b": (96,), "dt_bias": (2,), "A": (2,)}
+    make = lambda **kw: P.DeltaRule(2, 1, 24, 24, torch.float32, 1.0, 1e-6, taps=4, **{n: torch.zeros(kw.get(n, s)) for n, s in sizes.items()})
+    assert make().desc.taps == 4
+    with pytest.raises(ValueError, match=rf"^{name} "):
+        make(**{name: shape})
+
+
 def test_calls_that_do_not_fit_together_are_refused(monkeypatch):
     """Places of other experts, one state for two sequences, an object of another device (no device is reached)."""
     monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
