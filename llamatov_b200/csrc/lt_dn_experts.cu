@@ -125,6 +125,9 @@ __global__ void __launch_bounds__(FEW_THREADS, FEW_CTAS) k_few_sum(const __grid_
     }
 }
 
+// of the matrices together: a tile's row is an int coordinate of their tensor map
+constexpr long MAX_ROWS = 0x7fffffffL;
+
 static const char* choice_error(const lt_dn_choice* c) {
     if (c == nullptr || c->ids == nullptr) return "null choice";
     if (c->T <= 0 || c->top <= 0 || c->top > 32 || c->n <= 0 || c->n > 1024) return "tokens, top (at most 32) or experts (at most 1024)";
@@ -150,6 +153,7 @@ extern "C" int lt_dn_experts_glu(const void* W, int ldw, const void* X, int ldx,
     LT_REQUIRE(aligned16(W) && aligned16(X), "lt_dn_experts_glu: W and X must be 16-byte aligned");
     if (h_c->plan != nullptr) {
         LT_REQUIRE(f32 || (ws != nullptr && aligned16(ws)), "lt_dn_experts_glu: a plan needs the workspace, 16-byte aligned");
+        LT_REQUIRE(f32 || 2L * F * h_c->n <= MAX_ROWS, "lt_dn_experts_glu: %ld rows of all matrices", 2L * F * h_c->n);
         GroupP G = {W, X, H, device_status_ptr(), F, K, ldw, ldx, ldh, h_c->top, 0, *h_c, *h_epi};
         LT_REQUIRE(G.status != nullptr, "lt_dn_experts_glu: status word unavailable");
         return launch_group(G, true, f32, ws, (cudaStream_t)stream);
@@ -180,6 +184,7 @@ extern "C" int lt_dn_experts_sum(const void* W, int ldw, const void* H, int ldh,
     LT_REQUIRE(aligned16(W) && aligned16(H), "lt_dn_experts_sum: W and H must be 16-byte aligned");
     if (h_c->plan != nullptr) {
         LT_REQUIRE(ws != nullptr && aligned16(ws), "lt_dn_experts_sum: a plan needs the workspace, 16-byte aligned");
+        LT_REQUIRE(f32 || (long)M * h_c->n <= MAX_ROWS, "lt_dn_experts_sum: %ld rows of all matrices", (long)M * h_c->n);
         GroupP G = {W, H, ws, device_status_ptr(), M, K, ldw, ldh, M, 1, 0, *h_c, {}};
         LT_REQUIRE(G.status != nullptr, "lt_dn_experts_sum: status word unavailable");
         const int rc = launch_group(G, false, f32, ws + places_floats(h_c->T, h_c->top, M), (cudaStream_t)stream);

@@ -79,6 +79,13 @@ def test_experts_refusals():
     assert L.lt_dn_experts_sum_ws(5, 3, 9, 16, 1) == 136 and L.lt_dn_experts_sum_ws(5, 3, 9, 16, 0) == 256
 
 
+def test_matrices_of_more_rows_than_an_int_counts_are_refused():
+    """Tensor-map coordinates are ints: rows past 2^31 would be read as zeros."""
+    e, F = P.epilogue(_lib.DN_GLU, glu=(0, 0.0, 0.0)), 1 << 20
+    _refused("lt_dn_experts_glu", f"{1024 * 2 * F} rows", one, 8, one, 8, one, F, 0, F, 8, choice(n=1024, plan=256, T=400, top=4), ctypes.byref(e), one, None)
+    _refused("lt_dn_experts_sum", f"{1024 * 2 * F} rows", one, 8, one, 8, one, 2 * F, 0, 2 * F, 8, choice(n=1024, plan=256, T=400, top=4), one, None, one, None)
+
+
 def test_delta_refusals():
     rows = lambda text, d=delta(), q=seqs((0, 5, 256)), ld=96, ldh=4, ldo=96: _refused(
         "lt_dn_delta_rows", text, one, one, one, ld, one, ldh, one, ldh, one, ldo, 0, d, q, None)
