@@ -174,10 +174,11 @@ class Router:
 
 
 class Places:
-    """Chosen experts of T tokens (ids int32 [T, top]) and, with `plan`, the order of the places by expert."""
+    """Chosen experts of T tokens (ids int32 [T, top]) and, with `plan`, the order of the places by expert.  stream: the handle of
+    the stream that `plan` was allocated on, None where its memory is the caller's to keep."""
 
-    def __init__(self, ids, n, plan=None):
-        self.ids, self.n, self.buf = ids, n, plan
+    def __init__(self, ids, n, plan=None, stream=None):
+        self.ids, self.n, self.buf, self.stream = ids, n, plan, stream
         self.T, self.top = ids.shape
         self.desc = _lib.DnChoice(ids.data_ptr(), None if plan is None else plan.data_ptr(), self.T, self.top, n)
         self.ref = ctypes.byref(self.desc)
@@ -214,27 +215,31 @@ class Experts:
             return Places(ids, self.n)
         buf = torch.empty(_lib.dense().lt_dn_experts_plan_ints(T, top, self.n), dtype=torch.int32, device="cuda")
         _lib.call("lt_dn_experts_plan", ids.data_ptr(), T, top, self.n, buf.data_ptr(), stream)
-        return Places(ids, self.n, buf)
+        return Places(ids, self.n, buf, stream)
 
     def hidden(self, x, ldx, places, h, ldh):
         """h[t*top + j] = glu of the gate and up rows of place (t, j)'s expert, for the rows of x."""
         if not self.gated:
             raise ValueError("the matrices have no gate and up rows: their products are add_sum's")
-        ws = self._workspace(places, "lt_dn_experts_glu_ws", self.K)
+        stream = _stream(self.home)
+        ws = self._workspace(places, stream, "lt_dn_experts_glu_ws", self.K)
         _lib.call("lt_dn_experts_glu", self.ptr, self.K, x, ldx, h, ldh, self.f32, self.M, self.K, places.ref, ctypes.byref(self.epi),
-                  None if ws is None else ws.data_ptr(), _stream(self.home))
+                  None if ws is None else ws.data_ptr(), stream)
 
     def add_sum(self, h, ldh, places, w, y, ldy, ls=None):
         """y[t] += ls * sum over j of w[t][j] W h[t*top + j]."""
         if self.gated:
             raise ValueError("the matrices are gate and up rows: their product is hidden's")
-        ws = self._workspace(places, "lt_dn_experts_sum_ws", self.M, self.K)
+        stream = _stream(self.home)
+        ws = self._workspace(places, stream, "lt_dn_experts_sum_ws", self.M, self.K)
         _lib.call("lt_dn_experts_sum", self.ptr, self.K, h, ldh, y, ldy, self.f32, self.M, self.K, places.ref, w, ls,
-                  None if ws is None else ws.data_ptr(), _stream(self.home))
+                  None if ws is None else ws.data_ptr(), stream)
 
-    def _workspace(self, places, query, *sizes):
+    def _workspace(self, places, stream, query, *sizes):
         if places.n != self.n:
             raise ValueError(f"places of {places.n} experts, the matrices are of {self.n}")
+        if places.stream is not None and places.stream != stream:        # the order's memory is ours to keep until this stream has read it
+            places.buf.record_stream(torch.cuda.current_stream())
         n = 0 if places.buf is None else getattr(_lib.dense(), query)(places.T, places.top, *sizes, self.f32)
         return torch.empty(n, dtype=torch.float32, device="cuda") if n else None
 

@@ -154,6 +154,35 @@ def test_objects_refuse():
         P.DeltaRule(3, 2, 8, 8, torch.float32, 1.0, 1e-6)
 
 
+def test_order_of_the_places_is_kept_for_another_stream(monkeypatch):
+    """Products on another stream than plan's: the order's memory may not go back to plan's stream before they have read it."""
+    now, kept = [7], []
+
+    class Buf:
+        data_ptr = staticmethod(lambda: 256)
+        record_stream = staticmethod(lambda s: kept.append(s))
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: f"stream {now[0]}")
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda d: now[0], raising=False)
+    monkeypatch.setattr(torch.Tensor, "cuda", lambda t: t)
+    monkeypatch.setattr(P, "_here", lambda t, what: t)
+    monkeypatch.setattr(P, "GROUP_FROM", 1)
+    monkeypatch.setattr(torch, "empty", lambda *a, **kw: Buf())
+    calls = []
+    monkeypatch.setattr(_lib, "call", lambda name, *a: calls.append((name, a[-1])))
+    up, down = P.Experts(torch.zeros(4, 8, 8), gated=True), P.Experts(torch.zeros(4, 8, 8), gated=False)
+    places = up.plan(torch.zeros(3, 2, dtype=torch.int32), 3)
+    up.hidden(256, 8, places, 256, 8)
+    down.add_sum(256, 8, places, 256, 256, 8)
+    assert kept == []
+    now[0] = 9
+    up.hidden(256, 8, places, 256, 8)
+    assert kept == ["stream 9"]
+    down.add_sum(256, 8, places, 256, 256, 8)
+    assert kept == ["stream 9"] * 2
+    assert calls == [("lt_dn_experts_plan", 7), ("lt_dn_experts_glu", 7), ("lt_dn_experts_sum", 7), ("lt_dn_experts_glu", 9), ("lt_dn_experts_sum", 9)]
+
+
 @pytest.mark.parametrize("gated", [False, True])
 @pytest.mark.parametrize("K", [1, 9, 12, 63])
 def test_columns_that_are_no_multiple_of_8_are_refused(monkeypatch, K, gated):
