@@ -255,7 +255,8 @@ def delta_chunked_from(ctas):
 
 
 DELTA_CHUNKED_FROM = None       # a number: whatever the sizes
-DELTA_PORTION = 4096            # rows of a sequence that are walked in chunks at a time (a multiple of 64): 32 heads of 128 have 6 MB of workspace a chunk
+DELTA_PORTION = 4096            # rows of a sequence that are walked in chunks at a time, at most (a multiple of 64)
+DELTA_WORKSPACE = 1 << 27       # fp32 elements of workspace that the chunks of all sequences in a walk take together, but for one chunk each
 
 
 class DeltaRule:
@@ -278,6 +279,9 @@ class DeltaRule:
         self.desc = _lib.DnDelta(H, G, dim, vdim, float(q_scale), float(eps), taps, *[None if t is None else _here(t, "a constant").data_ptr()
                                                                                    for t in self.keep])
         self._ref = ctypes.byref(self.desc)
+        one = _lib.DnSeqs(n=1)
+        one.rows[0], one.S[0] = 1, 16            # the size of one chunk's workspace; nothing is read
+        self.chunk = _lib.dense().lt_dn_delta_chunked_ws(self._ref, ctypes.byref(one))
 
     def rows(self, q, k, v, ld, la, beta, ldh, o, ldo, states, rows, ldb=None):
         """Consecutive rows of sequences: rows[i] of them with the state at states[i], from row 0 on.  la and beta have row stride
@@ -301,10 +305,13 @@ class DeltaRule:
             if self.f32 or max(part) < delta_chunked_from(ctas) or self.dim > 256 or self.vdim > 512:
                 _lib.call("lt_dn_delta_rows", *args, self.f32, self._ref, ctypes.byref(seqs), stream)
                 continue
-            starts = seqs.start[:len(part)]
-            for done in range(0, max(part), DELTA_PORTION):
+            starts, done = seqs.start[:len(part)], 0
+            while done < max(part):
+                left = sum(r > done for r in part)
+                portion = min(DELTA_PORTION, 64 * max(1, DELTA_WORKSPACE // max(1, self.chunk * left)))
                 for j, r in enumerate(part):
-                    seqs.start[j], seqs.rows[j] = starts[j] + min(done, r), max(0, min(r - done, DELTA_PORTION))
+                    seqs.start[j], seqs.rows[j] = starts[j] + min(done, r), max(0, min(r - done, portion))
+                done += portion
                 ws = torch.empty(_lib.dense().lt_dn_delta_chunked_ws(self._ref, ctypes.byref(seqs)), dtype=torch.float32, device="cuda")
                 _lib.call("lt_dn_delta_chunked", *args, self._ref, ctypes.byref(seqs), ws.data_ptr(), stream)
 

@@ -122,6 +122,37 @@ def test_delta_refusals():
     step("null pointer", S=None)
 
 
+@pytest.mark.parametrize("lengths,H,d,dv", [
+    ([4096] * 8, 32, 128, 128), ([20000] * 8, 32, 256, 512), ([9000], 64, 256, 512), ([5000, 0, 300, 64, 1], 4, 24, 40), ([70] * 11, 1, 8, 8),
+    ([100000, 100], 16, 128, 128)])
+def test_workspace_of_a_chunked_walk_is_bounded(monkeypatch, lengths, H, d, dv):
+    """Whatever the number of sequences: half a gigabyte, or one chunk of each; and every row is walked once, in order, in whole chunks."""
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda d: 0, raising=False)
+    monkeypatch.setattr(P, "DELTA_CHUNKED_FROM", 1)
+    rule = P.DeltaRule(H, H, d, dv, torch.bfloat16, 1.0, 1e-6)
+    chunk = _lib.dense().lt_dn_delta_chunked_ws(rule._ref, seqs((0, 1, 256)))
+    asked, walked = [], {}
+    monkeypatch.setattr(torch, "empty", lambda n, **kw: asked.append(n) or torch.zeros(4))
+
+    def call(name, *a):
+        assert name == "lt_dn_delta_chunked"
+        q = a[11]._obj
+        assert asked[-1] == _lib.dense().lt_dn_delta_chunked_ws(a[10], a[11]) <= max(1 << 27, chunk * q.n)
+        for j in range(q.n):
+            if q.rows[j]:
+                walked.setdefault(q.S[j], []).append((q.start[j], q.rows[j]))
+    monkeypatch.setattr(_lib, "call", call)
+    rule.rows(256, 256, 256, 3 * H * max(d, dv), 256, 256, H, 256, H * dv, [4096 * (i + 1) for i in range(len(lengths))], lengths)
+    at = 0
+    for i, n in enumerate(lengths):
+        parts = walked.get(4096 * (i + 1), [])
+        for start, rows in parts:
+            assert start == at and (rows % 64 == 0 or (start, rows) == parts[-1])
+            at += rows
+        assert sum(rows for _, rows in parts) == n
+
+
 def test_no_rows_is_no_launch():
     n = _lib.launch_count()
     assert _lib.dense().lt_dn_delta_rows(one, one, one, 96, one, 4, one, 4, one, 96, 0, delta(), seqs((0, 0, 256), (7, 0, 512)), None) == 0
