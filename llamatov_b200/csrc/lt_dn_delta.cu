@@ -314,8 +314,8 @@ __global__ void __launch_bounds__(DeltaScan<T, KPT, LN>::THREADS) k_delta_scan(c
                 const float u1 = fmaf(-k1.x, u0, fmaf(-bg.y, p[1], v1));
                 const float u2 = fmaf(-k2.y, u1, fmaf(-k2.x, u0, fmaf(-bg.z, p[2], v2)));
                 const float u3 = fmaf(-k3.z, u2, fmaf(-k3.y, u1, fmaf(-k3.x, u0, fmaf(-bg.w, p[3], v3))));
-                // above the diagonal the numbers are zero
-                const float y = fmaf(qk.w, u3, fmaf(qk.z, u2, fmaf(qk.y, u1, fmaf(qk.x, u0, gq * r[0]))));
+                // above the diagonal the numbers are zero, and a later token's u, which need not be finite, is taken for zero too
+                const float y = fmaf(qk.w, mine == 3 ? u3 : 0.0f, fmaf(qk.z, mine >= 2 ? u2 : 0.0f, fmaf(qk.y, mine >= 1 ? u1 : 0.0f, fmaf(qk.x, u0, gq * r[0]))));
                 if (col_ok && g < 4 && mine < left) *o = y;
                 const float w0 = z.x * u0, w1 = z.y * u1, w2 = z.z * u2, w3 = z.w * u3;
                 const f2 w[4] = {pack2(w0, w0), pack2(w1, w1), pack2(w2, w2), pack2(w3, w3)}, end2 = pack2(end, end);

@@ -407,6 +407,36 @@ def test_delta_extremes(walk, T):
     assert eo <= _delta_tol(T) and eS <= _delta_tol(T), (eo, eS)
 
 
+@pytest.mark.parametrize("what", ["v", "k", "q", "la", "beta"])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_delta_rows_that_are_not_finite(walk, monkeypatch, what, value):
+    """A number that is not finite reaches its head's outputs from its token on (in chunks: from its chunk on), and nothing else: the
+    rows before, the other heads and the other sequences keep their bits."""
+    f32, H, d, dv, lengths, at = walk, 2, 32, 24, [50, 200, 70], 50 + 135
+    first = 50 + 128 if P.DELTA_CHUNKED_FROM == 1 else at
+    out = []
+    for bad in (False, True):
+        rows, la, beta, S = _delta_case(lengths, H, H, d, dv, f32, seed=7)
+        if bad:
+            if what in ("la", "beta"):
+                (la if what == "la" else beta)[at, 0] = value
+            else:
+                rows[at, {"v": 0, "k": H * dv, "q": H * dv + H * d}[what] + 3] = value
+        o = torch.empty(sum(lengths), H * dv, device="cuda")
+        v, es, ld = rows.data_ptr(), rows.element_size(), rows.shape[1]
+        k = v + H * dv * es
+        P.DeltaRule(H, H, d, dv, DT[f32], 0.25, 1e-6).rows(k + H * d * es, k, v, ld, la.data_ptr(), beta.data_ptr(), H, o.data_ptr(), H * dv,
+                                                         [s.data_ptr() for s in S], lengths)
+        out.append((o, S))
+    (o, S), (p, Z) = out
+    assert torch.equal(p[:first], o[:first]) and torch.equal(p[250:], o[250:]) and torch.equal(p[:, dv:], o[:, dv:])
+    assert torch.equal(Z[0], S[0]) and torch.equal(Z[2], S[2]) and torch.equal(Z[1][1], S[1][1])
+    reached = ~torch.isfinite(p[:, :dv])
+    assert reached[at].any() and (what == "q" or reached[at:250].any(1).all())
+    if what == "q":
+        assert torch.equal(p[at + 1:250], o[at + 1:250]) and torch.equal(Z[1], S[1])
+
+
 @pytest.mark.parametrize("f32", [0, 1])
 @pytest.mark.parametrize("H,G,d,dv,taps", [(1, 1, 8, 8, 1), (4, 2, 16, 24, 4), (6, 3, 40, 72, 3), (2, 2, 128, 128, 4), (3, 1, 264, 16, 5), (2, 1, 512, 40, 2)])
 def test_delta_steps(f32, H, G, d, dv, taps):
