@@ -256,7 +256,10 @@ def delta_chunked_from(ctas):
 
 DELTA_CHUNKED_FROM = None       # a number: whatever the sizes
 DELTA_PORTION = 4096            # rows of a sequence that are walked in chunks at a time, at most (a multiple of 64)
-DELTA_WORKSPACE = 1 << 27       # fp32 elements of workspace that the chunks of all sequences in a walk take together, but for one chunk each
+# fp32 elements of workspace that the chunks of all sequences in a walk take together, or one chunk of each: 1 GB.  (us with 512 MB / 1 GB / 2 GB /
+# all at once: eight sequences of 4096 rows, 32 heads of 128 3417 / 3281 / 3213 / 3168; of 2048 rows, 16 heads 878 / 840 / 841 / 840; one of 4096
+# rows, 16 heads of 256 x 512 1383 / 1308 / 1236 / 1236.)
+DELTA_WORKSPACE = 1 << 28
 
 
 class DeltaRule:

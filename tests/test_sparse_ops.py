@@ -126,7 +126,7 @@ def test_delta_refusals():
     ([4096] * 8, 32, 128, 128), ([20000] * 8, 32, 256, 512), ([9000], 64, 256, 512), ([5000, 0, 300, 64, 1], 4, 24, 40), ([70] * 11, 1, 8, 8),
     ([100000, 100], 16, 128, 128)])
 def test_workspace_of_a_chunked_walk_is_bounded(monkeypatch, lengths, H, d, dv):
-    """Whatever the number of sequences: half a gigabyte, or one chunk of each; and every row is walked once, in order, in whole chunks."""
+    """Whatever the number of sequences: a gigabyte, or one chunk of each; and every row is walked once, in order, in whole chunks."""
     monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
     monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda d: 0, raising=False)
     monkeypatch.setattr(P, "DELTA_CHUNKED_FROM", 1)
@@ -138,7 +138,7 @@ def test_workspace_of_a_chunked_walk_is_bounded(monkeypatch, lengths, H, d, dv):
     def call(name, *a):
         assert name == "lt_dn_delta_chunked"
         q = a[11]._obj
-        assert asked[-1] == _lib.dense().lt_dn_delta_chunked_ws(a[10], a[11]) <= max(1 << 27, chunk * q.n)
+        assert asked[-1] == _lib.dense().lt_dn_delta_chunked_ws(a[10], a[11]) <= max(1 << 28, chunk * q.n)
         for j in range(q.n):
             if q.rows[j]:
                 walked.setdefault(q.S[j], []).append((q.start[j], q.rows[j]))
