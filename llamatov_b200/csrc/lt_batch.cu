@@ -756,12 +756,11 @@ extern "C" int lt_attn_decode_batch(const float* Q, int q_ld, const float* K, co
     const size_t sc_bytes = ((size_t)rep * hd + (size_t)SC_PT * hd) * sizeof(float);
     LT_REQUIRE(sc_bytes <= 200 * 1024, "lt_attn_decode_batch: hd=%d needs %zu bytes of shared memory for a K tile", hd, sc_bytes);
     static PerDeviceOnce attr_once;
-    if (attr_once.first()) {
-        LT_CUDA(cudaFuncSetAttribute(k_attn_scores, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
-        LT_CUDA(cudaFuncSetAttribute(k_attn_softmax, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
-        LT_CUDA(cudaFuncSetAttribute(k_attn_pv<4, 128>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pv_smem(4, 128)));
-        LT_CUDA(cudaFuncSetAttribute(k_attn_pv<2, 64>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pv_smem(2, 64)));
-    }
+    LT_ONCE(attr_once,
+            LT_CUDA(cudaFuncSetAttribute(k_attn_scores, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+            LT_CUDA(cudaFuncSetAttribute(k_attn_softmax, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+            LT_CUDA(cudaFuncSetAttribute(k_attn_pv<4, 128>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pv_smem(4, 128)));
+            LT_CUDA(cudaFuncSetAttribute(k_attn_pv<2, 64>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pv_smem(2, 64))));
     cudaError_t e = launch_chained(k_attn_scores, dim3((max_seq + SC_PT - 1) / SC_PT, nkv, B), dim3(BT), sc_bytes, s, Q,
                                    q_ld, K, lens, S, s_ld, hd, nh, nkv, scale, max_seq, st);
     if (e == cudaSuccess)
@@ -820,9 +819,7 @@ static int attn_split_launch(const char* what, const float* Q, int q_ld, const f
     const int kstage = smem + kbytes <= 227 * 1024 ? 1 : 0;
     if (kstage) smem += kbytes;
     static PerDeviceOnce attr_once;
-    if (attr_once.first()) {
-        LT_CUDA(cudaFuncSetAttribute(k_attn_split, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
-    }
+    LT_ONCE(attr_once, LT_CUDA(cudaFuncSetAttribute(k_attn_split, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024)));
     int threads = ((rep * hd + 31) / 32) * 32;
     if (threads < 256) threads = 256;
     if (threads > 1024) threads = 1024;

@@ -6,6 +6,7 @@
 #include <stdio.h>
 
 #include "../../include/llamatov_b200.h"
+#include "lt_once.cuh"
 
 namespace lt {
 
@@ -74,21 +75,6 @@ inline cudaError_t launch_chained(void (*kern)(P...), dim3 grid, dim3 block, siz
             return LT_ERR_CUDA;                                              \
         }                                                                    \
     } while (0)
-
-// Per-device "done once" flags.  cudaFuncSetAttribute and occupancy are per-device properties, so a
-// launcher that caches either must key the cache by the current device (a process may drive several
-// GPUs).  first() returns true exactly once per device (racing threads may both see true: the guarded
-// calls are idempotent).
-struct PerDeviceOnce {
-    bool done[64] = {};
-    bool first() {
-        int dev = 0;
-        if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return true;
-        if (done[dev]) return false;
-        done[dev] = true;
-        return true;
-    }
-};
 
 inline int sm_count() {
     static int cache[64] = {0};

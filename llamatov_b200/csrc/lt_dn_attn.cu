@@ -238,8 +238,7 @@ static int launch_window(const WinP& P, int H, cudaStream_t s) {
     const size_t smem = (size_t)((WQ + 2 * WK) * (DK + 8) + 2 * WK * (DV + 8)) * 2;
     LT_REQUIRE(smem <= 220 * 1024, "attention of a portion: key size %d needs %zu bytes of shared memory", P.dp + P.rtp, smem);
     static PerDeviceOnce once;
-    if (once.first())
-        LT_CUDA(cudaFuncSetAttribute(k_window_attn<DV, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024));
+    LT_ONCE(once, LT_CUDA(cudaFuncSetAttribute(k_window_attn<DV, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024)));
     k_window_attn<DV, CAP><<<dim3((P.T + WQ - 1) / WQ, H, (P.dvp + DV - 1) / DV), 128, smem, s>>>(P);
     return check_launch("attention of a portion");
 }

@@ -413,10 +413,9 @@ static int launch_chunked(const ChunkP& P, cudaStream_t s) {
     const size_t sm2 = (size_t)CH * (2 * qs + P.dvp + 8 + 2 * (CH + 8)) * 2 + (LOG ? (size_t)(CH + 4) * bs * 4 : (CH + 4) * 4);
     LT_REQUIRE(sm1 <= 220 * 1024 && sm2 <= 220 * 1024, "lt_dn_recurrence_chunked: head sizes %d, %d need too much shared memory", P.dp, P.dvp);
     static PerDeviceOnce once;
-    if (once.first()) {
-        LT_CUDA(cudaFuncSetAttribute(k_chunk_state<LOG>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024));
-        LT_CUDA(cudaFuncSetAttribute(k_chunk_out<LOG>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024));
-    }
+    LT_ONCE(once,
+            LT_CUDA(cudaFuncSetAttribute(k_chunk_state<LOG>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024));
+            LT_CUDA(cudaFuncSetAttribute(k_chunk_out<LOG>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024)));
     k_chunk_state<LOG><<<dim3(P.nchunk, P.H), 256, sm1, s>>>(P);
     int rc = check_launch("lt_dn_recurrence_chunked (state)");
     if (rc != LT_OK) return rc;

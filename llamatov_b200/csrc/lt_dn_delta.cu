@@ -357,7 +357,7 @@ template <typename T, int KPT, int LN>
 static int launch_delta_scan(const DeltaScanP& P, cudaStream_t s) {
     using L = DeltaScan<T, KPT, LN>;
     static PerDeviceOnce once;
-    if (once.first()) LT_CUDA(cudaFuncSetAttribute(k_delta_scan<T, KPT, LN>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM));
+    LT_ONCE(once, LT_CUDA(cudaFuncSetAttribute(k_delta_scan<T, KPT, LN>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM)));
     k_delta_scan<T, KPT, LN><<<dim3((P.D.dvp + SCAN_COLS - 1) / SCAN_COLS, P.D.H, P.Q.n), L::THREADS, L::SMEM, s>>>(P);
     return check_launch("lt_dn_delta_rows");
 }

@@ -716,7 +716,7 @@ __global__ void __launch_bounds__(NW * 32, DeltaOut<NK, NW>::CTAS) k_delta_out(c
 template <int NK, int NW>
 static int launch_delta_out(const DeltaChunkP& P, int chunks, cudaStream_t s) {
     static PerDeviceOnce once;
-    if (once.first()) LT_CUDA(cudaFuncSetAttribute(k_delta_out<NK, NW>, cudaFuncAttributeMaxDynamicSharedMemorySize, DeltaOut<NK, NW>::SMEM));
+    LT_ONCE(once, LT_CUDA(cudaFuncSetAttribute(k_delta_out<NK, NW>, cudaFuncAttributeMaxDynamicSharedMemorySize, DeltaOut<NK, NW>::SMEM)));
     k_delta_out<NK, NW><<<dim3(chunks, P.D.H), NW * 32, DeltaOut<NK, NW>::SMEM, s>>>(P);
     return check_launch("lt_dn_delta_chunked (outputs)");
 }
@@ -773,7 +773,7 @@ extern "C" int lt_dn_delta_chunked(const void* q, const void* k, const void* v, 
     cudaStream_t s = (cudaStream_t)stream;
     const int dp = P.D.dp;
     static PerDeviceOnce once;
-    if (once.first()) LT_CUDA(cudaFuncSetAttribute(k_delta_prep, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)prep_smem(256, 32)));
+    LT_ONCE(once, LT_CUDA(cudaFuncSetAttribute(k_delta_prep, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)prep_smem(256, 32))));
     k_delta_prep<<<dim3(chunks, P.D.H), PREP_THREADS, prep_smem(dp, P.nvt), s>>>(P);
     int rc = check_launch("lt_dn_delta_chunked (prepare)");
     if (rc != LT_OK) return rc;

@@ -369,7 +369,7 @@ static int launch_group_tc(GroupP P, void* rows, cudaStream_t s) {
     rc = group_map(&tmX, rows, places, P.K, P.K, XBOX);
     if (rc != LT_OK) return rc;
     static PerDeviceOnce once;
-    if (once.first()) LT_CUDA(cudaFuncSetAttribute(k_group_tc<NT, GLU>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    LT_ONCE(once, LT_CUDA(cudaFuncSetAttribute(k_group_tc<NT, GLU>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM)));
     k_gather<<<(unsigned)((places + 7) / 8), 256, 0, s>>>(P, (uint4*)rows);
     rc = check_launch("experts' products (rows in order)");
     if (rc != LT_OK) return rc;
@@ -628,7 +628,7 @@ template <bool GLU, int MQ>
 static int launch_group_f32(const GroupP& P, cudaStream_t s) {
     constexpr int BN = 8 * MQ, SMEM = GF_STAGES * ((GLU ? 2 : 1) * GF_BM + BN) * GF_ST * 4;
     static PerDeviceOnce once;
-    if (once.first()) LT_CUDA(cudaFuncSetAttribute(k_group_f32<GLU, MQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+    LT_ONCE(once, LT_CUDA(cudaFuncSetAttribute(k_group_f32<GLU, MQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM)));
     long tiles;
     const int rc = f32_tiles(P, BN, &tiles);
     if (rc != LT_OK) return rc;

@@ -271,8 +271,7 @@ static int launch_tc(const void* W, int ldw, const void* X, int ldx, GemmP P, cu
     rc = make_map_bf16(&tmX, X, P.T, P.K, ldx, NT);
     if (rc != LT_OK) return rc;
     static PerDeviceOnce once;
-    if (once.first())
-        LT_CUDA(cudaFuncSetAttribute(k_gemm_tc<NT, MA>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    LT_ONCE(once, LT_CUDA(cudaFuncSetAttribute(k_gemm_tc<NT, MA>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM)));
     P.row_tiles = (P.M + 127) / 128;
     P.t_tiles = (P.T + NT - 1) / NT;
     P.up_row = P.M;
@@ -478,7 +477,7 @@ template <bool GLU, int MQ, bool SHARED>
 static int launch_f32(const void* W, int ldw, const void* X, int ldx, const GemmP& P, cudaStream_t s) {
     using C = F32Cfg<GLU, MQ, SHARED>;
     static PerDeviceOnce once;
-    if (once.first()) LT_CUDA(cudaFuncSetAttribute(k_gemm_f32<GLU, MQ, SHARED>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    LT_ONCE(once, LT_CUDA(cudaFuncSetAttribute(k_gemm_f32<GLU, MQ, SHARED>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM)));
     const long gx = (P.M + F32_BM - 1) / F32_BM, gy = (P.T + C::BN - 1) / C::BN;
     LT_REQUIRE(gy <= 65535, "lt_dn_linear: T=%d too large", P.T);
     const int parts = f32_parts(P.K), S = SHARED ? parts : 1;

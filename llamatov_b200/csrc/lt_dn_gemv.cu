@@ -297,12 +297,11 @@ extern "C" int lt_dn_gemv(const void* W, int ldw, void* Y, int f32, int M, int K
     P.nstore = (P.mstore + 1) / 2;
     P.npair = P.nstore + M - P.mstore;
     static PerDeviceOnce once;
-    if (once.first()) {
-        LT_CUDA(cudaFuncSetAttribute(k_gemv<bf16, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
-        LT_CUDA(cudaFuncSetAttribute(k_gemv<bf16, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
-        LT_CUDA(cudaFuncSetAttribute(k_gemv<float, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
-        LT_CUDA(cudaFuncSetAttribute(k_gemv<float, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
-    }
+    LT_ONCE(once,
+            LT_CUDA(cudaFuncSetAttribute(k_gemv<bf16, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+            LT_CUDA(cudaFuncSetAttribute(k_gemv<bf16, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+            LT_CUDA(cudaFuncSetAttribute(k_gemv<float, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+            LT_CUDA(cudaFuncSetAttribute(k_gemv<float, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024)));
     const int per = smem <= 100 * 1024 ? 2 : 1;
     // warps per pair: as many as the resident CTAs have for every pair, each with at least one whole batch.  A bf16 batch is
     // twice the products of an fp32 one for the same bytes, and the chain through the warps then costs what is gained

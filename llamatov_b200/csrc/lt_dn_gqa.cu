@@ -459,10 +459,9 @@ __global__ void __launch_bounds__(GT) k_gqa_step(const __grid_constant__ GqaStep
 template <typename T>
 static int launch_step(const GqaStepP& P, size_t smem, cudaStream_t s) {
     static PerDeviceOnce once;
-    if (once.first()) {
-        LT_CUDA(cudaFuncSetAttribute(k_gqa_step<T, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024));
-        LT_CUDA(cudaFuncSetAttribute(k_gqa_step<T, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024));
-    }
+    LT_ONCE(once,
+            LT_CUDA(cudaFuncSetAttribute(k_gqa_step<T, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024));
+            LT_CUDA(cudaFuncSetAttribute(k_gqa_step<T, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024)));
     const dim3 grid(P.splits, P.A.G * P.nb);
     if (P.A.dvp <= 2 * GT) k_gqa_step<T, 1><<<grid, GT, smem, s>>>(P);
     else k_gqa_step<T, 2><<<grid, GT, smem, s>>>(P);

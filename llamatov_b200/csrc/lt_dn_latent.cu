@@ -364,11 +364,10 @@ static int launch_step(const StepP& P, cudaStream_t s) {
     LT_REQUIRE(smem <= 220 * 1024, "lt_dn_latent_step: a cache row of %d elements needs %zu bytes of shared memory", wr, smem);
     const dim3 grid(P.splits, (L.H + SH - 1) / SH);
     static PerDeviceOnce once;
-    if (once.first()) {
-        LT_CUDA(cudaFuncSetAttribute(k_latent_scan<T, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024));
-        LT_CUDA(cudaFuncSetAttribute(k_latent_scan<T, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024));
-        LT_CUDA(cudaFuncSetAttribute(k_latent_scan<T, 4>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024));
-    }
+    LT_ONCE(once,
+            LT_CUDA(cudaFuncSetAttribute(k_latent_scan<T, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024));
+            LT_CUDA(cudaFuncSetAttribute(k_latent_scan<T, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024));
+            LT_CUDA(cudaFuncSetAttribute(k_latent_scan<T, 4>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024)));
     if (L.rp <= 256) k_latent_scan<T, 1><<<grid, 128, smem, s>>>(P);
     else if (L.rp <= 512) k_latent_scan<T, 2><<<grid, 128, smem, s>>>(P);
     else k_latent_scan<T, 4><<<grid, 128, smem, s>>>(P);

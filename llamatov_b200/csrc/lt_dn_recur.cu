@@ -107,8 +107,7 @@ template <typename T, int KPT, int MODE>
 static int launch_scan(const RecurP& P, cudaStream_t s) {
     const size_t smem = ((size_t)RT * 8 * KPT * (MODE == DEC_CONST || MODE == DEC_HEAD ? 2 : 3) + (size_t)RT * 33) * 4;
     static PerDeviceOnce once;
-    if (once.first())
-        LT_CUDA(cudaFuncSetAttribute(k_recur_scan<T, KPT, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+    LT_ONCE(once, LT_CUDA(cudaFuncSetAttribute(k_recur_scan<T, KPT, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024)));
     k_recur_scan<T, KPT, MODE><<<dim3((P.dvp + 31) / 32, P.H), 256, smem, s>>>(P);
     return check_launch("lt_dn_recurrence");
 }

@@ -318,8 +318,7 @@ __global__ void __launch_bounds__(128, SsdOut<NK>::CTAS) k_ssd_out(const __grid_
 template <int NK>
 static int launch_out(SsdChunkP P, cudaStream_t s) {
     static PerDeviceOnce once;
-    if (once.first())
-        LT_CUDA(cudaFuncSetAttribute(k_ssd_out<NK>, cudaFuncAttributeMaxDynamicSharedMemorySize, SsdOut<NK>::SMEM));
+    LT_ONCE(once, LT_CUDA(cudaFuncSetAttribute(k_ssd_out<NK>, cudaFuncAttributeMaxDynamicSharedMemorySize, SsdOut<NK>::SMEM)));
     // heads of a CTA: q . k is computed once for them, but the GPU should be filled in whole waves
     float best = 0.0f;
     for (int n = 1; n <= 8 && n <= P.per; n++) {
@@ -339,10 +338,9 @@ static int launch_out(SsdChunkP P, cudaStream_t s) {
 int launch_ssd_chunked(const SsdChunkP& P, cudaStream_t s) {
     const int nv = (P.dvp + VT - 1) / VT;
     static PerDeviceOnce once;
-    if (once.first()) {
-        LT_CUDA(cudaFuncSetAttribute(k_ssd_states<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, SsdStates<64>::SMEM));
-        LT_CUDA(cudaFuncSetAttribute(k_ssd_states<32>, cudaFuncAttributeMaxDynamicSharedMemorySize, SsdStates<32>::SMEM));
-    }
+    LT_ONCE(once,
+            LT_CUDA(cudaFuncSetAttribute(k_ssd_states<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, SsdStates<64>::SMEM));
+            LT_CUDA(cudaFuncSetAttribute(k_ssd_states<32>, cudaFuncAttributeMaxDynamicSharedMemorySize, SsdStates<32>::SMEM)));
     if ((long)P.H * nv * ((P.dp + 63) / 64) >= 100)
         k_ssd_states<64><<<dim3((P.dp + 63) / 64, nv, P.H), 256, SsdStates<64>::SMEM, s>>>(P);
     else

@@ -824,10 +824,9 @@ int run(const Args& a, cudaStream_t s) {
     const int rc = res ? fill(P, tmW, tmX, a, 32, 128) : fill(P, tmW, tmX, a, 64, 64);
     if (rc != LT_OK) return rc;
     static PerDeviceOnce attr_once;
-    if (attr_once.first()) {
-        LT_CUDA(cudaFuncSetAttribute(k_q8_gemm_res, cudaFuncAttributeMaxDynamicSharedMemorySize, ResSmem(RES_MAX_K / 32).total + 1024));
-        LT_CUDA(cudaFuncSetAttribute(k_q8_gemm_pair, cudaFuncAttributeMaxDynamicSharedMemorySize, PairSmem::TOTAL + 1024));
-    }
+    LT_ONCE(attr_once,
+            LT_CUDA(cudaFuncSetAttribute(k_q8_gemm_res, cudaFuncAttributeMaxDynamicSharedMemorySize, ResSmem(RES_MAX_K / 32).total + 1024));
+            LT_CUDA(cudaFuncSetAttribute(k_q8_gemm_pair, cudaFuncAttributeMaxDynamicSharedMemorySize, PairSmem::TOTAL + 1024)));
     const int sms = sm_count(), grid = P.units < sms ? P.units : sms;
     if (res) k_q8_gemm_res<<<grid, RES_THREADS, ResSmem(a.K / 32).total + 1024, s>>>(tmW, tmX, P);
     else k_q8_gemm_pair<<<grid, P_THREADS, PairSmem::TOTAL + 1024, s>>>(tmW, tmX, P);

@@ -604,9 +604,7 @@ static int launch(const int8_t* Wq, const uint16_t* Wd, const int8_t* Xq, const 
     const size_t smem = smem_bytes<NT, CB, EW, S, NST>(nb);
     LT_REQUIRE(smem <= MAX_SMEM, "lt_q8_gemm_tc: K=%d needs %zu bytes of shared memory per CTA", K, smem);
     static PerDeviceOnce attr_once;
-    if (attr_once.first()) {
-        LT_CUDA(cudaFuncSetAttribute(k_q8_gemm_tc<NT, CB, EW, S, NST>, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_SMEM));
-    }
+    LT_ONCE(attr_once, LT_CUDA(cudaFuncSetAttribute(k_q8_gemm_tc<NT, CB, EW, S, NST>, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_SMEM)));
     Params P;
     P.Wd = (const __half*)Wd; P.Xd = (const __half*)Xd; P.Resid = Resid; P.Y = Y;
     P.status = device_status_ptr();

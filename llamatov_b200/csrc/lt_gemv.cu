@@ -410,8 +410,8 @@ static int launch_gemv(const int8_t* Wq, const uint16_t* Wd, const int8_t* Xq, c
     const int col_stride = ((K + nb * 2 + 15) / 16) * 16;
     const size_t smem = (size_t)col_stride * TB;
     static PerDeviceOnce attr_once;
-    if (smem > 48 * 1024 && attr_once.first()) {
-        LT_CUDA(cudaFuncSetAttribute(k_q8_gemv<R, TB>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+    if (smem > 48 * 1024) {
+        LT_ONCE(attr_once, LT_CUDA(cudaFuncSetAttribute(k_q8_gemv<R, TB>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024)));
     }
     LT_REQUIRE(smem <= 200 * 1024, "lt_q8_gemv: K=%d needs %zu bytes of shared memory per CTA (limit 204800)", K, smem);
     int ctas = gemv_grid(((long)M + R - 1) / R);
@@ -427,8 +427,8 @@ static int launch_gemv1(const int8_t* Wq, const uint16_t* Wd, const void* Xq, co
     const int nb = K / 32;
     const size_t smem = (size_t)((K + nb * 2 + 15) / 16) * 16 + (PRO ? (size_t)(272 + 2 * K) * 4 : 0);
     static PerDeviceOnce attr_once;
-    if (smem > 48 * 1024 && attr_once.first()) {
-        LT_CUDA(cudaFuncSetAttribute(k_q8_gemv1<R, U, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+    if (smem > 48 * 1024) {
+        LT_ONCE(attr_once, LT_CUDA(cudaFuncSetAttribute(k_q8_gemv1<R, U, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024)));
     }
     LT_REQUIRE(smem <= 200 * 1024, "lt_q8_gemv: K=%d needs %zu bytes of shared memory per CTA (limit 204800)", K, smem);
     // one wave: as many CTAs as are resident at once (by this instantiation's registers and shared memory)

@@ -547,9 +547,7 @@ static int launch_attn_prefill_wide(const float* Q, int q_ld, const AttnSeqs& S,
     LT_REQUIRE(st != nullptr, "lt_attn_prefill: status word unavailable");
     const size_t smem = attn_prefill_wide_smem<HD>(maxt);
     static PerDeviceOnce attr_once;
-    if (attr_once.first()) {
-        LT_CUDA(cudaFuncSetAttribute(k_attn_prefill_wide<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
-    }
+    LT_ONCE(attr_once, LT_CUDA(cudaFuncSetAttribute(k_attn_prefill_wide<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024)));
     dim3 grid((nrows + PW_QT - 1) / PW_QT, nh, nseq);
     k_attn_prefill_wide<HD><<<grid, PW_THREADS, smem, s>>>(Q, q_ld, S, OUT, out_ld, nh, nkv, scale, nrows, maxt, st);
     return check_launch("lt_attn_prefill");
@@ -978,9 +976,7 @@ static int launch_attn_prefill_block(const float* Q, int q_ld, const AttnSeqs& S
     LT_REQUIRE(st != nullptr, "lt_attn_prefill: status word unavailable");
     constexpr int smem = PrefillBlock<HD, QT>::SMEM;
     static PerDeviceOnce attr_once;
-    if (attr_once.first()) {
-        LT_CUDA(cudaFuncSetAttribute(k_attn_prefill_block<HD, QT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    }
+    LT_ONCE(attr_once, LT_CUDA(cudaFuncSetAttribute(k_attn_prefill_block<HD, QT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)));
     k_attn_prefill_block<HD, QT><<<(nrows + QT - 1) / QT * nh * nseq, PrefillBlock<HD, QT>::THREADS, smem, s>>>(
         Q, q_ld, S, nseq, OUT, out_ld, nh, nkv, scale, nrows, maxt, st);
     return check_launch("lt_attn_prefill");
@@ -995,9 +991,7 @@ static int launch_attn_prefill(const float* Q, int q_ld, const float* K, const f
                          (size_t)QT * ((maxt + 3) & ~3)) * sizeof(float);
     LT_REQUIRE(smem <= 200 * 1024, "lt_attn_prefill: maxt=%d needs %zu bytes of shared memory", maxt, smem);
     static PerDeviceOnce attr_once;
-    if (attr_once.first()) {
-        LT_CUDA(cudaFuncSetAttribute(k_attn_prefill<HD, QT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
-    }
+    LT_ONCE(attr_once, LT_CUDA(cudaFuncSetAttribute(k_attn_prefill<HD, QT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024)));
     dim3 grid((nrows + QT - 1) / QT, nh);
     k_attn_prefill<HD, QT><<<grid, PF_THREADS, smem, s>>>(Q, q_ld, K, V, len, OUT, out_ld, nh, nkv, scale, nrows, maxt,
                                                          st);
