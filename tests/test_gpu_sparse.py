@@ -111,6 +111,54 @@ def test_captured_step_equals_eager_step(name, dtype):
     assert S.live["a"].runner.captured
 
 
+@pytest.mark.parametrize("form", ["few", "group"])
+@pytest.mark.parametrize("name", sorted(DESIGNS))
+def test_bf16_models_that_choose(name, form, monkeypatch):
+    """A prompt and tokens of bf16 models with 2 of 8 and 3 of 16 experts.  A choice may hang on a rounding of the scores, so the oracle is
+    given the experts that the model chose; their weights are its own."""
+    from llamatov_b200 import mixers
+    from oracle import layered as L, pakalix as O, sparse
+    monkeypatch.setattr(dense_ops, "GROUP_FROM", 1 if form == "group" else 10 ** 9)
+    D = DESIGNS[name]
+    cfg = X.config(D)
+    t = X.random_tensors(D, cfg, 17)
+    c, w = U.product(cfg, t, "bfloat16")
+    chosen = []
+    plan, step = dense_ops.Experts.plan, mixers.ExpertsFeedForward.step
+
+    def seen_plan(self, ids, T):
+        chosen.append(ids.clone())
+        return plan(self, ids, T)
+
+    def seen_step(self, pk, *a):
+        step(self, pk, *a)
+        chosen.append(pk.step.ids[:self.top].clone()[None])
+    monkeypatch.setattr(dense_ops.Experts, "plan", seen_plan)
+    monkeypatch.setattr(mixers.ExpertsFeedForward, "step", seen_step)
+    route, own = sparse.route, []
+
+    def given(l, m, bias):
+        ids = next(fed)
+        own.append(set(ids) == set(route(l, m, bias)[0]))
+        s = sparse._sigmoid(l) if m.get("score") == "sigmoid" else np.exp(l - l.max()) / np.exp(l - l.max()).sum()
+        return ids, s[ids] / s[ids].sum() * m.get("scale", 1.0)
+    monkeypatch.setattr(sparse, "route", given)
+    A = archs.of(c)
+    A.ensure_buffers(w, c)
+    toks, kv = _tokens(cfg, 100, 5), [None] * A.n_slots(c)
+    m = (L if D is U else O).Model(cfg, U.as_numpy(t))
+    for n, part in [(90, toks[:90])] + [(1, [x]) for x in toks[90:]]:
+        chosen.clear()
+        if n > 1:
+            got = pf.prefill_resident(w, c, torch.tensor(part), kv, want_rows=list(range(n))).numpy().reshape(n, -1)
+        else:
+            got = dr.forward_pass_resident(w, c, torch.tensor(part), torch.tensor([m.pos]), kv).reshape(1, -1).numpy()
+        fed = iter([row for ids in chosen for row in ids.tolist()])
+        assert U.rel_rms(got, m.run(part)) < TOL["bfloat16"], n
+        assert next(fed, None) is None
+    assert np.mean(own) > 0.8                    # nearly all of them are the oracle's own
+
+
 @pytest.mark.parametrize("name", sorted(DESIGNS))
 def test_sequences_in_one_prompt_pass(name):
     """More sequences than one launch of the delta rule takes, continued, then emptied and used again."""

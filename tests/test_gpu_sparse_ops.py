@@ -97,6 +97,20 @@ def test_route(score, T, n, top, groups, top_groups, biased):
 
 
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("T,n,top,groups,top_groups", [(37, 1020, 10, 17, 5), (5, 1023, 32, 31, 31), (130, 1007, 7, 19, 1)])
+def test_route_many_experts_a_lane(score, T, n, top, groups, top_groups):
+    """Groups that are no power of two and have more than 32 experts, all of one lane; equal scores among them."""
+    l = _randn((T, n), T, scale=2.0)
+    l[::3] = torch.round(l[::3])
+    l[1, :n // 2] = -float("inf")
+    bias = _randn((n,), 6, scale=0.25).mul(8).round().div(8)
+    ids, w = _route(l, n, top, bias=bias, score=score, groups=groups, top_groups=top_groups)
+    want, ww = route64(_np(l), top, score, _np(bias), groups, top_groups, True, 1.0)
+    assert np.array_equal(ids, want)
+    assert np.allclose(w, ww, rtol=2 * E32, atol=1e-38)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 def test_route_ties_and_masks(score):
     n, inf = 16, float("inf")
     rows = [[0.0] * n, [1.0, 2.0] * 8, [-inf] * n, [-inf] * 15 + [3.0], [float("nan")] * 8 + [0.5] * 8, [5.0] + [-inf] * 14 + [float("nan")],
@@ -368,6 +382,21 @@ def test_delta_rows(walk, lengths, H, G, d, dv):
         assert eo <= _delta_tol(max(lengths)) and eS <= _delta_tol(max(lengths)), (eo, eS)
 
 
+@pytest.mark.parametrize("lengths,H,G,d,dv", [
+    ([130, 65], 2, 1, 256, 256), ([70], 1, 1, 192, 128), ([70, 64], 2, 1, 256, 512), ([129], 3, 3, 136, 72), ([200], 1, 1, 248, 504), ([65], 2, 2, 128, 512),
+    ([140], 1, 1, 64, 200)])
+def test_delta_chunks_of_large_heads(lengths, H, G, d, dv, monkeypatch):
+    """Every variant of the chunked walk and of its outputs, full and with ragged tiles, and that it is the one that runs."""
+    names, call = [], _lib.call
+    monkeypatch.setattr(P, "DELTA_CHUNKED_FROM", 1)
+    monkeypatch.setattr(_lib, "call", lambda name, *a: (names.append(name), call(name, *a)))
+    for strong in (False, True):
+        rows, la, beta, S = _delta_case(lengths, H, G, d, dv, 0, seed=d, strong=strong)
+        eo, eS = _delta_run(rows, la, beta, S, lengths, H, G, d, dv, 0)
+        assert eo <= _delta_tol(max(lengths)) and eS <= _delta_tol(max(lengths)), (eo, eS)
+    assert names == ["lt_dn_delta_chunked"] * 2
+
+
 @pytest.mark.parametrize("chunks,f32", [(0, 0), (0, 1), (1, 0)])
 def test_delta_rows_between_other_rows(chunks, f32):
     lengths, H, G, d, dv = [5, 0, 70], 4, 2, 24, 40
@@ -619,6 +648,63 @@ def test_many_places(f32):
             want[s] += w[s, j, None] * torch.einsum("tmk,tk->tm", D[e[s]].double(), hj)
             size[s] += w[s, j, None] * torch.einsum("tmk,tk->tm", D[e[s]].double().abs(), hj.abs())
     assert ((y - want).abs() <= (8 * M ** 0.5 + top + 2) * E32 * size).all()
+
+
+@pytest.mark.parametrize("each", [15, 48, 200])
+def test_grouped_products_in_several_rounds(each):
+    """Three and more tiles a CTA, eleven blocks of k each (the last ragged), for 64, 128 and 256 places a tile: places of the ring and
+    sets of accumulators are used again from one tile to the next.  Shares of the experts are unequal, some have none."""
+    n, top, M, K = 34, 2, 4144, 648
+    T = each * n // top
+    g = torch.Generator().manual_seed(each)
+    share = torch.rand(n - 2, generator=g) + 0.2
+    ids = torch.multinomial(share, T * top, replacement=True, generator=g).reshape(T, top).int().cuda()
+    W, X = _randn((n, M, K), 1, torch.bfloat16, 1.5 * K ** -0.5), _randn((T, K), 2, torch.bfloat16)
+    H, w, Y0 = _randn((T * top, K), 3, torch.bfloat16), torch.rand(T, top, generator=g).cuda(), _randn((T, M), 4)
+    gu, down, F = P.Experts(W, gated=True), P.Experts(W, gated=False), M // 2
+    out = []
+    for _ in range(2):
+        places = gu.plan(ids, T)
+        h, y = torch.full((T * top, F), 7.0, dtype=torch.bfloat16, device="cuda"), Y0.clone()
+        gu.hidden(X.data_ptr(), K, places, h.data_ptr(), F)
+        down.add_sum(H.data_ptr(), K, places, w.data_ptr(), y.data_ptr(), M)
+        out.append((h, y))
+    assert torch.equal(out[0][0], out[1][0]) and torch.equal(out[0][1], out[1][1])
+    want, size = Y0.double(), Y0.double().abs()
+    for e in range(n):
+        at = (ids.reshape(-1) == e).nonzero()[:, 0]
+        t, We = at // top, W[e].double()
+        v = X[t].double() @ We.T
+        a, b = v[:, :F], v[:, F:]
+        glu = 0.5 * a * (1 + torch.tanh((2 / np.pi) ** 0.5 * (a + 0.044715 * a ** 3))) * b
+        # of _check_glu; the tensor cores cut off at most 2^-23 of a sum at each of K / 16 steps, which 8 sqrt(K) 2^-24 covers up to K = 4096
+        tol = (8 * K ** 0.5 + 16) * E32 * (1 + a.abs()) * (1 + b.abs()) * 3 + 2.0 ** -8 * glu.abs()
+        assert ((h[at].double() - glu).abs() <= tol).all(), e
+        a = w.reshape(-1)[at, None].double()
+        want.index_add_(0, t, a * (H[at].double() @ We.T))
+        size.index_add_(0, t, a * (H[at].double().abs() @ We.abs().T))
+    assert ((y.double() - want).abs() <= (8 * K ** 0.5 + top + 2) * E32 * size).all()
+
+
+def test_order_of_the_places_read_on_another_stream():
+    """The products of a plan run on another stream, behind a delay, after the plan's object is gone and its stream allocates again."""
+    T, top, n, K, F = 3000, 4, 16, 64, 40
+    ids, X = _ids(T, top, n, 1).cuda(), _randn((T, K), 2, torch.bfloat16)
+    gu = P.Experts(_randn((n, 2 * F, K), 3, torch.bfloat16, K ** -0.5), gated=True)
+    h = torch.zeros(2, T * top, F, dtype=torch.bfloat16, device="cuda")
+    gu.hidden(X.data_ptr(), K, gu.plan(ids, T), h[0].data_ptr(), F)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    places = gu.plan(ids, T)
+    size = places.buf.numel()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)            # about 10 ms
+        gu.hidden(X.data_ptr(), K, places, h[1].data_ptr(), F)
+    del places
+    junk = [torch.zeros(size, dtype=torch.int32, device="cuda") for _ in range(8)]
+    torch.cuda.synchronize()
+    assert torch.equal(h[0], h[1]) and len(junk) == 8
 
 
 def test_matrices_past_32_bits(form):
