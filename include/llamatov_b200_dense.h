@@ -242,12 +242,14 @@ typedef struct {
 } lt_dn_seqs;
 
 /* Rows of up to LT_DN_SEQS sequences, in token order.  q, k: element type, key head g at columns g*dp; v: head h at h*dvp; row
- * stride ld for all three.  o: fp32, row stride ldo. */
+ * stride ld for all three.  o: fp32, row stride ldo.  Numbers that are not finite reach the outputs and states of the heads that read them,
+ * from their row on. */
 int lt_dn_delta_rows(const void* q, const void* k, const void* v, int ld, const float* la, int ldla, const float* beta, int ldb, float* o,
                      int ldo, int f32, const lt_dn_delta* h_d, const lt_dn_seqs* h_q, void* stream);
 
-/* The same in chunks of 64 tokens on the tensor cores (bf16 only; dp <= 256, dvp <= 512; sums as exact as in token order).  ws: fp32
- * workspace of lt_dn_delta_chunked_ws elements. */
+/* The same in chunks of 64 tokens on the tensor cores (bf16 only; dp <= 256, dvp <= 512; sums as exact as in token order).  Numbers that are
+ * not finite reach the outputs of the heads that read them from their chunk on: up to 63 rows ahead of them too.  ws: fp32 workspace of
+ * lt_dn_delta_chunked_ws elements. */
 long lt_dn_delta_chunked_ws(const lt_dn_delta* h_d, const lt_dn_seqs* h_q);
 int lt_dn_delta_chunked(const void* q, const void* k, const void* v, int ld, const float* la, int ldla, const float* beta, int ldb, float* o,
                         int ldo, const lt_dn_delta* h_d, const lt_dn_seqs* h_q, float* ws, void* stream);
@@ -283,13 +285,15 @@ long lt_dn_experts_plan_ints(int T, int top, int n);
 int lt_dn_experts_plan(const int* ids, int T, int top, int n, int* plan, void* stream);
 
 /* H[t*top + j] = glu(gate, up) of x_t and the expert's matrix: W [n][2F][ldw], F gate rows, then F up rows.  h_epi: LT_DN_GLU.
- * Rows of H whose place is left out stay as they are.  With a plan ws holds lt_dn_experts_glu_ws(T, top, K, f32) fp32 elements. */
+ * Rows of H whose place is left out stay as they are.  With a plan the matrices have at most 2^31 - 1 rows together (bf16) and ws
+ * holds lt_dn_experts_glu_ws(T, top, K, f32) fp32 elements. */
 long lt_dn_experts_glu_ws(int T, int top, int K, int f32);
 int lt_dn_experts_glu(const void* W, int ldw, const void* X, int ldx, void* H, int ldh, int f32, int F, int K, const lt_dn_choice* h_c,
                       const lt_dn_epilogue* h_epi, void* ws, void* stream);
 
-/* Y[t] (fp32) += ls * sum_j w[t*top + j] * (W of the expert) H[t*top + j]; W [n][M][ldw]; ls [M] or NULL (1).  With a plan ws holds
- * lt_dn_experts_sum_ws(T, top, M, K, f32) fp32 elements. */
+/* Y[t] (fp32) += ls * sum_j w[t*top + j] * (W of the expert) H[t*top + j]; W [n][M][ldw]; ls [M] or NULL (1).  Without a plan T is at most
+ * 65535; with one the matrices have at most 2^31 - 1 rows together (bf16) and ws holds lt_dn_experts_sum_ws(T, top, M, K, f32) fp32
+ * elements. */
 long lt_dn_experts_sum_ws(int T, int top, int M, int K, int f32);
 int lt_dn_experts_sum(const void* W, int ldw, const void* H, int ldh, float* Y, int ldy, int f32, int M, int K, const lt_dn_choice* h_c,
                       const float* w, const float* ls, float* ws, void* stream);

@@ -13,7 +13,7 @@
 // the blocks' numbers.  Four warps make those numbers for the next batch, a warp per block, from rows that bulk copies have brought a
 // batch earlier.  What bounds it is how many instructions a block is for one warp (four to five clocks each, as its scheduler has
 // little else): products are of pairs (fma.rn.f32x2), and of S q^ a lane gets the one sum that it stores.
-// (14 heads of 64 in fp32, 300 rows: 94 us token by token, staged without overlap; 47 in blocks with two columns a lane; 33 now.)
+// (14 heads of 64 in fp32, 300 rows: 94 us token by token, staged without overlap; 47 in blocks with two columns a lane; 34 now.)
 // k_delta_step is one token with its convolution and step size.
 #include "lt_dn_delta.cuh"
 #include "lt_tc.cuh"

@@ -16,11 +16,12 @@
 //
 // What is bf16 in memory (q, k, v) enters exactly.  Everything else is fp32: it enters as the sum of three bf16 (24 significant
 // bits), three products against bf16 and six against another such sum, so that chunks are as exact as token order.  The
-// products of the leading parts have accumulators of their own: the tensor cores cut sums off instead of rounding them, which costs
-// up to 2^-24 of the accumulator at every step.
+// tensor cores cut sums off instead of rounding them, which costs up to 2^-23 of the accumulator at every step.  So the products of the
+// leading parts have accumulators of their own in U0, in the update of the state and in the outputs; in W and W S^T all parts share one,
+// the smallest first, as there the leading ones are four steps and at most two.
 //
-// A row that is not finite (infinities, NaN) makes the outputs of its whole chunk not finite, earlier tokens' among them: products
-// over a chunk have zeros where token order has nothing.  Other sequences and earlier chunks are as they would be.
+// A row that is not finite (infinities, NaN) makes the outputs of its heads not finite over its whole chunk, earlier tokens' among them: products
+// over a chunk have zeros where token order has nothing.  Other heads, other sequences and earlier chunks are as they would be.
 //
 // The walk over the chunks is the longest of the three, and bound by the instructions and waits of a chunk's dependent chain.  So W, U0
 // and the keys lie in memory as the lanes hold them (16 bytes a lane, side by side) and go straight into registers, asked for when
@@ -80,7 +81,8 @@ __device__ __forceinline__ Chunk chunk_of(const DeltaChunkP& P, int c) {
     return r;
 }
 
-// sums of a chunk's log decays (base 2), by one warp: doubles, so that differences are exact
+// sums of a chunk's log decays (base 2), by one warp: doubles, so that a difference of two sums is as near as its own terms, which are
+// fp32 products (2^-24 of each, and 2^-26 of the constant)
 __device__ __forceinline__ void log_sums(const DeltaChunkP& P, const Chunk& c, int h, int lane, double* sb) {
     const int t = 2 * lane;
     const double l0 = t < c.rows ? (double)(delta_log(P.la[(c.row0 + t) * P.ldla + h]) * DLOG2E) : 0.0;

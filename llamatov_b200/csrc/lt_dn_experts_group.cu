@@ -10,9 +10,12 @@
 //   warp 16 : producer, TMA
 //   warp 17 : MMAs (a warp's loop with one thread picked at the instructions: 2 % less than that thread's own loop)
 //   warps 0-15 : epilogue, a thread per weight row and a quarter of the places
-// What bounds it is the matrices' bytes with what shares the way: of 143 us (gate|up, 537 MB in 607 MB of reads) the copies of W alone take
-// 109, 5.6 TB/s; the sums' fp32 outputs are 23 us of 92.  (Two SMs on a tile, cta_group::2 with M = 256, halve X's bytes: 137 and 92 us for as
+// What bounds it is the matrices' bytes with what shares the way: of 141 us (gate|up, 537 MB in 620 MB of reads) the copies of W alone take
+// 109, 5.6 TB/s; the sums' fp32 outputs are 23 us of 91.  (Two SMs on a tile, cta_group::2 with M = 256, halve X's bytes: 137 and 92 us for as
 // much code again.  An L2 prefetch four stages ahead: 4 % more; one accumulator of the sums kept in registers over its release: nothing.)
+// All of K adds up in one accumulator, and the tensor cores cut sums off toward zero instead of rounding them: over K = 2048 a product is
+// 2e-6 of its size from 64 bits (fp32 matrix products of the plain form 4e-7), 1.8e-6 of it one-sided.  Of gated outputs 0.2 % round to the
+// next bf16 for it; their distance from 64 bits, 1.7e-3, is that of the rounding with or without.
 // fp32 (k_group_f32): register-blocked tiles on the CUDA cores.
 #include "lt_dn_experts.cuh"
 #include "lt_tc.cuh"
@@ -377,6 +380,12 @@ static int launch_group_tc(GroupP P, void* rows, cudaStream_t s) {
     k_group_tc<NT, GLU><<<sm_count(), C::THREADS, C::SMEM, s>>>(tmW, tmX, P);
     return check_launch("experts' products");
 }
+// By the mean share, though shares differ: a larger expert has more than one tile.  The fewer columns, the deeper the ring (5, 4 and 3 stages)
+// and, up to 128, two sets of accumulators; the more, the fewer times a matrix is read from L2.  (us of the product alone with 64 / 128 /
+// 256 columns at so many places an expert.  64 experts of 2 x 1024 x 2048: 16 85.6 / 87.5 / 89.3, 24 85.7 / 88.8 / 91.1, 32 86.9 / 89.4 / 92.7,
+// 48 91.8 / 90.4 / 93.8, 64 98.1 / 92.2 / 95.8, 80 102.9 / 96.5 / 96.3, 128 122 / 109 / 103, 250 197 / 149 / 139; of 2048 x 1024: 24 47.2 / 48.3 /
+// 49.4, 32 48.6 / 50.8 / 52.3, 48 51.1 / 50.4 / 53.3, 64 56.4 / 53.0 / 55.9, 80 61.3 / 59.3 / 57.2, 250 113 / 94.0 / 90.8; 128 experts of 1024 x 512:
+// 24 27.1 / 27.3 / 29.1, 32 29.5 / 28.6 / 30.2, 64 35.7 / 33.1 / 34.0, 96 41.3 / 37.1 / 37.2, 250 73.4 / 61.5 / 62.2.)
 template <bool GLU>
 static int pick_group_tc(const GroupP& P, void* rows, cudaStream_t s) {
     const long each = (long)P.c.T * P.c.top / P.c.n;        // places of an expert

@@ -248,9 +248,11 @@ class Experts:
 
 def delta_chunked_from(ctas):
     """Tokens of the longest sequence from which on bf16 rows are walked in chunks, and not in token order, which takes no
-    preparation but more per token, the more CTAs (of 16 value columns) share an SM.  (us in token order / in chunks: 16 heads of 128,
-    128 CTAs: 256 tokens 37 / 39, 512 68 / 46; 32 heads: 128 tokens 32 / 38, 256 56 / 44; four sequences of 16 heads: 64 tokens 34 / 38,
-    128 57 / 45.)"""
+    preparation but more per token, the more CTAs (of 16 value columns) share one of the 148 SMs.  (us in token order / in chunks: 16 heads of
+    128, 128 CTAs: 256 tokens 35 / 37, 384 51 / 41; 32 heads: 128 tokens 29 / 36, 176 38 / 39, 256 54 / 42; four sequences of 16 heads: 64 tokens
+    31 / 36, 96 43 / 43, 128 55 / 43.  The limits are those of heads of 128; smaller ones meet later, larger ones sooner: 28 heads of 64 256 tokens 28 / 29,
+    64 of them 176 tokens 29 / 34 and 256 40 / 36, four sequences of 28 96 tokens 31 / 37 and 128 40 / 37; 8 heads of 256 176 tokens 53 / 53, 16 of
+    them 96 tokens 60 / 57 and 176 105 / 62.)"""
     return DELTA_CHUNKED_FROM if DELTA_CHUNKED_FROM is not None else 256 if ctas <= 148 else 176 if ctas <= 296 else 96
 
 
