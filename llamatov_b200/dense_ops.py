@@ -319,6 +319,7 @@ class DeltaRule:
                 done += portion
                 ws = torch.empty(_lib.dense().lt_dn_delta_chunked_ws(self._ref, ctypes.byref(seqs)), dtype=torch.float32, device="cuda")
                 _lib.call("lt_dn_delta_chunked", *args, self._ref, ctypes.byref(seqs), ws.data_ptr(), stream)
+                del ws           # ahead of the next portion's, which takes its place
 
     def step(self, row, dt, beta, ring, S, o, len_, ticket):
         _lib.call("lt_dn_delta_step", row, dt, beta, ring, S, o, self.f32, len_, ticket, self._ref, _stream(self.home))

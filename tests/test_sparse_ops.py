@@ -153,6 +153,26 @@ def test_workspace_of_a_chunked_walk_is_bounded(monkeypatch, lengths, H, d, dv):
         assert sum(rows for _, rows in parts) == n
 
 
+def test_portions_have_one_workspace_at_a_time(monkeypatch):
+    import weakref
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda d: 0, raising=False)
+    monkeypatch.setattr(P, "DELTA_CHUNKED_FROM", 1)
+    monkeypatch.setattr(P, "DELTA_PORTION", 64)
+    rule = P.DeltaRule(2, 2, 16, 16, torch.bfloat16, 1.0, 1e-6)
+    made, zeros = [], torch.zeros
+
+    def empty(n, **kw):
+        assert all(r() is None for r in made)
+        t = zeros(4)
+        made.append(weakref.ref(t))
+        return t
+    monkeypatch.setattr(torch, "empty", empty)
+    monkeypatch.setattr(_lib, "call", lambda *a: None)
+    rule.rows(256, 256, 256, 96, 256, 256, 2, 256, 32, [4096 * (i + 1) for i in range(9)], [300] * 9)
+    assert len(made) == 10
+
+
 def test_no_rows_is_no_launch():
     n = _lib.launch_count()
     assert _lib.dense().lt_dn_delta_rows(one, one, one, 96, one, 4, one, 4, one, 96, 0, delta(), seqs((0, 0, 256), (7, 0, 512)), None) == 0
